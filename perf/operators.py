@@ -40,7 +40,7 @@ def listed():
         {"name": "distill_loss_small", "op": "distill_loss", "dtype": "fp32", "n": 16, "vocab": 10_007, "k": 20, "tau": 2.0, "lse": False, "pad": 0},
         # forward only over a large batch, lists of 100
         {"name": "distill_loss_batch", "op": "distill_loss", "dtype": "bf16", "n": 2048, "vocab": 100_000, "k": 100, "tau": 1.0, "lse": True, "pad": 0},
-        # a training step that keeps the log-sums between forward and backward, MovieLens catalogue, lists of 200
+        # a training step that keeps the rows' statistics between forward and backward, MovieLens catalogue, lists of 200
         {"name": "distill_step", "op": "distill_step", "dtype": "fp32", "n": 1024, "vocab": 84_432, "k": 200, "tau": 2.0, "lse": False, "pad": 0},
         # the same step in one call: loss and gradient from one reading of the scores
         {"name": "distill_loss_grad", "op": "distill_loss_grad", "dtype": "bf16", "n": 4096, "vocab": 100_000, "k": 100, "tau": 1.0, "lse": False, "pad": 0},
@@ -193,8 +193,8 @@ def _run_own(s):
     if s["op"] == "distill_loss":
         return dense.distill_loss(s["student"], *lists, temperature=s["tau"], teacher_lse=s["lse"])
     if s["op"] == "distill_step":
-        loss, lse = dense.distill_loss(s["student"], *lists, temperature=s["tau"], teacher_lse=s["lse"], return_lse=True)
-        return loss, dense.distill_grad(s["student"], lse, *lists, grad_loss=s["grad_loss"], temperature=s["tau"], teacher_lse=s["lse"])
+        loss, stats = dense.distill_loss(s["student"], *lists, temperature=s["tau"], teacher_lse=s["lse"], return_stats=True)
+        return loss, dense.distill_grad(s["student"], stats, *lists, grad_loss=s["grad_loss"], temperature=s["tau"], teacher_lse=s["lse"])
     return dense.distill_loss_grad(s["student"], *lists, grad_loss=s["grad_loss"], temperature=s["tau"], teacher_lse=s["lse"])
 
 
