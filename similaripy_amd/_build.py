@@ -9,6 +9,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -17,8 +18,14 @@ CSRC_DIR = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "lib"
 LIB_PATH = LIB_DIR / "libsimilaripy_hip.so"
 
-SOURCES = [CSRC_DIR / "sp_knn.hip"]
-HEADERS = [REPO_DIR / "include" / "sp_knn.h", REPO_DIR / "include" / "sp_prep.h", *sorted(CSRC_DIR.glob("*.hpp")), *sorted(CSRC_DIR.glob("*.inc"))]
+INCLUDE_DIR = REPO_DIR / "include"
+# every translation unit with the files it reads: each is compiled to an object of its own, all at once, and linked into the one library
+UNITS = {
+    CSRC_DIR / "sp_knn.hip": [INCLUDE_DIR / "sp_knn.h", INCLUDE_DIR / "sp_prep.h",
+                              *sorted(CSRC_DIR.glob("*.hpp")), *sorted(CSRC_DIR.glob("*.inc"))],
+}
+SOURCES = list(UNITS)
+HEADERS = sorted({h for hs in UNITS.values() for h in hs})
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
@@ -28,8 +35,9 @@ HIPCC_FLAGS = [
     # one lane's returning atomic on the row queue must stay PENDING until its value is used a row later: the atomic optimizer
     # rewrites it into a wave-aggregated form whose lanes need the result at once (s_waitcnt vmcnt(0) right behind the atomic)
     "-mllvm", "-amdgpu-atomic-optimizer-strategy=None",
+    # no packed float32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this hardware
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-fPIC",
-    "-shared",
     "-Wno-unused-function",
 ]
 
@@ -48,15 +56,16 @@ def is_stale() -> bool:
     return any(p.exists() and p.stat().st_mtime > t for p in SOURCES + HEADERS)
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the HIP library if missing or older than its sources. Returns its path."""
-    srcs = [s for s in SOURCES if s.exists()]
-    if not force and not is_stale():
-        return LIB_PATH
-    LIB_DIR.mkdir(parents=True, exist_ok=True)
-    tmp = LIB_PATH.with_suffix(".so.tmp%d" % os.getpid())
+def _object(src: Path) -> Path:
+    return LIB_DIR / (src.stem + ".o")
+
+
+def _compile(src: Path, verbose: bool) -> None:
+    """One translation unit -> its object next to the library (written aside, then moved into place)."""
+    obj = _object(src)
+    tmp = obj.with_suffix(".o.tmp%d" % os.getpid())
     extra = os.environ.get("SIMILARIPY_AMD_HIPCC_EXTRA", "").split()      # profiling builds only, e.g. -DSP_ABLATION=1
-    cmd = [find_hipcc(), *HIPCC_FLAGS, *extra, "-I", str(REPO_DIR / "include"), "-o", str(tmp), *map(str, srcs)]
+    cmd = [find_hipcc(), *HIPCC_FLAGS, *extra, "-I", str(INCLUDE_DIR), "-c", "-o", str(tmp), str(src)]
     if verbose:
         print(" ".join(cmd))
     proc = subprocess.run(cmd, capture_output=True, text=True)
@@ -67,6 +76,27 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError("hipcc failed:\n" + proc.stdout + proc.stderr)
+    os.replace(tmp, obj)
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the HIP library if missing or older than its sources (the units that changed; all of them with `force`). Returns its path."""
+    if not force and not is_stale():
+        return LIB_PATH
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+
+    def stale(src):
+        obj = _object(src)
+        return force or not obj.exists() or any(p.exists() and p.stat().st_mtime > obj.stat().st_mtime for p in [src, *UNITS[src]])
+    todo = [s for s in SOURCES if stale(s)]
+    with ThreadPoolExecutor(max_workers=max(1, len(todo))) as pool:
+        for done in [pool.submit(_compile, s, verbose) for s in todo]:
+            done.result()
+    tmp = LIB_PATH.with_suffix(".so.tmp%d" % os.getpid())
+    cmd = [find_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", str(tmp), *(str(_object(s)) for s in SOURCES)]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError("hipcc failed to link:\n" + proc.stdout + proc.stderr)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 
