@@ -1,4 +1,4 @@
-"""ctypes binding of include/sp_knn.h and include/sp_prep.h (libsimilaripy_hip.so).
+"""ctypes binding of include/sp_knn.h, include/sp_prep.h and include/sp_dense.h (libsimilaripy_hip.so).
 
 This is the only way the Python layer reaches compute.  There is no CPU fallback:
 if the library is missing, cannot be loaded, or sees no HIP device, the call raises.
@@ -232,6 +232,130 @@ EXPORTED_SYMBOLS = (
     "sp_knn_partition",
 )
 
+# ---- include/sp_dense.h ----
+SP_DT_F32, SP_DT_BF16, SP_DT_F16 = range(3)
+SP_DISTILL_KMAX = 4096
+
+
+class SpEmbedArgs(C.Structure):
+    """Mirror of ``struct sp_embed_args`` (include/sp_dense.h) — keep field order identical."""
+
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("flags", C.c_uint32),
+        ("device", C.c_int32),
+        ("dtype", C.c_int32),
+        ("out_dtype", C.c_int32),
+        ("index64", C.c_int32),
+        ("accumulate", C.c_int32),
+        ("scale", C.c_float),
+        ("n_rows", C.c_int64),
+        ("n_vocab", C.c_int64),
+        ("dim", C.c_int64),
+        ("nnz", C.c_int64),
+        ("ld_src", C.c_int64),
+        ("ld_out", C.c_int64),
+        ("src", C.c_void_p),
+        ("indices", C.c_void_p),
+        ("indptr", C.c_void_p),
+        ("data", C.c_void_p),
+        ("out", C.c_void_p),
+        ("stream", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+    ]
+
+
+class SpCsrPattern(C.Structure):
+    """Mirror of ``struct sp_csr_pattern`` (include/sp_dense.h) — keep field order identical."""
+
+    _fields_ = [
+        ("indptr", C.c_void_p),
+        ("indices", C.c_void_p),
+        ("n_rows", C.c_int64),
+        ("nnz", C.c_int64),
+        ("index64", C.c_int32),
+        ("_pad0", C.c_int32),
+    ]
+
+
+class SpAdjustArgs(C.Structure):
+    """Mirror of ``struct sp_adjust_args`` (include/sp_dense.h) — keep field order identical."""
+
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("flags", C.c_uint32),
+        ("device", C.c_int32),
+        ("dtype", C.c_int32),
+        ("n_rows", C.c_int64),
+        ("n_cols", C.c_int64),
+        ("ld_scores", C.c_int64),
+        ("ld_out", C.c_int64),
+        ("scores", C.c_void_p),
+        ("out", C.c_void_p),
+        ("targets", C.c_void_p),
+        ("targets64", C.c_int32),
+        ("bias_dtype", C.c_int32),
+        ("history", SpCsrPattern),
+        ("filter", SpCsrPattern),
+        ("target", SpCsrPattern),
+        ("repetition", C.c_void_p),
+        ("presence", C.c_void_p),
+        ("frequency", C.c_void_p),
+        ("repetition_all", C.c_float),
+        ("presence_all", C.c_float),
+        ("frequency_all", C.c_float),
+        ("_pad0", C.c_int32),
+        ("bias", C.c_void_p),
+        ("ld_bias", C.c_int64),
+        ("allowed", C.c_void_p),
+        ("ld_allowed", C.c_int64),
+        ("stream", C.c_void_p),
+    ]
+
+
+class SpDistillArgs(C.Structure):
+    """Mirror of ``struct sp_distill_args`` (include/sp_dense.h) — keep field order identical."""
+
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("flags", C.c_uint32),
+        ("device", C.c_int32),
+        ("dtype", C.c_int32),
+        ("n_rows", C.c_int64),
+        ("n_cols", C.c_int64),
+        ("ld_student", C.c_int64),
+        ("ld_grad", C.c_int64),
+        ("k", C.c_int32),
+        ("cols64", C.c_int32),
+        ("values_dtype", C.c_int32),
+        ("temperature", C.c_float),
+        ("student", C.c_void_p),
+        ("cols", C.c_void_p),
+        ("values", C.c_void_p),
+        ("counts", C.c_void_p),
+        ("teacher_lse", C.c_void_p),
+        ("loss", C.c_void_p),
+        ("stats", C.c_void_p),
+        ("grad_loss", C.c_void_p),
+        ("grad", C.c_void_p),
+        ("stream", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+    ]
+
+
+DENSE_SYMBOLS = (
+    "sp_embed_rows",
+    "sp_embed_rows_grad",
+    "sp_embed_rows_grad_workspace_bytes",
+    "sp_adjust_scores",
+    "sp_distill_loss",
+    "sp_distill_grad",
+    "sp_distill_loss_grad",
+    "sp_distill_workspace_bytes",
+)
+
 
 class HipLibraryError(RuntimeError):
     pass
@@ -319,6 +443,10 @@ def load(build_if_missing: bool = True):
     lib.sp_knn_target_costs.restype = C.c_int
     lib.sp_knn_partition.argtypes = [C.POINTER(SpKnnArgs), C.c_int, C.c_void_p]
     lib.sp_knn_partition.restype = C.c_int
+    for sym in DENSE_SYMBOLS:
+        args = SpEmbedArgs if sym.startswith("sp_embed") else SpAdjustArgs if sym.startswith("sp_adjust") else SpDistillArgs
+        getattr(lib, sym).argtypes = [C.POINTER(args)]
+        getattr(lib, sym).restype = C.c_int64 if sym.endswith("_bytes") else C.c_int
     _lib = lib
     return lib
 
@@ -401,6 +529,15 @@ def call_col_sums(args: SpCsrColsumsArgs) -> None:
     rc = lib.sp_csr_col_sums_f32(C.byref(args))
     if rc != 0:
         raise HipLibraryError(f"sp_csr_col_sums_f32 failed ({rc}): {last_error()}")
+
+
+def call_dense(symbol: str, args) -> int:
+    """One entry of include/sp_dense.h: 0, or the bytes a workspace query answers."""
+    args.struct_size = C.sizeof(args)
+    rc = getattr(load(), symbol)(C.byref(args))
+    if rc < 0:
+        raise HipLibraryError(f"{symbol} failed ({rc}): {last_error()}")
+    return rc
 
 
 def _cost_args(call):

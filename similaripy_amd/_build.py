@@ -19,10 +19,13 @@ LIB_DIR = PKG_DIR / "lib"
 LIB_PATH = LIB_DIR / "libsimilaripy_hip.so"
 
 INCLUDE_DIR = REPO_DIR / "include"
+# the kernels of the dense operators and what they include
+DENSE_HEADERS = [CSRC_DIR / n for n in ("sp_dense_common.hpp", "sp_embed_kernels.hpp", "sp_adjust_kernel.hpp", "sp_distill_kernels.hpp")]
 # every translation unit with the files it reads: each is compiled to an object of its own, all at once, and linked into the one library
 UNITS = {
     CSRC_DIR / "sp_knn.hip": [INCLUDE_DIR / "sp_knn.h", INCLUDE_DIR / "sp_prep.h",
-                              *sorted(CSRC_DIR.glob("*.hpp")), *sorted(CSRC_DIR.glob("*.inc"))],
+                              *sorted(p for p in CSRC_DIR.glob("*.hpp") if p not in DENSE_HEADERS), *sorted(CSRC_DIR.glob("*.inc"))],
+    CSRC_DIR / "sp_dense.hip": [INCLUDE_DIR / "sp_knn.h", INCLUDE_DIR / "sp_dense.h", *DENSE_HEADERS],
 }
 SOURCES = list(UNITS)
 HEADERS = sorted({h for hs in UNITS.values() for h in hs})

@@ -1,0 +1,422 @@
+// sp_dense.hip — the operators on dense tensors (include/sp_dense.h): argument checks, launch shapes, C ABI.
+//
+// Everything here is device mode: pointers on `device`, launches on the caller's stream, scratch from the caller's workspace, no
+// allocation, no synchronisation and no memset (a fill kernel where memory has to be cleared), so that every call can be captured.
+#include <hip/hip_runtime.h>
+#include <stdarg.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <type_traits>
+
+#include "../../include/sp_dense.h"
+#include "../../include/sp_knn.h"
+#include "sp_adjust_kernel.hpp"
+#include "sp_dense_common.hpp"
+#include "sp_distill_kernels.hpp"
+#include "sp_embed_kernels.hpp"
+
+__attribute__((visibility("hidden"))) int sp_set_error(int code, const char *text);      // sp_knn.hip
+
+namespace {
+
+int fail(int code, const char *fmt, ...) {
+    char text[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(text, sizeof(text), fmt, ap);
+    va_end(ap);
+    return sp_set_error(code, text);
+}
+
+#define TRY(expr) do { int _rc = (expr); if (_rc) return _rc; } while (0)
+#define HIP_TRY(expr)                                                                              \
+    do {                                                                                           \
+        hipError_t _e = (expr);                                                                    \
+        if (_e != hipSuccess)                                                                      \
+            return fail(SP_EHIP, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(_e), __FILE__, __LINE__); \
+    } while (0)
+
+// the call's device while it launches; the thread's own afterwards
+struct OnDevice {
+    int before = -1;
+    bool moved = false;
+    int enter(int device) {
+        const hipError_t e = hipGetDevice(&before);
+        if (e != hipSuccess) { (void)hipGetLastError(); return fail(SP_ENODEVICE, "no HIP device visible: similaripy_amd has no CPU fallback"); }
+        if (device == before) return SP_OK;
+        int n = 0;
+        HIP_TRY(hipGetDeviceCount(&n));
+        if (device < 0 || device >= n) return fail(SP_EINVAL, "device %d out of range (have %d)", device, n);
+        HIP_TRY(hipSetDevice(device));
+        moved = true;
+        return SP_OK;
+    }
+    ~OnDevice() { if (moved) (void)hipSetDevice(before); }
+};
+
+i64 ceil_div(i64 a, i64 b) { return (a + b - 1) / b; }
+constexpr i64 I32_MAX = 0x7FFFFFFFLL;
+bool bad_dtype(int d) { return d < SP_DT_F32 || d > SP_DT_F16; }
+
+// calls f with a value of the element type
+template <typename F> int with_type(int dtype, F f) {
+    if (dtype == SP_DT_F32) return f(float());
+    if (dtype == SP_DT_BF16) return f((__bf16)0.f);
+    return f((_Float16)0.f);
+}
+
+// ---- embedding rows ------------------------------------------------------------------------------------------------------------
+
+int check_embed(const sp_embed_args *a) {
+    if (!a || a->struct_size != sizeof(sp_embed_args)) return fail(SP_EINVAL, "sp_embed_args size mismatch");
+    if (a->flags) return fail(SP_EINVAL, "flags must be 0");
+    if (bad_dtype(a->dtype) || bad_dtype(a->out_dtype)) return fail(SP_EINVAL, "bad dtype");
+    if (a->n_rows < 0 || a->n_rows > I32_MAX || a->n_vocab < 0 || a->n_vocab >= I32_MAX || a->dim < 0 || a->dim > I32_MAX / 2 || a->nnz < 0 || a->nnz > I32_MAX)
+        return fail(SP_EINVAL, "bad shape / nnz");
+    if (!a->indptr && a->nnz != a->n_rows) return fail(SP_EINVAL, "without indptr nnz must equal n_rows");
+    if (a->nnz > 0 && !a->indices) return fail(SP_EINVAL, "NULL indices");
+    return SP_OK;
+}
+
+// lanes of a group: the fewest that cover a row with N elements each, 8 .. 64; columns beyond 64 lanes make further slabs
+int group_of(i64 dim, int n) {
+    const i64 lanes = ceil_div(dim, n);
+    int g = 8;
+    while (g < 64 && g < lanes) g *= 2;
+    return g;
+}
+template <typename F> int with_group(int g, F f) {
+    switch (g) {
+    case 8: return f(std::integral_constant<int, 8>());
+    case 16: return f(std::integral_constant<int, 16>());
+    case 32: return f(std::integral_constant<int, 32>());
+    default: return f(std::integral_constant<int, 64>());
+    }
+}
+
+EmbedParams embed_params(const sp_embed_args *a) {
+    EmbedParams p{};
+    p.in = a->src; p.indices = a->indices; p.indptr = a->indptr; p.data = a->data; p.out = a->out;
+    p.n_rows = a->n_rows; p.n_vocab = a->n_vocab; p.nnz = a->nnz; p.ld_in = a->ld_src; p.ld_out = a->ld_out;
+    p.dim = (int)a->dim; p.index64 = a->index64; p.accumulate = a->accumulate; p.scale = a->scale;
+    return p;
+}
+
+int run_embed(const sp_embed_args *a) {
+    hipStream_t stream = (hipStream_t)a->stream;
+    return with_type(a->dtype, [&](auto tag) {
+        using T = decltype(tag);
+        constexpr int N = VecOf<T>::N;
+        return with_group(group_of(a->dim, N), [&](auto gc) {
+            constexpr int G = decltype(gc)::value;
+            EmbedParams p = embed_params(a);
+            p.slabs = (int)ceil_div(a->dim, G * N);
+            const i64 blocks = ceil_div(a->n_rows * p.slabs, 256 / G);
+            if (blocks > I32_MAX) return fail(SP_EINVAL, "too many rows for one launch");
+            if (a->index64) hipLaunchKernelGGL((sp_embed_rows_kernel<T, i64, G>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+            else hipLaunchKernelGGL((sp_embed_rows_kernel<T, int, G>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+            HIP_TRY(hipGetLastError());
+            return (int)SP_OK;
+        });
+    });
+}
+
+// workspace of the gradient: two copies of the sorted entries (the passes alternate), the digit counts, the partial sums
+struct GradLayout {
+    int wgs, sort_chunk, passes, bits, chunk;
+    i64 chunks;
+    size_t key[2], pay[2], w[2], hist, part, total;
+};
+GradLayout grad_layout(const sp_embed_args *a) {
+    GradLayout L{};
+    const i64 n = a->nnz;
+    L.sort_chunk = (int)(ceil_div(ceil_div(n, SORT_WGS), SORT_NT) * SORT_NT);
+    if (L.sort_chunk < 1024) L.sort_chunk = 1024;
+    L.wgs = (int)ceil_div(n, L.sort_chunk);
+    int kb = 1;                                                  // bits of the keys 0 .. n_vocab
+    while (kb < 31 && (1ll << kb) <= a->n_vocab) ++kb;
+    L.passes = (kb + 8) / 9;
+    L.bits = (kb + L.passes - 1) / L.passes;
+    L.chunk = (int)ceil_div(n, 8192);
+    L.chunk = L.chunk < 16 ? 16 : L.chunk > 1024 ? 1024 : L.chunk;
+    L.chunks = ceil_div(n, L.chunk);
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) & ~(size_t)255; return o; };
+    for (int i = 0; i < 2; ++i) {
+        L.key[i] = take((size_t)n * 4);
+        L.pay[i] = take((size_t)n * 4);
+        L.w[i] = a->data ? take((size_t)n * 4) : 0;
+    }
+    L.hist = take((size_t)L.wgs * SORT_BINS * 4);
+    L.part = take((size_t)L.chunks * 2 * (size_t)a->dim * 4);
+    L.total = at;
+    return L;
+}
+
+template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a) {
+    hipStream_t stream = (hipStream_t)a->stream;
+    constexpr int N = VecOf<T>::N;
+    if (!a->accumulate) {
+        const i64 blocks = ceil_div(a->n_vocab * a->dim, 256 * VecOf<TO>::N);
+        hipLaunchKernelGGL((sp_fill_rows_kernel<TO>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream, (TO *)a->out, a->n_vocab, a->dim, a->ld_out);
+    }
+    if (a->nnz > 0) {
+        const GradLayout L = grad_layout(a);
+        unsigned char *ws = (unsigned char *)a->workspace;
+        SortParams s{};
+        s.n = a->nnz; s.chunk = L.sort_chunk; s.wgs = L.wgs; s.bits = L.bits;
+        s.hist = (unsigned *)(ws + L.hist);
+        s.indices = a->indices; s.indptr = a->indptr; s.n_rows = a->n_rows; s.n_vocab = a->n_vocab;
+        s.w_in = a->data;
+        for (int pass = 0; pass < L.passes; ++pass) {
+            const int to = pass & 1;
+            s.shift = pass * L.bits;
+            s.key_out = (unsigned *)(ws + L.key[to]);
+            s.pay_out = (unsigned *)(ws + L.pay[to]);
+            s.w_out = a->data ? (float *)(ws + L.w[to]) : nullptr;
+            if (a->index64) {
+                hipLaunchKernelGGL((sp_sort_count_kernel<i64>), dim3(L.wgs), dim3(SORT_NT), 0, stream, s);
+                hipLaunchKernelGGL((sp_sort_move_kernel<i64>), dim3(L.wgs), dim3(SORT_NT), 0, stream, s);
+            } else {
+                hipLaunchKernelGGL((sp_sort_count_kernel<int>), dim3(L.wgs), dim3(SORT_NT), 0, stream, s);
+                hipLaunchKernelGGL((sp_sort_move_kernel<int>), dim3(L.wgs), dim3(SORT_NT), 0, stream, s);
+            }
+            s.key_in = s.key_out;
+            s.pay_in = s.pay_out;
+            s.w_in = s.w_out;
+        }
+        ReduceParams r{};
+        r.in = a->src; r.out = a->out; r.key = s.key_in; r.pay = s.pay_in; r.w = s.w_in;
+        r.part = (float *)(ws + L.part);
+        r.n = a->nnz; r.n_vocab = a->n_vocab; r.n_rows = a->n_rows; r.ld_in = a->ld_src; r.ld_out = a->ld_out;
+        r.chunks = L.chunks; r.chunk = L.chunk; r.dim = (int)a->dim; r.accumulate = a->accumulate; r.scale = a->scale;
+        TRY(with_group(group_of(a->dim, N), [&](auto gc) {
+            constexpr int G = decltype(gc)::value;
+            r.slabs = (int)ceil_div(a->dim, G * N);
+            const i64 blocks = ceil_div(L.chunks * r.slabs, 256 / G);
+            if (blocks > I32_MAX) return fail(SP_EINVAL, "too many entries for one launch");
+            hipLaunchKernelGGL((sp_embed_reduce_kernel<T, TO, G>), dim3((unsigned)blocks), dim3(256), 0, stream, r);
+            if (L.chunks > 1) hipLaunchKernelGGL((sp_embed_join_kernel<TO, N, G>), dim3((unsigned)blocks), dim3(256), 0, stream, r);
+            return (int)SP_OK;
+        }));
+    }
+    HIP_TRY(hipGetLastError());
+    return SP_OK;
+}
+
+// ---- score adjustment ------------------------------------------------------------------------------------------------------------
+
+int check_pattern(const sp_csr_pattern &m, const char *what) {
+    if (!m.indptr) return SP_OK;
+    if (m.n_rows < 0 || m.nnz < 0) return fail(SP_EINVAL, "%s: negative size", what);
+    if (m.nnz > 0 && !m.indices) return fail(SP_EINVAL, "%s: NULL indices", what);
+    return SP_OK;
+}
+CsrPattern pattern_of(const sp_csr_pattern &m) { return {m.indptr, m.indices, m.n_rows, m.nnz, m.index64}; }
+
+template <typename T, int U> int launch_adjust(AdjustParams p, bool counts, hipStream_t stream) {
+    p.tiles = (int)ceil_div(p.n_cols, AD_NT * VecOf<T>::N * U);
+    const i64 blocks = p.n_rows * p.tiles;
+    if (blocks > I32_MAX) return fail(SP_EINVAL, "too many scores for one launch");
+    if (counts) hipLaunchKernelGGL((sp_adjust_kernel<T, U, true>), dim3((unsigned)blocks), dim3(AD_NT), 0, stream, p);
+    else hipLaunchKernelGGL((sp_adjust_kernel<T, U, false>), dim3((unsigned)blocks), dim3(AD_NT), 0, stream, p);
+    HIP_TRY(hipGetLastError());
+    return SP_OK;
+}
+
+// ---- distillation ------------------------------------------------------------------------------------------------------------------
+
+enum { DISTILL_LOSS = 1, DISTILL_GRAD = 2 };
+
+int check_distill(const sp_distill_args *a, int what) {
+    if (!a || a->struct_size != sizeof(sp_distill_args)) return fail(SP_EINVAL, "sp_distill_args size mismatch");
+    if (a->flags) return fail(SP_EINVAL, "flags must be 0");
+    if (bad_dtype(a->dtype) || bad_dtype(a->values_dtype)) return fail(SP_EINVAL, "bad dtype");
+    if (a->n_rows < 0 || a->n_rows > I32_MAX || a->n_cols < 0 || a->n_cols > I32_MAX) return fail(SP_EINVAL, "bad shape");
+    if (a->k < 0 || a->k > SP_DISTILL_KMAX) return fail(SP_EINVAL, "k = %d out of range [0, %d]", a->k, SP_DISTILL_KMAX);
+    if (!(a->temperature > 0.f) || a->temperature > 1e30f || a->temperature < 1e-30f) return fail(SP_EINVAL, "temperature must be positive");
+    if (a->n_rows == 0) return SP_OK;
+    if ((a->n_cols > 0 && !a->student) || (a->k > 0 && (!a->cols || !a->values))) return fail(SP_EINVAL, "NULL pointer");
+    if (what & DISTILL_GRAD) {
+        if (a->n_cols > 0 && !a->grad) return fail(SP_EINVAL, "grad is NULL");
+        if (what == DISTILL_GRAD && !a->stats) return fail(SP_EINVAL, "stats is NULL");
+    }
+    return SP_OK;
+}
+
+constexpr int DI_NT = 512;
+
+// Workgroups of a row: few rows are cut so that about `want` workgroups run, in pieces of at least 2048 columns.
+int splits_of(const sp_distill_args *a, i64 want) {
+    if (a->n_rows <= 0) return 1;
+    i64 s = ceil_div(want, a->n_rows);
+    const i64 most = a->n_cols / 2048;
+    s = s > most ? most : s;
+    return s < 1 ? 1 : (int)s;
+}
+i64 chunk_of(const sp_distill_args *a, int splits) { return ceil_div(ceil_div(a->n_cols, splits), 64) * 64; }
+
+size_t distill_stats_bytes(const sp_distill_args *a) { return ((size_t)a->n_rows * 8 + 255) & ~(size_t)255; }
+
+DistillParams distill_params(const sp_distill_args *a) {
+    DistillParams p{};
+    p.student = a->student; p.grad = a->grad;
+    p.n_rows = a->n_rows; p.n_cols = a->n_cols; p.ld_student = a->ld_student; p.ld_grad = a->ld_grad;
+    p.k = a->k; p.cols64 = a->cols64; p.values_dtype = a->values_dtype;
+    p.tau = a->temperature; p.inv_tau = 1.f / a->temperature; p.c = (float)(1.4426950408889634074 / (double)a->temperature);
+    p.cols = a->cols; p.values = a->values; p.counts = a->counts; p.teacher_lse = a->teacher_lse;
+    p.loss = a->loss; p.stats = a->stats; p.grad_loss = a->grad_loss;
+    p.part = (float *)((unsigned char *)a->workspace + distill_stats_bytes(a));
+    return p;
+}
+
+constexpr i64 SCAN_WGS = 1024, GRAD_WGS = 2048;
+constexpr i64 FUSED_ROWS = 256;      // from as many rows on a workgroup per row fills the card
+
+int launch_scan(const sp_distill_args *a, DistillParams p, hipStream_t stream) {
+    p.splits = splits_of(a, SCAN_WGS);
+    p.chunk = chunk_of(a, p.splits);
+    return with_type(a->dtype, [&](auto tag) {
+        using T = decltype(tag);
+        hipLaunchKernelGGL((sp_distill_scan_kernel<T, DI_NT>), dim3((unsigned)(a->n_rows * p.splits)), dim3(DI_NT), 0, stream, p);
+        if (p.splits > 1) hipLaunchKernelGGL((sp_distill_join_kernel<T>), dim3((unsigned)a->n_rows), dim3(64), 0, stream, p);
+        HIP_TRY(hipGetLastError());
+        return (int)SP_OK;
+    });
+}
+int launch_grad(const sp_distill_args *a, DistillParams p, hipStream_t stream) {
+    p.splits = splits_of(a, GRAD_WGS);
+    p.chunk = chunk_of(a, p.splits);
+    return with_type(a->dtype, [&](auto tag) {
+        using T = decltype(tag);
+        hipLaunchKernelGGL((sp_distill_grad_kernel<T, DI_NT>), dim3((unsigned)(a->n_rows * p.splits)), dim3(DI_NT), (size_t)a->k * 12, stream, p);
+        HIP_TRY(hipGetLastError());
+        return (int)SP_OK;
+    });
+}
+
+i64 distill_ws_bytes(const sp_distill_args *a) {
+    return (i64)distill_stats_bytes(a) + a->n_rows * splits_of(a, SCAN_WGS) * 8;
+}
+int check_workspace(const void *ws, i64 have, i64 need) {
+    if (need > 0 && (!ws || have < need)) return fail(SP_EWORKSPACE, "workspace too small: need %lld bytes, got %lld", need, ws ? have : 0ll);
+    return SP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sp_embed_rows(const sp_embed_args *a) {
+    sp_set_error(0, "");
+    TRY(check_embed(a));
+    if (a->out_dtype != a->dtype) return fail(SP_EINVAL, "out_dtype must be the table's dtype");
+    if (a->n_rows == 0 || a->dim == 0) return SP_OK;
+    if (!a->out || (a->n_vocab > 0 && !a->src)) return fail(SP_EINVAL, "NULL table or out");
+    if (a->n_rows > 1 && a->ld_out < a->dim) return fail(SP_EINVAL, "rows of out overlap");
+    OnDevice dev;
+    TRY(dev.enter(a->device));
+    return run_embed(a);
+}
+
+int64_t sp_embed_rows_grad_workspace_bytes(const sp_embed_args *a) {
+    TRY(check_embed(a));
+    return (int64_t)grad_layout(a).total;
+}
+
+int sp_embed_rows_grad(const sp_embed_args *a) {
+    sp_set_error(0, "");
+    TRY(check_embed(a));
+    if (a->out_dtype != a->dtype && a->out_dtype != SP_DT_F32) return fail(SP_EINVAL, "out_dtype must be dtype or SP_DT_F32");
+    if (a->n_vocab == 0 || a->dim == 0) return SP_OK;
+    if (!a->out || (a->n_rows > 0 && !a->src)) return fail(SP_EINVAL, "NULL gradient or out");
+    if (a->n_vocab > 1 && a->ld_out < a->dim) return fail(SP_EINVAL, "rows of out overlap");
+    TRY(check_workspace(a->workspace, a->workspace_bytes, a->nnz > 0 ? (i64)grad_layout(a).total : 0));
+    OnDevice dev;
+    TRY(dev.enter(a->device));
+    return with_type(a->dtype, [&](auto tag) {
+        using T = decltype(tag);
+        return a->out_dtype == a->dtype ? run_embed_grad_as<T, T>(a) : run_embed_grad_as<T, float>(a);
+    });
+}
+
+int sp_adjust_scores(const sp_adjust_args *a) {
+    sp_set_error(0, "");
+    if (!a || a->struct_size != sizeof(sp_adjust_args)) return fail(SP_EINVAL, "sp_adjust_args size mismatch");
+    if (a->flags) return fail(SP_EINVAL, "flags must be 0");
+    if (bad_dtype(a->dtype) || (a->bias && bad_dtype(a->bias_dtype))) return fail(SP_EINVAL, "bad dtype");
+    if (a->n_rows < 0 || a->n_rows > I32_MAX || a->n_cols < 0 || a->n_cols > I32_MAX) return fail(SP_EINVAL, "bad shape");
+    TRY(check_pattern(a->history, "history"));
+    TRY(check_pattern(a->filter, "filter"));
+    TRY(check_pattern(a->target, "target"));
+    if (a->n_rows == 0 || a->n_cols == 0) return SP_OK;
+    if (!a->scores || !a->out) return fail(SP_EINVAL, "NULL scores or out");
+    if (a->n_rows > 1 && a->ld_out < a->n_cols) return fail(SP_EINVAL, "rows of out overlap");
+    OnDevice dev;
+    TRY(dev.enter(a->device));
+    AdjustParams p{};
+    p.scores = a->scores; p.out = a->out; p.n_rows = a->n_rows; p.n_cols = a->n_cols; p.ld_scores = a->ld_scores; p.ld_out = a->ld_out;
+    p.targets = a->targets; p.targets64 = a->targets64; p.bias_dtype = a->bias_dtype;
+    p.history = pattern_of(a->history); p.filter = pattern_of(a->filter); p.target = pattern_of(a->target);
+    p.repetition = a->repetition; p.presence = a->presence; p.frequency = a->frequency;
+    p.repetition_all = a->repetition_all; p.presence_all = a->presence_all; p.frequency_all = a->frequency_all;
+    p.bias = a->bias; p.ld_bias = a->ld_bias; p.allowed = a->allowed; p.ld_allowed = a->ld_allowed;
+    // a history without any penalty changes nothing
+    const bool counts = a->history.indptr && (a->repetition || a->presence || a->frequency || a->repetition_all != 1.f || a->presence_all != 0.f || a->frequency_all != 0.f);
+    return with_type(a->dtype, [&](auto tag) {
+        using T = decltype(tag);
+        const i64 big = a->n_rows * ceil_div(a->n_cols, AD_NT * VecOf<T>::N * 4);
+        return big >= 512 ? launch_adjust<T, 4>(p, counts, (hipStream_t)a->stream) : launch_adjust<T, 1>(p, counts, (hipStream_t)a->stream);
+    });
+}
+
+int64_t sp_distill_workspace_bytes(const sp_distill_args *a) {
+    if (!a || a->struct_size != sizeof(sp_distill_args)) return fail(SP_EINVAL, "sp_distill_args size mismatch");
+    if (a->n_rows < 0 || a->n_rows > I32_MAX || a->n_cols < 0 || a->n_cols > I32_MAX) return fail(SP_EINVAL, "bad shape");
+    return (int64_t)distill_ws_bytes(a);
+}
+
+int sp_distill_loss(const sp_distill_args *a) {
+    sp_set_error(0, "");
+    TRY(check_distill(a, DISTILL_LOSS));
+    if (a->n_rows == 0) return SP_OK;
+    TRY(check_workspace(a->workspace, a->workspace_bytes, distill_ws_bytes(a)));
+    OnDevice dev;
+    TRY(dev.enter(a->device));
+    return launch_scan(a, distill_params(a), (hipStream_t)a->stream);
+}
+
+int sp_distill_grad(const sp_distill_args *a) {
+    sp_set_error(0, "");
+    TRY(check_distill(a, DISTILL_GRAD));
+    if (a->n_rows == 0 || a->n_cols == 0) return SP_OK;
+    if (a->n_rows > 1 && a->ld_grad < a->n_cols) return fail(SP_EINVAL, "rows of grad overlap");
+    OnDevice dev;
+    TRY(dev.enter(a->device));
+    return launch_grad(a, distill_params(a), (hipStream_t)a->stream);
+}
+
+int sp_distill_loss_grad(const sp_distill_args *a) {
+    sp_set_error(0, "");
+    TRY(check_distill(a, DISTILL_LOSS | DISTILL_GRAD));
+    if (a->n_rows == 0) return SP_OK;
+    if (a->n_rows > 1 && a->ld_grad < a->n_cols) return fail(SP_EINVAL, "rows of grad overlap");
+    TRY(check_workspace(a->workspace, a->workspace_bytes, distill_ws_bytes(a)));
+    OnDevice dev;
+    TRY(dev.enter(a->device));
+    hipStream_t stream = (hipStream_t)a->stream;
+    DistillParams p = distill_params(a);
+    if (a->n_rows < FUSED_ROWS) {
+        p.stats = (float *)a->workspace;
+        TRY(launch_scan(a, p, stream));
+        return launch_grad(a, p, stream);
+    }
+    return with_type(a->dtype, [&](auto tag) {
+        using T = decltype(tag);
+        hipLaunchKernelGGL((sp_distill_loss_grad_kernel<T, DI_NT>), dim3((unsigned)a->n_rows), dim3(DI_NT), (size_t)a->k * 12, stream, p);
+        HIP_TRY(hipGetLastError());
+        return (int)SP_OK;
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,330 @@
+// sp_distill_kernels.hpp — divergence of a student's dense scores from a teacher's top-k lists, and its gradient.
+//
+//   p_j = softmax of t_j / tau over the list (or exp(t_j / tau - teacher_lse)),   q = softmax of z / tau over all columns
+//   loss = tau^2 sum_j p_j (log p_j - log q[c_j]),     dz_v = g tau (P q_v - sum_{c_j = v} p_j),   P = sum_j p_j
+//
+// One reading of the row gives its maximum and the sum of exp2((z - max) c), c = log2(e) / tau, in a single pass: every thread
+// keeps a running maximum and rescales its sum when a vector raises it.  Between forward and backward a row keeps both, not their
+// log-sum-exp: one float32 of about 20 would tilt all of q by its rounding, and for scores near the type's lowest value (masks) it
+// would lose the sum altogether.  The list is one wave's work.
+#pragma once
+#include "sp_dense_common.hpp"
+
+namespace {
+
+struct DistillParams {
+    const void *student;
+    void *grad;
+    i64 n_rows, n_cols, ld_student, ld_grad;
+    int k, cols64, values_dtype;
+    float tau, inv_tau, c;             // c = log2(e) / tau
+    const void *cols, *values;
+    const int *counts;
+    const float *teacher_lse;
+    float *loss;
+    float *stats;                      // [n_rows, 2] maximum of z, sum of exp((z - maximum) / tau)
+    const float *grad_loss;
+    int splits;                        // workgroups of a row
+    i64 chunk;                         // columns of one of them (a multiple of the vector)
+    float *part;                       // [n_rows, splits, 2] maximum, sum
+};
+
+// maximum and sum of exp2((z - max) c) of some columns
+struct MaxSum {
+    float m, s;
+};
+__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c) {
+    const float m = fmaxf(a.m, b.m);
+    return {m, a.s * (a.m == m ? 1.f : exp2_fast((a.m - m) * c)) + b.s * (b.m == m ? 1.f : exp2_fast((b.m - m) * c))};
+}
+__device__ __forceinline__ MaxSum wave_join(MaxSum a, float c) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) a = join(a, MaxSum{__shfl_xor(a.m, d, 64), __shfl_xor(a.s, d, 64)}, c);
+    return a;
+}
+
+// exp2((z - m) c) is taken as exp2(z c - off) 2^-r, one fused operation per score with off = m c rounded and r = m c - off what the
+// rounding left (exact as a fused operation, the same for the whole row): scores far from 0 lose nothing.  Where m c leaves float32 (a row of the type's
+// lowest value) the scores that are not m itself are too far below it to count: a power of two in the place of c then keeps
+// z c - off exactly 0 for them that are.
+struct Exponent {
+    float c, off;
+};
+__device__ __forceinline__ bool off_fits(float m, float c) { return fabsf(m * c) <= 3.402823466e38f || m == NEG_INF; }
+__device__ __forceinline__ Exponent exponent_of(float m, float c) {
+    if (m == NEG_INF) return {c, 0.f};
+    if (off_fits(m, c)) return {c, m * c};
+    if (fabsf(m) > 3.402823466e38f) return {c, m};              // +inf, NaN: every q is NaN or 0
+    int e;
+    (void)frexpf(m, &e);
+    const float pow2 = ldexpf(1.f, 126 - e);
+    return {pow2, m * pow2};
+}
+__device__ __forceinline__ float correction_of(float m, Exponent x) { return m == NEG_INF ? 1.f : exp2_fast(-__fmaf_rn(m, x.c, -x.off)); }      // 2^-r
+// (sh: one slot per wave; the result is everybody's)
+template <int NT> __device__ __forceinline__ MaxSum block_join(MaxSum a, float c, MaxSum *sh) {
+    a = wave_join(a, c);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = sh[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) a = join(a, sh[w], c);
+    return a;
+}
+
+// a thread's running sum, relative to 2^off
+struct Running {
+    float m, off, s;
+};
+template <int N> __device__ __forceinline__ void add_vec(Running &a, const float *z, float c) {
+    float m = a.m;
+#pragma unroll
+    for (int j = 0; j < N; ++j) m = fmaxf(m, z[j]);
+    const float off = fminf(fmaxf(m * c, -3.402823466e38f), 3.402823466e38f);
+    float s = a.s * exp2_fast(a.off - off);
+#pragma unroll
+    for (int j = 0; j < N; ++j) s += exp2_fast(__fmaf_rn(z[j], c, -off));
+    a = {m, off, s};
+}
+
+// maximum and sum over columns [c0, c1) of a row, by the NT threads of the workgroup (each its share)
+template <typename T, int NT> __device__ __forceinline__ MaxSum thread_columns(const T *z, i64 c0, i64 c1, float c) {
+    constexpr int N = VecOf<T>::N, U = 4;
+    Running a{NEG_INF, NEG_INF, 0.f};
+    i64 i = c0 + (i64)threadIdx.x * N;
+    for (; i + (U - 1) * NT * N + N <= c1; i += U * NT * N) {
+        RawVec<T, N> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = vec_load<T, N>(z + i + u * NT * N);
+        float v[U * N];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[u * N + j] = up(x[u].v[j]);
+        add_vec<U * N>(a, v, c);
+    }
+    for (; i + N <= c1; i += NT * N) {
+        const RawVec<T, N> x = vec_load<T, N>(z + i);
+        float v[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = up(x.v[j]);
+        add_vec<N>(a, v, c);
+    }
+    for (int j = 0; j < N; ++j)
+        if (i + j < c1) {
+            const float v = up(z[i + j]);
+            add_vec<1>(a, &v, c);
+        }
+    // (a maximum whose m c leaves float32 has no sum here: it is nothing next to a larger one, and scan_columns sums again otherwise)
+    return {a.m, a.m == NEG_INF || !off_fits(a.m, c) ? (a.s != a.s ? a.s : 0.f) : a.s * exp2_fast(-__fmaf_rn(a.m, c, -a.off))};
+}
+
+// the same for the workgroup: the result is everybody's
+template <typename T, int NT> __device__ __forceinline__ MaxSum scan_columns(const T *z, i64 c0, i64 c1, float c, MaxSum *sh) {
+    MaxSum a = block_join<NT>(thread_columns<T, NT>(z, c0, c1, c), c, sh);
+    if (!off_fits(a.m, c)) {                                    // (uniform) summed once more, with an exponent that fits
+        const Exponent x = exponent_of(a.m, c);
+        a.s = 0.f;
+        for (i64 i = c0 + threadIdx.x; i < c1; i += NT) a.s += exp2_fast(__fmaf_rn(up(z[i]), x.c, -x.off));
+        __syncthreads();
+        a = block_join<NT>(a, c, sh);
+    }
+    return a;
+}
+
+struct ListSums {
+    float mass;       // P
+    float loss;       // sum p_j (log p_j - log q[c_j]) when asked for, else 0
+};
+// The teacher's list of a row, by the 64 lanes of one wave.  scol / sp (NULL or [k] in LDS): the columns (-1: not in the list) and
+// probabilities for the gradient.  a: the row's maximum and sum (read with LOSS only); log q is taken from score - maximum, so that the
+// type's lowest value as a mask stays finite.
+template <typename T, bool LOSS>
+__device__ __forceinline__ ListSums list_sums(const DistillParams &p, i64 row, const T *z, MaxSum a, int *scol, float *sprob) {
+    const int lane = threadIdx.x & 63;
+    int n = p.counts ? p.counts[row] : p.k;
+    n = n < 0 ? 0 : n > p.k ? p.k : n;
+    const i64 base = row * p.k;
+    const float high = a.m == NEG_INF ? 0.f : a.m, logs = LOSS ? logf(a.s) : 0.f;
+    float top = NEG_INF, shift = 0.f;
+    if (p.teacher_lse) shift = -p.teacher_lse[row];
+    else {
+        for (int j = lane; j < n; j += 64) {
+            const i64 col = load_index(p.cols, p.cols64, base + j);
+            if (col >= 0 && col < p.n_cols) top = fmaxf(top, load_scalar(p.values, p.values_dtype, base + j));
+        }
+        top = wave_max(top);
+        float sum = 0.f;
+        for (int j = lane; j < n; j += 64) {
+            const i64 col = load_index(p.cols, p.cols64, base + j);
+            if (col >= 0 && col < p.n_cols && top != NEG_INF) sum += exp2_fast((load_scalar(p.values, p.values_dtype, base + j) - top) * p.inv_tau * LOG2E);
+        }
+        sum = wave_sum(sum);
+        shift = sum > 0.f || sum != sum ? -logf(sum) : NEG_INF;       // (nothing in the list, or -inf only: all p_j are 0)
+    }
+    ListSums r{0.f, 0.f};
+    for (int j = lane; j < p.k; j += 64) {
+        float prob = 0.f;
+        int at = -1;
+        if (j < n) {
+            const i64 col = load_index(p.cols, p.cols64, base + j);
+            if (col >= 0 && col < p.n_cols) {
+                const float t = load_scalar(p.values, p.values_dtype, base + j);
+                const float logp = p.teacher_lse ? __fmaf_rn(t, p.inv_tau, shift) : top == NEG_INF ? NEG_INF : __fmaf_rn(t - top, p.inv_tau, shift);
+                prob = exp2_fast(logp * LOG2E);
+                at = (int)col;
+                r.mass += prob;
+                if (LOSS && prob != 0.f) {
+                    const float zc = up(z[col]);
+                    r.loss += prob * (logp - (zc == NEG_INF ? NEG_INF : __fmaf_rn(zc - high, p.inv_tau, -logs)));
+                }
+            }
+        }
+        if (scol) {
+            scol[j] = at;
+            sprob[j] = prob;
+        }
+    }
+    r.mass = wave_sum(r.mass);
+    if (LOSS) r.loss = wave_sum(r.loss);
+    return r;
+}
+
+template <typename T> __device__ __forceinline__ void finish_loss(const DistillParams &p, i64 row, MaxSum a) {
+    if (p.loss) {
+        const ListSums l = list_sums<T, true>(p, row, (const T *)p.student + row * p.ld_student, a, nullptr, nullptr);
+        if ((threadIdx.x & 63) == 0) p.loss[row] = p.tau * p.tau * l.loss;
+    }
+    if (p.stats && (threadIdx.x & 63) == 0) {
+        p.stats[2 * row] = a.m;
+        p.stats[2 * row + 1] = a.s;
+    }
+}
+
+// one workgroup per row and split; a row in one piece is finished here
+template <typename T, int NT> __global__ __launch_bounds__(NT) void sp_distill_scan_kernel(DistillParams p) {
+    __shared__ MaxSum sh[NT / 64];
+    const i64 row = blockIdx.x / p.splits, c0 = (blockIdx.x % p.splits) * p.chunk, c1 = min(p.n_cols, c0 + p.chunk);
+    const T *z = (const T *)p.student + row * p.ld_student;
+    const MaxSum a = scan_columns<T, NT>(z, c0, c1, p.c, sh);
+    if (p.splits == 1) {
+        if (threadIdx.x < 64) finish_loss<T>(p, row, a);
+    } else if (threadIdx.x == 0) {
+        p.part[2 * blockIdx.x] = a.m;
+        p.part[2 * blockIdx.x + 1] = a.s;
+    }
+}
+
+__device__ __forceinline__ MaxSum join_parts(const DistillParams &p, i64 row) {
+    MaxSum a{NEG_INF, 0.f};
+    for (int i = threadIdx.x & 63; i < p.splits; i += 64) a = join(a, MaxSum{p.part[2 * (row * p.splits + i)], p.part[2 * (row * p.splits + i) + 1]}, p.c);
+    return wave_join(a, p.c);
+}
+
+// rows in several pieces: one wave joins them
+template <typename T> __global__ __launch_bounds__(64) void sp_distill_join_kernel(DistillParams p) { finish_loss<T>(p, blockIdx.x, join_parts(p, blockIdx.x)); }
+
+// The gradient of columns [c0, c1) of a row by the NT threads of a workgroup: g tau P q everywhere, then the listed columns once
+// more with their probabilities taken off.  scol / sprob hold the list; sz [k] is scratch: the listed scores are kept before
+// anything is written, so `grad` may be `student`.  A column listed several times is written by its first entry.  A row whose list
+// has no mass gets zeros, whatever its scores hold (a padded row of a batch).
+template <typename T, int NT>
+__device__ __forceinline__ void grad_columns(const DistillParams &p, i64 row, i64 c0, i64 c1, MaxSum a, float mass, float gt, const int *scol, const float *sprob, float *sz) {
+    constexpr int N = VecOf<T>::N, U = 4;
+    const int tid = threadIdx.x;
+    const T *z = (const T *)p.student + row * p.ld_student;
+    T *d = (T *)p.grad + row * p.ld_grad;
+    if (mass == 0.f) {
+        RawVec<T, N> o;
+#pragma unroll
+        for (int j = 0; j < N; ++j) o.v[j] = (T)0.f;
+        i64 i = c0 + (i64)tid * N;
+        for (; i + N <= c1; i += NT * N) vec_store<T, N>(d + i, o);
+        for (int j = 0; j < N; ++j)
+            if (i + j < c1) d[i + j] = (T)0.f;
+        return;
+    }
+    const Exponent x = exponent_of(a.m, p.c);
+    const float coef = a.s == 0.f ? 0.f : gt * mass / a.s * correction_of(a.m, x);       // (a row of -inf only has q = 0)
+    for (int j = tid; j < p.k; j += NT) {
+        const int c = scol[j];
+        sz[j] = c >= c0 && c < c1 ? up(z[c]) : 0.f;
+    }
+    __syncthreads();
+    auto one = [&](float v) { return coef * exp2_fast(__fmaf_rn(v, x.c, -x.off)); };
+    i64 i = c0 + (i64)tid * N;
+    for (; i + (U - 1) * NT * N + N <= c1; i += U * NT * N) {
+        RawVec<T, N> y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) y[u] = vec_load<T, N>(z + i + u * NT * N);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            RawVec<T, N> o;
+#pragma unroll
+            for (int j = 0; j < N; ++j) o.v[j] = (T)one(up(y[u].v[j]));
+            vec_store<T, N>(d + i + u * NT * N, o);
+        }
+    }
+    for (; i + N <= c1; i += NT * N) {
+        const RawVec<T, N> y = vec_load<T, N>(z + i);
+        RawVec<T, N> o;
+#pragma unroll
+        for (int j = 0; j < N; ++j) o.v[j] = (T)one(up(y.v[j]));
+        vec_store<T, N>(d + i, o);
+    }
+    for (int j = 0; j < N; ++j)
+        if (i + j < c1) d[i + j] = (T)one(up(z[i + j]));
+    __syncthreads();
+    for (int j = tid; j < p.k; j += NT) {
+        const int c = scol[j];
+        if (c < c0 || c >= c1) continue;
+        float prob = 0.f;
+        bool first = true;
+        for (int i2 = 0; i2 < p.k; ++i2)
+            if (scol[i2] == c) {
+                first = first && i2 >= j;
+                prob += sprob[i2];
+            }
+        if (first) d[c] = (T)(one(sz[j]) - gt * prob);
+    }
+}
+
+extern __shared__ int distill_list[];      // [k] columns, [k] probabilities, [k] scores
+
+template <typename T, int NT> __global__ __launch_bounds__(NT) void sp_distill_grad_kernel(DistillParams p) {
+    __shared__ float mass;
+    int *scol = distill_list;
+    float *sprob = (float *)(distill_list + p.k), *sz = sprob + p.k;
+    const i64 row = blockIdx.x / p.splits, c0 = (blockIdx.x % p.splits) * p.chunk, c1 = min(p.n_cols, c0 + p.chunk);
+    if (threadIdx.x < 64) {
+        const ListSums l = list_sums<T, false>(p, row, nullptr, MaxSum{0.f, 1.f}, scol, sprob);
+        if (threadIdx.x == 0) mass = l.mass;
+    }
+    const MaxSum a{p.stats[2 * row], p.stats[2 * row + 1]};
+    const float gt = (p.grad_loss ? p.grad_loss[row] : 1.f) * p.tau;
+    __syncthreads();
+    grad_columns<T, NT>(p, row, c0, c1, a, mass, gt, scol, sprob, sz);
+}
+
+// loss and gradient of a row by one workgroup: the second reading of the row finds it in the caches
+template <typename T, int NT> __global__ __launch_bounds__(NT) void sp_distill_loss_grad_kernel(DistillParams p) {
+    __shared__ MaxSum sh[NT / 64];
+    __shared__ float mass;
+    int *scol = distill_list;
+    float *sprob = (float *)(distill_list + p.k), *sz = sprob + p.k;
+    const i64 row = blockIdx.x;
+    const T *z = (const T *)p.student + row * p.ld_student;
+    const MaxSum a = scan_columns<T, NT>(z, 0, p.n_cols, p.c, sh);
+    if (threadIdx.x < 64) {
+        const ListSums l = list_sums<T, true>(p, row, z, a, scol, sprob);
+        if (threadIdx.x == 0) {
+            mass = l.mass;
+            if (p.loss) p.loss[row] = p.tau * p.tau * l.loss;
+        }
+    }
+    const float gt = (p.grad_loss ? p.grad_loss[row] : 1.f) * p.tau;
+    __syncthreads();
+    grad_columns<T, NT>(p, row, 0, p.n_cols, a, mass, gt, scol, sprob, sz);
+}
+
+}  // namespace

@@ -65,6 +65,12 @@ namespace {
 
 }  // namespace
 
+// the error text of the library's other translation unit (sp_dense.hip): one thread-local buffer, the one sp_last_error() reads
+__attribute__((visibility("hidden"))) int sp_set_error(int code, const char *text) {
+    snprintf(g_err, sizeof(g_err), "%s", text);
+    return code;
+}
+
 extern "C" {
 
 int sp_abi_version(void) { return SP_KNN_ABI_VERSION; }

@@ -142,3 +142,37 @@ class DeviceProblem:
             _abi.call_knn(a)
         return {"kernel_ms": float(a.kernel_ms), "passes_total": int(a.passes_total), "phase_cycles": [int(x) for x in a.phase_cycles], "num_wgs": int(a.num_wgs_used),
                 "sparse_kernel_ms": int(a.reserved[1]) / 1e3, "generic_kernel_ms": int(a.reserved[2]) / 1e3, "transpose_ms": int(a.reserved[3]) / 1e3}
+
+    # ------------------------------------------------------------------ dense operators on the resident operands
+    def embed(self, table, scale: float = 1.0):
+        """Rows of m1 (the histories) times an embedding table: :func:`similaripy_amd.dense.embed_rows` on the resident CSR."""
+        from . import dense
+        torch = _torch()
+        t = self.t
+        if t["m1_indices"] is None:
+            empty = torch.zeros(0, dtype=torch.int32, device=self.device)
+            return dense.embed_rows(table, empty, torch.zeros(self.call.n_rows_m1 + 1, dtype=torch.int32, device=self.device), scale=scale)
+        return dense.embed_rows(table, t["m1_indices"], t["m1_indptr"], t["m1_data"], scale=scale)
+
+    def adjust_scores(self, scores, targets=None, **kw):
+        """:func:`similaripy_amd.dense.adjust_scores` with this problem's MATRIX selectors: row i of the scores is target i of the
+        problem (or ``targets[i]``); columns that ``filter_cols`` lists and that ``target_cols`` does not list become ``-inf``."""
+        from . import dense
+        from ._host import MODE_ARRAY, MODE_MATRIX
+        torch = _torch()
+        c, t = self.call, self.t
+        if MODE_ARRAY in (c.filter_mode, c.target_col_mode):
+            raise ValueError("adjust_scores: ARRAY selectors are applied to matrix2 and not kept; pass their columns as packed bits to dense.adjust_scores")
+
+        def pattern(mode, indptr, indices):
+            if mode != MODE_MATRIX:
+                return None
+            return (t[indptr], t[indices] if t[indices] is not None else torch.zeros(0, dtype=torch.int32, device=self.device))
+        return dense.adjust_scores(scores, targets=self.t["targets"] if targets is None else targets,
+                                   filter_cols=pattern(c.filter_mode, "filter_m_indptr", "filter_m_indices"),
+                                   target_cols=pattern(c.target_col_mode, "target_col_m_indptr", "target_col_m_indices"), **kw)
+
+    def distill_loss(self, student, cols, vals, counts, **kw):
+        """:func:`similaripy_amd.dense.distill_loss` of a student's scores (one row per target) from the lists that :meth:`run` wrote."""
+        from . import dense
+        return dense.distill_loss(student, cols, vals, counts, **kw)
