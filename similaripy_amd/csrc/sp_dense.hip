@@ -212,14 +212,20 @@ int check_pattern(const sp_csr_pattern &m, const char *what) {
     if (m.nnz > 0 && !m.indices) return fail(SP_EINVAL, "%s: NULL indices", what);
     return SP_OK;
 }
+constexpr i64 AD_WGS = 2048;
 CsrPattern pattern_of(const sp_csr_pattern &m) { return {m.indptr, m.indices, m.n_rows, m.nnz, m.index64}; }
 
-template <typename T, int U> int launch_adjust(AdjustParams p, bool counts, hipStream_t stream) {
-    p.tiles = (int)ceil_div(p.n_cols, AD_NT * VecOf<T>::N * U);
-    const i64 blocks = p.n_rows * p.tiles;
+template <typename T> int launch_adjust(AdjustParams p, bool counts, hipStream_t stream) {
+    // a row in segments of up to AD_SEG columns; few rows in shorter ones, down to 2048, so that about AD_WGS workgroups run
+    i64 segs = ceil_div(p.n_cols, AD_SEG);
+    const i64 want = ceil_div(AD_WGS, p.n_rows), most = ceil_div(p.n_cols, 2048);
+    if (segs < want) segs = want < most ? want : most;
+    p.seg = (int)(ceil_div(ceil_div(p.n_cols, segs), 2048) * 2048);
+    p.segs = (int)ceil_div(p.n_cols, p.seg);
+    const i64 blocks = p.n_rows * p.segs;
     if (blocks > I32_MAX) return fail(SP_EINVAL, "too many scores for one launch");
-    if (counts) hipLaunchKernelGGL((sp_adjust_kernel<T, U, true>), dim3((unsigned)blocks), dim3(AD_NT), 0, stream, p);
-    else hipLaunchKernelGGL((sp_adjust_kernel<T, U, false>), dim3((unsigned)blocks), dim3(AD_NT), 0, stream, p);
+    if (counts) hipLaunchKernelGGL((sp_adjust_kernel<T, true>), dim3((unsigned)blocks), dim3(AD_NT), 0, stream, p);
+    else hipLaunchKernelGGL((sp_adjust_kernel<T, false>), dim3((unsigned)blocks), dim3(AD_NT), 0, stream, p);
     HIP_TRY(hipGetLastError());
     return SP_OK;
 }
@@ -365,8 +371,7 @@ int sp_adjust_scores(const sp_adjust_args *a) {
     const bool counts = a->history.indptr && (a->repetition || a->presence || a->frequency || a->repetition_all != 1.f || a->presence_all != 0.f || a->frequency_all != 0.f);
     return with_type(a->dtype, [&](auto tag) {
         using T = decltype(tag);
-        const i64 big = a->n_rows * ceil_div(a->n_cols, AD_NT * VecOf<T>::N * 4);
-        return big >= 512 ? launch_adjust<T, 4>(p, counts, (hipStream_t)a->stream) : launch_adjust<T, 1>(p, counts, (hipStream_t)a->stream);
+        return launch_adjust<T>(p, counts, (hipStream_t)a->stream);
     });
 }
 
