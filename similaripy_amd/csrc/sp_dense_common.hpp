@@ -24,6 +24,16 @@ template <typename T, int N> __device__ __forceinline__ RawVec<T, N> vec_load(co
 }
 template <typename T, int N> __device__ __forceinline__ void vec_store(T *p, const RawVec<T, N> &r) { __builtin_memcpy(p, &r, sizeof(r)); }
 
+// the same past the caches: for results that the kernel does not read again
+template <typename T, int N> __device__ __forceinline__ void vec_store_once(T *p, const RawVec<T, N> &r) {
+    static_assert(sizeof(r) == 16, "16 bytes");
+    typedef unsigned Quad __attribute__((ext_vector_type(4)));
+    typedef Quad LooseQuad __attribute__((aligned(2)));
+    Quad q;
+    __builtin_memcpy(&q, &r, 16);
+    __builtin_nontemporal_store(q, (LooseQuad *)p);
+}
+
 __device__ __forceinline__ float up(float x) { return x; }
 __device__ __forceinline__ float up(__bf16 x) { return (float)x; }
 __device__ __forceinline__ float up(_Float16 x) { return (float)x; }
