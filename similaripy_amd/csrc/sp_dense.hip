@@ -111,10 +111,11 @@ int run_embed(const sp_embed_args *a) {
             constexpr int G = decltype(gc)::value;
             EmbedParams p = embed_params(a);
             p.slabs = (int)ceil_div(a->dim, G * N);
-            const i64 blocks = ceil_div(a->n_rows * p.slabs, 256 / G);
+            const i64 blocks = a->indptr ? ceil_div(a->n_rows * p.slabs, 4) : ceil_div(ceil_div(a->n_rows, 2) * p.slabs, 256 / G);
             if (blocks > I32_MAX) return fail(SP_EINVAL, "too many rows for one launch");
-            if (a->index64) hipLaunchKernelGGL((sp_embed_rows_kernel<T, i64, G>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
-            else hipLaunchKernelGGL((sp_embed_rows_kernel<T, int, G>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+            auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p); };
+            if (a->indptr) a->index64 ? launch(sp_embed_rows_kernel<T, i64, G>) : launch(sp_embed_rows_kernel<T, int, G>);
+            else a->index64 ? launch(sp_embed_lookup_kernel<T, i64, G>) : launch(sp_embed_lookup_kernel<T, int, G>);
             HIP_TRY(hipGetLastError());
             return (int)SP_OK;
         });
@@ -122,10 +123,12 @@ int run_embed(const sp_embed_args *a) {
 }
 
 // workspace of the gradient: two copies of the sorted entries (the passes alternate), the digit counts, the partial sums
+constexpr i64 REDUCE_CHUNKS = 4096;      // groups that sum sorted entries: about four waves per SIMD at one slab of 64 lanes
+constexpr int FILL_WGS = 512;
 struct GradLayout {
     int wgs, sort_chunk, passes, bits, chunk;
     i64 chunks;
-    size_t key[2], pay[2], w[2], hist, part, total;
+    size_t key[2], pay[2], w[2], hist, digits, part, total;
 };
 GradLayout grad_layout(const sp_embed_args *a) {
     GradLayout L{};
@@ -137,8 +140,8 @@ GradLayout grad_layout(const sp_embed_args *a) {
     while (kb < 31 && (1ll << kb) <= a->n_vocab) ++kb;
     L.passes = (kb + 8) / 9;
     L.bits = (kb + L.passes - 1) / L.passes;
-    L.chunk = (int)ceil_div(n, 8192);
-    L.chunk = L.chunk < 16 ? 16 : L.chunk > 1024 ? 1024 : L.chunk;
+    const i64 per = ceil_div(n, REDUCE_CHUNKS);
+    L.chunk = (int)(per < 16 ? 16 : per);
     L.chunks = ceil_div(n, L.chunk);
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) & ~(size_t)255; return o; };
@@ -148,6 +151,7 @@ GradLayout grad_layout(const sp_embed_args *a) {
         L.w[i] = a->data ? take((size_t)n * 4) : 0;
     }
     L.hist = take((size_t)L.wgs * SORT_BINS * 4);
+    L.digits = take((size_t)SORT_BINS * 4);
     L.part = take((size_t)L.chunks * 2 * (size_t)a->dim * 4);
     L.total = at;
     return L;
@@ -156,9 +160,14 @@ GradLayout grad_layout(const sp_embed_args *a) {
 template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a) {
     hipStream_t stream = (hipStream_t)a->stream;
     constexpr int N = VecOf<T>::N;
+    FillParams fill{};
     if (!a->accumulate) {
-        const i64 blocks = ceil_div(a->n_vocab * a->dim, 256 * VecOf<TO>::N);
-        hipLaunchKernelGGL((sp_fill_rows_kernel<TO>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream, (TO *)a->out, a->n_vocab, a->dim, a->ld_out);
+        fill.out = a->out;
+        fill.n_rows = a->n_vocab; fill.dim = a->dim; fill.ld = a->n_vocab > 1 ? a->ld_out : a->dim; fill.bytes = (int)sizeof(TO);
+    }
+    if (a->nnz == 0 && fill.out) {
+        fill.parts = 1;
+        hipLaunchKernelGGL(sp_fill_kernel<SORT_NT>, dim3(FILL_WGS * 2), dim3(SORT_NT), 0, stream, fill);
     }
     if (a->nnz > 0) {
         const GradLayout L = grad_layout(a);
@@ -166,21 +175,22 @@ template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a)
         SortParams s{};
         s.n = a->nnz; s.chunk = L.sort_chunk; s.wgs = L.wgs; s.bits = L.bits;
         s.hist = (unsigned *)(ws + L.hist);
+        s.total = (unsigned *)(ws + L.digits);
         s.indices = a->indices; s.indptr = a->indptr; s.n_rows = a->n_rows; s.n_vocab = a->n_vocab;
         s.w_in = a->data;
+        s.fill = fill;
+        s.fill.parts = 2 * L.passes;
+        const int grid = L.wgs + (fill.out ? FILL_WGS : 0);
         for (int pass = 0; pass < L.passes; ++pass) {
             const int to = pass & 1;
             s.shift = pass * L.bits;
             s.key_out = (unsigned *)(ws + L.key[to]);
             s.pay_out = (unsigned *)(ws + L.pay[to]);
             s.w_out = a->data ? (float *)(ws + L.w[to]) : nullptr;
-            if (a->index64) {
-                hipLaunchKernelGGL((sp_sort_count_kernel<i64>), dim3(L.wgs), dim3(SORT_NT), 0, stream, s);
-                hipLaunchKernelGGL((sp_sort_move_kernel<i64>), dim3(L.wgs), dim3(SORT_NT), 0, stream, s);
-            } else {
-                hipLaunchKernelGGL((sp_sort_count_kernel<int>), dim3(L.wgs), dim3(SORT_NT), 0, stream, s);
-                hipLaunchKernelGGL((sp_sort_move_kernel<int>), dim3(L.wgs), dim3(SORT_NT), 0, stream, s);
-            }
+            auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(SORT_NT), 0, stream, s); ++s.fill.part; };
+            a->index64 ? launch(sp_sort_count_kernel<i64>) : launch(sp_sort_count_kernel<int>);
+            hipLaunchKernelGGL(sp_sort_prefix_kernel, dim3(SORT_BINS / 64), dim3(64), 0, stream, s.hist, s.total, s.wgs);
+            a->index64 ? launch(sp_sort_move_kernel<i64>) : launch(sp_sort_move_kernel<int>);
             s.key_in = s.key_out;
             s.pay_in = s.pay_out;
             s.w_in = s.w_out;
@@ -194,9 +204,9 @@ template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a)
             constexpr int G = decltype(gc)::value;
             r.slabs = (int)ceil_div(a->dim, G * N);
             const i64 blocks = ceil_div(L.chunks * r.slabs, 256 / G);
-            if (blocks > I32_MAX) return fail(SP_EINVAL, "too many entries for one launch");
+            if (L.chunks * r.slabs > I32_MAX) return fail(SP_EINVAL, "too many entries for one launch");
             hipLaunchKernelGGL((sp_embed_reduce_kernel<T, TO, G>), dim3((unsigned)blocks), dim3(256), 0, stream, r);
-            if (L.chunks > 1) hipLaunchKernelGGL((sp_embed_join_kernel<TO, N, G>), dim3((unsigned)blocks), dim3(256), 0, stream, r);
+            if (L.chunks > 1) hipLaunchKernelGGL((sp_embed_join_kernel<TO, N, G>), dim3((unsigned)((L.chunks - 1) * r.slabs)), dim3(256), 0, stream, r);
             return (int)SP_OK;
         }));
     }

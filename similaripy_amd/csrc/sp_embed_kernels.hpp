@@ -48,44 +48,90 @@ template <typename T, int N> __device__ __forceinline__ void store_piece(T *row,
     }
 }
 
-// One group of G lanes per row and slab of G * N columns.
-template <typename T, typename I, int G> __global__ __launch_bounds__(256) void sp_embed_rows_kernel(EmbedParams p) {
-    constexpr int N = VecOf<T>::N, U = 4;
+// value of lane `at` of the group of G lanes
+template <int G> __device__ __forceinline__ int group_lane(int v, int at) { return G == 64 ? __builtin_amdgcn_readlane(v, at) : __shfl(v, at, G); }
+
+// Lookup: one group of G lanes per U rows and slab of G * N columns.
+template <typename T, typename I, int G> __global__ __launch_bounds__(256) void sp_embed_lookup_kernel(EmbedParams p) {
+    constexpr int N = VecOf<T>::N, U = 2;
     const int lane = threadIdx.x & (G - 1);
     const i64 item = (i64)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const i64 row = item / p.slabs * U;
+    const int c = ((int)(item % p.slabs) * G + lane) * N;
+    if (row >= p.n_rows || c >= p.dim) return;
+    Piece<T, N> x[U];
+    i64 id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = row + u < p.n_rows ? (i64)((const I *)p.indices)[row + u] : -1;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (id[u] >= 0 && id[u] < p.n_vocab) x[u].load((const T *)p.in + id[u] * p.ld_in, c, p.dim);
+        else x[u].zero();
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (row + u < p.n_rows) {
+            float v[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = up(x[u].r.v[j]) * p.scale;
+            store_piece<T, N>((T *)p.out + (row + u) * p.ld_out, c, p.dim, v);
+        }
+}
+
+// Bags: one wave per row and slab.  Its 64 / G groups take the row's entries in turn; 64 ids and weights are read at once, a lane each, and
+// U rows of the table are on their way per group.
+template <typename T, typename I, int G> __global__ __launch_bounds__(256) void sp_embed_rows_kernel(EmbedParams p) {
+    constexpr int N = VecOf<T>::N, S = 64 / G, U = 8;
+    static_assert(S * U <= 64, "a round stays inside the 64 entries read at once");
+    const int lane = threadIdx.x & 63, sub = lane / G;
+    const i64 item = (i64)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const i64 row = item / p.slabs;
     if (row >= p.n_rows) return;
-    const int c = ((int)(item % p.slabs) * G + lane) * N;
-    if (c >= p.dim) return;
+    const int c = ((int)(item % p.slabs) * G + (lane & (G - 1))) * N;
+    const bool active = c < p.dim;
     const I *ids = (const I *)p.indices;
-    i64 b = row, e = row + 1;
-    if (p.indptr) {
-        b = max((i64)0, (i64)((const I *)p.indptr)[row]);
-        e = min(p.nnz, (i64)((const I *)p.indptr)[row + 1]);
-    }
+    const i64 b = max((i64)0, (i64)((const I *)p.indptr)[row]), e = min(p.nnz, (i64)((const I *)p.indptr)[row + 1]);
     float acc[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
-    for (i64 i = b; i < e; i += U) {
-        Piece<T, N> x[U];
-        float w[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            i64 id = -1;
-            if (i + u < e) id = (i64)ids[i + u];
-            const bool ok = id >= 0 && id < p.n_vocab;
-            w[u] = !ok ? 0.f : p.data ? p.data[i + u] : 1.f;
-            if (ok) x[u].load((const T *)p.in + id * p.ld_in, c, p.dim);
-            else x[u].zero();
+    for (i64 i = b; i < e; i += 64) {
+        const int n = (int)min((i64)64, e - i);
+        int mine = -1;
+        float weight = 0.f;
+        if (lane < n) {
+            const i64 id = (i64)ids[i + lane];
+            mine = id >= 0 && id < p.n_vocab ? (int)id : -1;
+            weight = p.data ? p.data[i + lane] : 1.f;
         }
+        for (int j = 0; j < n; j += S * U) {
+            Piece<T, N> x[U];
+            float w[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                const int at = j + u * S + sub;
+                const int id = S == 1 ? __builtin_amdgcn_readlane(mine, j + u) : __shfl(mine, at, 64);
+                w[u] = __int_as_float(S == 1 ? __builtin_amdgcn_readlane(__float_as_int(weight), j + u) : __shfl(__float_as_int(weight), at, 64));
+                if (id >= 0 && active) x[u].load((const T *)p.in + (i64)id * p.ld_in, c, p.dim);
+                else {
+                    x[u].zero();
+                    w[u] = 0.f;
+                }
+            }
 #pragma unroll
-            for (int j = 0; j < N; ++j) acc[j] = __fmaf_rn(w[u], up(x[u].r.v[j]), acc[j]);
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int k = 0; k < N; ++k) acc[k] = __fmaf_rn(w[u], up(x[u].r.v[k]), acc[k]);
+        }
     }
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] *= p.scale;
-    store_piece<T, N>((T *)p.out + row * p.ld_out, c, p.dim, acc);
+    for (int d = G; d < 64; d <<= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += __shfl_xor(acc[k], d, 64);
+    if (sub == 0 && active) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] *= p.scale;
+        store_piece<T, N>((T *)p.out + row * p.ld_out, c, p.dim, acc);
+    }
 }
 
 // ---- the gradient: entries sorted by id, stably ------------------------------------------------------------------------------
@@ -94,6 +140,32 @@ template <typename T, typename I, int G> __global__ __launch_bounds__(256) void 
 // Ids outside the table take the key n_vocab and end up behind everything else.
 
 constexpr int SORT_NT = 512, SORT_WAVES = SORT_NT / 64, SORT_BINS = 512, SORT_WGS = 256;
+
+// The rows of the gradient that no entry names are 0: all of it is cleared, by workgroups behind those of the sort's launches, which leave
+// most of the card free.  part / parts: this launch's share of the rows.
+struct FillParams {
+    void *out;                   // NULL: nothing to clear
+    i64 n_rows, dim, ld;         // in elements
+    int bytes;                   // of an element
+    int part, parts;
+};
+__device__ __forceinline__ void fill_share(const FillParams &f, int block, int blocks) {
+    const i64 r0 = f.n_rows * f.part / f.parts, r1 = f.n_rows * (f.part + 1) / f.parts;
+    const i64 width = f.dim * f.bytes, ld = f.ld * f.bytes;
+    unsigned char *out = (unsigned char *)f.out + r0 * ld;
+    typedef unsigned Quad __attribute__((ext_vector_type(4), aligned(2)));
+    const Quad zero = {0, 0, 0, 0};
+    if (ld == width) {
+        const i64 total = (r1 - r0) * width, step = (i64)blocks * blockDim.x * 16;
+        i64 i = ((i64)block * blockDim.x + threadIdx.x) * 16;
+        for (; i + 16 <= total; i += step) *(Quad *)(out + i) = zero;
+        for (; i < total && i + 16 > total; i += 2) *(unsigned short *)(out + i) = 0;
+    } else {
+        for (i64 r = block; r < r1 - r0; r += blocks)
+            for (i64 c = (i64)threadIdx.x * 2; c < width; c += blockDim.x * 2) *(unsigned short *)(out + r * ld + c) = 0;
+    }
+}
+template <int NT> __global__ __launch_bounds__(NT) void sp_fill_kernel(FillParams f) { fill_share(f, blockIdx.x, gridDim.x); }
 
 struct SortParams {
     i64 n;                       // entries
@@ -104,9 +176,11 @@ struct SortParams {
     const float *w_in;
     unsigned *key_out, *pay_out;
     float *w_out;                // NULL without weights
-    unsigned *hist;              // [wgs][SORT_BINS]
+    unsigned *hist;              // [wgs][SORT_BINS] digits of every workgroup's chunk; then, of the workgroups before it
+    unsigned *total;             // [SORT_BINS] digits of all
     const void *indices, *indptr;
     i64 n_rows, n_vocab;
+    FillParams fill;
 };
 
 template <typename I> __device__ __forceinline__ unsigned sort_key(const SortParams &p, i64 i) {
@@ -117,6 +191,7 @@ template <typename I> __device__ __forceinline__ unsigned sort_key(const SortPar
 
 template <typename I> __global__ __launch_bounds__(SORT_NT) void sp_sort_count_kernel(SortParams p) {
     __shared__ unsigned h[SORT_BINS];
+    if ((int)blockIdx.x >= p.wgs) return fill_share(p.fill, blockIdx.x - p.wgs, gridDim.x - p.wgs);
     for (int i = threadIdx.x; i < SORT_BINS; i += SORT_NT) h[i] = 0;
     __syncthreads();
     const i64 b = (i64)blockIdx.x * p.chunk, e = min(p.n, b + p.chunk);
@@ -124,6 +199,23 @@ template <typename I> __global__ __launch_bounds__(SORT_NT) void sp_sort_count_k
     for (i64 i = b + threadIdx.x; i < e; i += SORT_NT) atomicAdd(&h[(sort_key<I>(p, i) >> p.shift) & mask], 1u);
     __syncthreads();
     for (int i = threadIdx.x; i < SORT_BINS; i += SORT_NT) p.hist[(i64)blockIdx.x * SORT_BINS + i] = h[i];
+}
+
+// hist[g][d] becomes the sum over the workgroups before g: a thread per digit, 32 counts on their way at once
+__global__ __launch_bounds__(64) void sp_sort_prefix_kernel(unsigned *hist, unsigned *total, int wgs) {
+    const int d = blockIdx.x * 64 + threadIdx.x;
+    unsigned run = 0;
+    for (int g = 0; g < wgs; g += 32) {
+        unsigned v[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = g + k < wgs ? hist[(i64)(g + k) * SORT_BINS + d] : 0u;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+            if (g + k < wgs) hist[(i64)(g + k) * SORT_BINS + d] = run;
+            run += v[k];
+        }
+    }
+    total[d] = run;
 }
 
 // the CSR row of entry i; n_rows for an entry that no row holds
@@ -143,14 +235,10 @@ template <typename I> __global__ __launch_bounds__(SORT_NT) void sp_sort_move_ke
     __shared__ unsigned wsum[SORT_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const unsigned mask = (1u << p.bits) - 1u;
+    if ((int)blockIdx.x >= p.wgs) return fill_share(p.fill, blockIdx.x - p.wgs, gridDim.x - p.wgs);
     for (int w = 0; w < SORT_WAVES; ++w) off[w][tid] = 0;
     // entries of digit `tid` before this workgroup: those of smaller digits anywhere, and of its own in the workgroups before
-    unsigned before = 0, all = 0;
-    for (int g = 0; g < p.wgs; ++g) {
-        const unsigned v = p.hist[(i64)g * SORT_BINS + tid];
-        before += g < (int)blockIdx.x ? v : 0u;
-        all += v;
-    }
+    const unsigned before = p.hist[(i64)blockIdx.x * SORT_BINS + tid], all = p.total[tid];
     unsigned inc = all;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -194,25 +282,6 @@ template <typename I> __global__ __launch_bounds__(SORT_NT) void sp_sort_move_ke
     }
 }
 
-// every row of the gradient starts at 0
-template <typename T> __global__ __launch_bounds__(256) void sp_fill_rows_kernel(T *out, i64 n_rows, i64 dim, i64 ld) {
-    constexpr int N = VecOf<T>::N;
-    RawVec<T, N> z;
-#pragma unroll
-    for (int j = 0; j < N; ++j) z.v[j] = (T)0.f;
-    const i64 first = ((i64)blockIdx.x * 256 + threadIdx.x) * N, step = (i64)gridDim.x * 256 * N;
-    if (ld == dim || n_rows == 1) {
-        const i64 total = n_rows * dim;
-        i64 i = first;
-        for (; i + N <= total; i += step) vec_store<T, N>(out + i, z);
-        for (int j = 0; j < N; ++j)
-            if (i + j < total) out[i + j] = (T)0.f;
-    } else {
-        for (i64 r = blockIdx.x; r < n_rows; r += gridDim.x)
-            for (i64 c = threadIdx.x; c < dim; c += 256) out[r * ld + c] = (T)0.f;
-    }
-}
-
 struct ReduceParams {
     const void *in;
     void *out;
@@ -240,13 +309,14 @@ template <typename TO, int N> __device__ __forceinline__ void write_row(const Re
 // One group of G lanes per chunk of the sorted entries and slab of columns: runs of equal ids are summed as they come.  A run that
 // lies inside the chunk is a row of the gradient and is written; one that began before or goes on behind it leaves its sum in `part`.
 template <typename T, typename TO, int G> __global__ __launch_bounds__(256) void sp_embed_reduce_kernel(ReduceParams p) {
-    constexpr int N = VecOf<T>::N, U = 4;
+    constexpr int N = VecOf<T>::N, U = 8;
     const int lane = threadIdx.x & (G - 1);
-    const i64 item = (i64)blockIdx.x * (256 / G) + threadIdx.x / G;
+    i64 item = (i64)blockIdx.x * (256 / G) + threadIdx.x / G;
+    if (G == 64) item = (i64)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const i64 ch = item / p.slabs;
     if (ch >= p.chunks) return;
     const int c = ((int)(item % p.slabs) * G + lane) * N;
-    if (c >= p.dim) return;
+    const bool active = c < p.dim;
     const i64 b = ch * p.chunk, e = min(p.n, b + p.chunk);
     const unsigned none = (unsigned)p.n_vocab;
     const unsigned prev = b > 0 ? p.key[b - 1] : none, next = e < p.n ? p.key[e] : none;
@@ -256,70 +326,119 @@ template <typename T, typename TO, int G> __global__ __launch_bounds__(256) void
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
     auto flush = [&](bool last) {
-        if (run == none) return;
+        if (run == none || !active) return;
         float *slot = nullptr;
         if (head) slot = p.part + (2 * ch) * p.dim;
-        else if (last && next == run && e < p.n) slot = p.part + (2 * ch + 1) * p.dim;
+        else if (last && e < p.n && next == run) slot = p.part + (2 * ch + 1) * p.dim;
         if (slot) store_piece<float, N>(slot, c, p.dim, acc);
         else write_row<TO, N>(p, run, c, acc);
     };
-    for (i64 i = b; i < e; i += U) {
-        Piece<T, N> x[U];
-        float w[U];
-        unsigned k[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            k[u] = none;
-            w[u] = 0.f;
-            if (i + u < e) k[u] = p.key[i + u];
-            const unsigned r = k[u] != none ? p.pay[i + u] : 0u;
-            const bool ok = k[u] != none && (i64)r < p.n_rows;
-            if (ok) {
-                w[u] = p.w ? p.w[i + u] : 1.f;
-                x[u].load((const T *)p.in + (i64)r * p.ld_in, c, p.dim);
-            } else x[u].zero();
+    for (i64 i = b; i < e; i += G) {                           // G entries at once, a lane each
+        const int n = (int)min((i64)G, e - i);
+        int key = (int)none, from = -1;
+        float weight = 0.f;
+        if (lane < n) {
+            key = (int)p.key[i + lane];
+            const unsigned r = p.pay[i + lane];
+            if ((i64)r < p.n_rows) {
+                from = (int)r;
+                weight = p.w ? p.w[i + lane] : 1.f;
+            }
         }
+        if (key == (int)none) from = -1;
+        for (int j = 0; j < n; j += U) {
+            Piece<T, N> x[U];
+            float w[U];
+            unsigned k[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i + u >= e) break;
-            if (k[u] != run) {
-                flush(false);
-                run = k[u];
-                head = false;
-#pragma unroll
-                for (int j = 0; j < N; ++j) acc[j] = 0.f;
+            for (int u = 0; u < U; ++u) {
+                k[u] = (unsigned)group_lane<G>(key, j + u);
+                const int r = group_lane<G>(from, j + u);
+                w[u] = __int_as_float(group_lane<G>(__float_as_int(weight), j + u));
+                if (r >= 0 && active) x[u].load((const T *)p.in + (i64)r * p.ld_in, c, p.dim);
+                else {
+                    x[u].zero();
+                    w[u] = 0.f;
+                }
             }
 #pragma unroll
-            for (int j = 0; j < N; ++j) acc[j] = __fmaf_rn(w[u], up(x[u].r.v[j]), acc[j]);
+            for (int u = 0; u < U; ++u) {
+                if (j + u >= n) break;
+                if (k[u] != run) {
+                    flush(false);
+                    run = k[u];
+                    head = false;
+#pragma unroll
+                    for (int q = 0; q < N; ++q) acc[q] = 0.f;
+                }
+#pragma unroll
+                for (int q = 0; q < N; ++q) acc[q] = __fmaf_rn(w[u], up(x[u].r.v[q]), acc[q]);
+            }
         }
     }
     flush(true);
 }
 
-// Runs over several chunks: the group of the chunk in which a run begins adds up its parts, in order, and writes the row.
+// Runs over several chunks: the workgroup of the chunk in which a run begins adds up its parts and writes the row.  All threads look how
+// far the run goes, 256 chunks at once; the 256 / G groups then sum contiguous shares of the parts, which are joined in their order.
 template <typename TO, int N, int G> __global__ __launch_bounds__(256) void sp_embed_join_kernel(ReduceParams p) {
-    const int lane = threadIdx.x & (G - 1);
-    const i64 item = (i64)blockIdx.x * (256 / G) + threadIdx.x / G;
-    const i64 ch = item / p.slabs;
-    if (ch + 1 >= p.chunks) return;
-    const int c = ((int)(item % p.slabs) * G + lane) * N;
-    if (c >= p.dim) return;
-    const i64 b = ch * p.chunk, e = b + p.chunk;               // (not the last chunk: it is full, and key[e] exists)
+    constexpr int GROUPS = 256 / G, U = 8;
+    __shared__ float sums[GROUPS][G * N];
+    __shared__ int ends;
+    const int tid = threadIdx.x, lane = tid & (G - 1), g = tid / G;
+    const i64 ch = blockIdx.x / p.slabs;
+    const int c = ((int)(blockIdx.x % p.slabs) * G + lane) * N;
+    const bool active = c < p.dim;
+    const i64 b = ch * p.chunk, e = b + p.chunk;               // (there is a chunk behind this one: it is full, and key[e] exists)
     const unsigned run = p.key[e - 1];
     if (run == (unsigned)p.n_vocab || p.key[e] != run) return;                              // nothing goes on behind it
-    if (p.key[b] == run && b > 0 && p.key[b - 1] == run) return;                            // the run began before this chunk
+    if (b > 0 && p.key[b - 1] == run) return;                                               // the run began before this chunk
+    // chunks ch + 1 .. last hold the rest of it: the first one that does not go on into the next
+    i64 last = ch + 1;
+    for (;; last += 256) {
+        if (tid == 0) ends = 256;
+        __syncthreads();
+        const i64 k = last + tid;
+        if (k + 1 >= p.chunks || p.key[(k + 1) * p.chunk] != run) atomicMin(&ends, tid);
+        __syncthreads();
+        const int first = ends;
+        __syncthreads();
+        if (first < 256) {
+            last += first;
+            break;
+        }
+    }
+    const i64 count = last - ch, share = (count + GROUPS - 1) / GROUPS;
+    const i64 k0 = ch + 1 + g * share, k1 = min(last + 1, k0 + share);
     float acc[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] = 0.f;
+    if (active) {
+        for (i64 k = k0; k < k1; k += U) {
+            Piece<float, N> x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (k + u < k1) x[u].load(p.part + (2 * (k + u)) * p.dim, c, p.dim);
+                else x[u].zero();
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < N; ++j) acc[j] += x[u].r.v[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) sums[g][lane * N + j] = acc[j];
+    __syncthreads();
+    if (g != 0 || !active) return;
     Piece<float, N> x;
     x.load(p.part + (2 * ch + 1) * p.dim, c, p.dim);
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = x.r.v[j];
-    for (i64 k = ch + 1; k < p.chunks; ++k) {
-        x.load(p.part + (2 * k) * p.dim, c, p.dim);
+    const int parts = (int)min((i64)GROUPS, (count + share - 1) / share);
+    for (int q = 0; q < parts; ++q)
 #pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] += x.r.v[j];
-        const i64 last = min(p.n, (k + 1) * (i64)p.chunk);
-        if (p.key[last - 1] != run || last >= p.n || p.key[last] != run) break;
-    }
+        for (int j = 0; j < N; ++j) acc[j] += sums[q][lane * N + j];
     write_row<TO, N>(p, run, c, acc);
 }
 
