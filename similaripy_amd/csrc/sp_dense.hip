@@ -111,7 +111,7 @@ int run_embed(const sp_embed_args *a) {
             constexpr int G = decltype(gc)::value;
             EmbedParams p = embed_params(a);
             p.slabs = (int)ceil_div(a->dim, G * N);
-            const i64 blocks = a->indptr ? ceil_div(a->n_rows * p.slabs, 4) : ceil_div(ceil_div(a->n_rows, 2) * p.slabs, 256 / G);
+            const i64 blocks = a->indptr ? ceil_div(a->n_rows * p.slabs, 4) : ceil_div(ceil_div(a->n_rows, LOOKUP_ROWS) * p.slabs, 256 / G);
             if (blocks > I32_MAX) return fail(SP_EINVAL, "too many rows for one launch");
             auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p); };
             if (a->indptr) a->index64 ? launch(sp_embed_rows_kernel<T, i64, G>) : launch(sp_embed_rows_kernel<T, int, G>);
@@ -124,15 +124,16 @@ int run_embed(const sp_embed_args *a) {
 
 // workspace of the gradient: two copies of the sorted entries (the passes alternate), the digit counts, the partial sums
 constexpr i64 REDUCE_CHUNKS = 4096;      // groups that sum sorted entries: about four waves per SIMD at one slab of 64 lanes
-constexpr int FILL_WGS = 512;
+constexpr int FILL_WGS = 512, SORT_WGS = 512;
 struct GradLayout {
     int wgs, sort_chunk, passes, bits, chunk;
     i64 chunks;
-    size_t key[2], pay[2], w[2], hist, digits, part, total;
+    size_t key[2], pay[2], w[2], rows, hist, digits, part, total;
 };
 GradLayout grad_layout(const sp_embed_args *a) {
     GradLayout L{};
     const i64 n = a->nnz;
+    // chunks of 1024 entries, or more of them once that makes more than SORT_WGS workgroups
     L.sort_chunk = (int)(ceil_div(ceil_div(n, SORT_WGS), SORT_NT) * SORT_NT);
     if (L.sort_chunk < 1024) L.sort_chunk = 1024;
     L.wgs = (int)ceil_div(n, L.sort_chunk);
@@ -150,6 +151,7 @@ GradLayout grad_layout(const sp_embed_args *a) {
         L.pay[i] = take((size_t)n * 4);
         L.w[i] = a->data ? take((size_t)n * 4) : 0;
     }
+    L.rows = a->indptr ? take((size_t)n * 4) : 0;
     L.hist = take((size_t)L.wgs * SORT_BINS * 4);
     L.digits = take((size_t)SORT_BINS * 4);
     L.part = take((size_t)L.chunks * 2 * (size_t)a->dim * 4);
@@ -180,17 +182,18 @@ template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a)
         s.w_in = a->data;
         s.fill = fill;
         s.fill.parts = 2 * L.passes;
-        const int grid = L.wgs + (fill.out ? FILL_WGS : 0);
+        s.entry_row = a->indptr ? (unsigned *)(ws + L.rows) : nullptr;
         for (int pass = 0; pass < L.passes; ++pass) {
             const int to = pass & 1;
             s.shift = pass * L.bits;
             s.key_out = (unsigned *)(ws + L.key[to]);
             s.pay_out = (unsigned *)(ws + L.pay[to]);
             s.w_out = a->data ? (float *)(ws + L.w[to]) : nullptr;
-            auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(SORT_NT), 0, stream, s); ++s.fill.part; };
-            a->index64 ? launch(sp_sort_count_kernel<i64>) : launch(sp_sort_count_kernel<int>);
-            hipLaunchKernelGGL(sp_sort_prefix_kernel, dim3(SORT_BINS / 64), dim3(64), 0, stream, s.hist, s.total, s.wgs);
-            a->index64 ? launch(sp_sort_move_kernel<i64>) : launch(sp_sort_move_kernel<int>);
+            auto launch = [&](auto kernel, int wgs, bool more) { hipLaunchKernelGGL(kernel, dim3(wgs + (more ? FILL_WGS : 0)), dim3(SORT_NT), 0, stream, s); ++s.fill.part; };
+            const bool more = fill.out || (pass == 0 && s.entry_row);
+            a->index64 ? launch(sp_sort_count_kernel<i64>, L.wgs, more) : launch(sp_sort_count_kernel<int>, L.wgs, more);
+            if (L.wgs > SORT_DIRECT) hipLaunchKernelGGL(sp_sort_prefix_kernel, dim3(SORT_BINS / 64), dim3(1024), 0, stream, s.hist, s.total, s.wgs);
+            a->index64 ? launch(sp_sort_move_kernel<i64>, 8 * (int)ceil_div(L.wgs, 8), fill.out) : launch(sp_sort_move_kernel<int>, 8 * (int)ceil_div(L.wgs, 8), fill.out);
             s.key_in = s.key_out;
             s.pay_in = s.pay_out;
             s.w_in = s.w_out;

@@ -51,9 +51,10 @@ template <typename T, int N> __device__ __forceinline__ void store_piece(T *row,
 // value of lane `at` of the group of G lanes
 template <int G> __device__ __forceinline__ int group_lane(int v, int at) { return G == 64 ? __builtin_amdgcn_readlane(v, at) : __shfl(v, at, G); }
 
-// Lookup: one group of G lanes per U rows and slab of G * N columns.
+constexpr int LOOKUP_ROWS = 1;       // rows of a group (16 k rows of 2 KB: 14.4 us with 1, 19 with 2, 20 with 4: more waves beat more loads per wave)
+// Lookup: one group of G lanes per LOOKUP_ROWS rows and slab of G * N columns.
 template <typename T, typename I, int G> __global__ __launch_bounds__(256) void sp_embed_lookup_kernel(EmbedParams p) {
-    constexpr int N = VecOf<T>::N, U = 2;
+    constexpr int N = VecOf<T>::N, U = LOOKUP_ROWS;
     const int lane = threadIdx.x & (G - 1);
     const i64 item = (i64)blockIdx.x * (256 / G) + threadIdx.x / G;
     const i64 row = item / p.slabs * U;
@@ -135,11 +136,13 @@ template <typename T, typename I, int G> __global__ __launch_bounds__(256) void 
 }
 
 // ---- the gradient: entries sorted by id, stably ------------------------------------------------------------------------------
-// A radix sort from the low digit: per pass one launch counts the digits of every workgroup's chunk, one moves the entries.  Every
-// wave owns a contiguous part of the chunk and goes through it in order; equal digits of 64 entries are ranked by their lane.
-// Ids outside the table take the key n_vocab and end up behind everything else.
+// A radix sort from the low digit: per pass one launch counts the digits of every workgroup's chunk, one moves the entries (with many
+// workgroups one more adds the counts up between them).  Every wave owns a contiguous part of the chunk and goes through it in order;
+// equal digits of 64 entries are ranked by their lane.  Ids outside the table take the key n_vocab and end up behind everything else.
+// An entry carries its row of the gradient and its weight.  The rows of a CSR's entries are written out beside the first count.
 
-constexpr int SORT_NT = 512, SORT_WAVES = SORT_NT / 64, SORT_BINS = 512, SORT_WGS = 256;
+constexpr int SORT_NT = 512, SORT_WAVES = SORT_NT / 64, SORT_BINS = 512;
+constexpr int SORT_DIRECT = 32;      // up to so many workgroups the moving launch adds up the counts itself
 
 // The rows of the gradient that no entry names are 0: all of it is cleared, by workgroups behind those of the sort's launches, which leave
 // most of the card free.  part / parts: this launch's share of the rows.
@@ -179,6 +182,7 @@ struct SortParams {
     unsigned *hist;              // [wgs][SORT_BINS] digits of every workgroup's chunk; then, of the workgroups before it
     unsigned *total;             // [SORT_BINS] digits of all
     const void *indices, *indptr;
+    unsigned *entry_row;         // [n] rows of a CSR's entries (n_rows: in no row), or NULL: entry i is row i
     i64 n_rows, n_vocab;
     FillParams fill;
 };
@@ -189,9 +193,27 @@ template <typename I> __device__ __forceinline__ unsigned sort_key(const SortPar
     return id >= 0 && id < p.n_vocab ? (unsigned)id : (unsigned)p.n_vocab;
 }
 
+// entry_row of every entry, one wave per row; what lies before the first row and behind the last is in none
+template <typename I> __device__ __forceinline__ void spread_rows(const SortParams &p, int block, int blocks) {
+    const int lane = threadIdx.x & 63;
+    const i64 waves = (i64)blocks * SORT_WAVES;
+    for (i64 r = (i64)block * SORT_WAVES + threadIdx.x / 64; r < p.n_rows + 2; r += waves) {
+        i64 b = r == 0 ? 0 : (i64)((const I *)p.indptr)[r - 1], e = r == p.n_rows + 1 ? p.n : (i64)((const I *)p.indptr)[r];
+        b = b < 0 ? 0 : b;
+        e = e > p.n ? p.n : e;
+        const unsigned row = r == 0 || r == p.n_rows + 1 ? (unsigned)p.n_rows : (unsigned)(r - 1);
+        for (i64 i = b + lane; i < e; i += 64) p.entry_row[i] = row;
+    }
+}
+
 template <typename I> __global__ __launch_bounds__(SORT_NT) void sp_sort_count_kernel(SortParams p) {
     __shared__ unsigned h[SORT_BINS];
-    if ((int)blockIdx.x >= p.wgs) return fill_share(p.fill, blockIdx.x - p.wgs, gridDim.x - p.wgs);
+    if ((int)blockIdx.x >= p.wgs) {                            // the workgroups behind the sort's: rows of the entries, clearing
+        const int block = blockIdx.x - p.wgs, blocks = gridDim.x - p.wgs;
+        if (!p.key_in && p.entry_row) spread_rows<I>(p, block, blocks);
+        if (p.fill.out) fill_share(p.fill, block, blocks);
+        return;
+    }
     for (int i = threadIdx.x; i < SORT_BINS; i += SORT_NT) h[i] = 0;
     __syncthreads();
     const i64 b = (i64)blockIdx.x * p.chunk, e = min(p.n, b + p.chunk);
@@ -201,32 +223,35 @@ template <typename I> __global__ __launch_bounds__(SORT_NT) void sp_sort_count_k
     for (int i = threadIdx.x; i < SORT_BINS; i += SORT_NT) p.hist[(i64)blockIdx.x * SORT_BINS + i] = h[i];
 }
 
-// hist[g][d] becomes the sum over the workgroups before g: a thread per digit, 32 counts on their way at once
-__global__ __launch_bounds__(64) void sp_sort_prefix_kernel(unsigned *hist, unsigned *total, int wgs) {
-    const int d = blockIdx.x * 64 + threadIdx.x;
+// hist[g][d] becomes the sum over the workgroups before g.  64 digits per workgroup of 16 waves: a wave takes a share of the workgroups, the
+// shares' sums are joined in LDS.
+__global__ __launch_bounds__(1024) void sp_sort_prefix_kernel(unsigned *hist, unsigned *total, int wgs) {
+    __shared__ unsigned sums[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = blockIdx.x * 64 + lane;
+    const int share = (wgs + 15) / 16, g0 = wave * share, g1 = min(wgs, g0 + share);
+    unsigned sum = 0;
+    for (int g = g0; g < g1; g += 16) {
+        unsigned v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = g + k < g1 ? hist[(i64)(g + k) * SORT_BINS + d] : 0u;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) sum += v[k];
+    }
+    sums[wave][lane] = sum;
+    __syncthreads();
     unsigned run = 0;
-    for (int g = 0; g < wgs; g += 32) {
-        unsigned v[32];
+    for (int w = 0; w < wave; ++w) run += sums[w][lane];
+    if (wave == 15) total[d] = run + sum;
+    for (int g = g0; g < g1; g += 16) {
+        unsigned v[16];
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = g + k < wgs ? hist[(i64)(g + k) * SORT_BINS + d] : 0u;
+        for (int k = 0; k < 16; ++k) v[k] = g + k < g1 ? hist[(i64)(g + k) * SORT_BINS + d] : 0u;
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-            if (g + k < wgs) hist[(i64)(g + k) * SORT_BINS + d] = run;
+        for (int k = 0; k < 16; ++k) {
+            if (g + k < g1) hist[(i64)(g + k) * SORT_BINS + d] = run;
             run += v[k];
         }
     }
-    total[d] = run;
-}
-
-// the CSR row of entry i; n_rows for an entry that no row holds
-template <typename I> __device__ __forceinline__ i64 row_of(const void *indptr, i64 n_rows, i64 i) {
-    i64 lo = 0, hi = n_rows;                 // first r with indptr[r + 1] > i
-    while (lo < hi) {
-        const i64 mid = (lo + hi) >> 1;
-        if ((i64)((const I *)indptr)[mid + 1] > i) hi = mid;
-        else lo = mid + 1;
-    }
-    return lo < n_rows && (i64)((const I *)indptr)[lo] > i ? n_rows : lo;
 }
 static_assert(SORT_NT == SORT_BINS, "a thread per digit");
 
@@ -235,10 +260,30 @@ template <typename I> __global__ __launch_bounds__(SORT_NT) void sp_sort_move_ke
     __shared__ unsigned wsum[SORT_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const unsigned mask = (1u << p.bits) - 1u;
-    if ((int)blockIdx.x >= p.wgs) return fill_share(p.fill, blockIdx.x - p.wgs, gridDim.x - p.wgs);
+    // consecutive chunks go to one XCD (workgroups are dealt to the eight in turn): what they write next to each other meets in its L2
+    const int per_xcd = (p.wgs + 7) / 8;
+    if ((int)blockIdx.x >= 8 * per_xcd) {
+        if (p.fill.out) fill_share(p.fill, blockIdx.x - 8 * per_xcd, gridDim.x - 8 * per_xcd);
+        return;
+    }
+    const int wg = (int)(blockIdx.x % 8) * per_xcd + (int)blockIdx.x / 8;
+    if (wg >= p.wgs) return;
     for (int w = 0; w < SORT_WAVES; ++w) off[w][tid] = 0;
     // entries of digit `tid` before this workgroup: those of smaller digits anywhere, and of its own in the workgroups before
-    const unsigned before = p.hist[(i64)blockIdx.x * SORT_BINS + tid], all = p.total[tid];
+    unsigned before = 0, all = 0;
+    if (p.wgs <= SORT_DIRECT) {
+        unsigned v[SORT_DIRECT];
+#pragma unroll
+        for (int g = 0; g < SORT_DIRECT; ++g) v[g] = g < p.wgs ? p.hist[(i64)g * SORT_BINS + tid] : 0u;
+#pragma unroll
+        for (int g = 0; g < SORT_DIRECT; ++g) {
+            before += g < wg ? v[g] : 0u;
+            all += v[g];
+        }
+    } else {
+        before = p.hist[(i64)wg * SORT_BINS + tid];
+        all = p.total[tid];
+    }
     unsigned inc = all;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -251,7 +296,7 @@ template <typename I> __global__ __launch_bounds__(SORT_NT) void sp_sort_move_ke
     for (int w = 0; w < wave; ++w) base += wsum[w];
     // digits of every wave's part
     const int per = p.chunk / SORT_WAVES;
-    const i64 b = (i64)blockIdx.x * p.chunk + (i64)wave * per, e = min(p.n, b + per);
+    const i64 b = (i64)wg * p.chunk + (i64)wave * per, e = min(p.n, b + per);
     for (i64 i = b + lane; i < e; i += 64) atomicAdd(&off[wave][(sort_key<I>(p, i) >> p.shift) & mask], 1u);
     __syncthreads();
     for (int w = 0; w < SORT_WAVES; ++w) {
@@ -261,23 +306,36 @@ template <typename I> __global__ __launch_bounds__(SORT_NT) void sp_sort_move_ke
     }
     __syncthreads();
     volatile unsigned *mine = off[wave];
-    for (i64 i0 = b; i0 < e; i0 += 64) {
-        const i64 i = i0 + lane;
-        const bool ok = i < e;
-        const unsigned key = ok ? sort_key<I>(p, i) : 0u, digit = (key >> p.shift) & mask;
-        u64 same = __ballot(ok);
-        for (int k = 0; k < p.bits; ++k) {
-            const u64 set = __ballot((digit >> k) & 1u);
-            same &= (digit >> k) & 1u ? set : ~set;
+    constexpr int Q = 4;                                       // 64 entries each, requested together
+    for (i64 i0 = b; i0 < e; i0 += 64 * Q) {
+        unsigned key[Q], pay[Q];
+        float weight[Q];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const i64 i = i0 + q * 64 + lane;
+            if (i < e) {
+                key[q] = sort_key<I>(p, i);
+                pay[q] = p.key_in ? p.pay_in[i] : p.entry_row ? p.entry_row[i] : (unsigned)i;
+                if (p.w_out) weight[q] = p.w_in[i];
+            }
         }
-        if (ok) {
-            const unsigned rank = (unsigned)__popcll(same & ((1ull << lane) - 1ull));
-            const unsigned at = mine[digit] + rank;
-            if (rank == 0) mine[digit] = at + (unsigned)__popcll(same);       // (a wave's LDS accesses keep their order: everybody has read)
-            p.key_out[at] = key;
-            if (p.key_in) p.pay_out[at] = p.pay_in[i];
-            else p.pay_out[at] = p.indptr ? (unsigned)row_of<I>(p.indptr, p.n_rows, i) : (unsigned)i;
-            if (p.w_out) p.w_out[at] = p.w_in[i];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const bool ok = i0 + q * 64 + lane < e;
+            const unsigned digit = ok ? (key[q] >> p.shift) & mask : 0u;
+            u64 same = __ballot(ok);
+            for (int k = 0; k < p.bits; ++k) {
+                const u64 set = __ballot((digit >> k) & 1u);
+                same &= (digit >> k) & 1u ? set : ~set;
+            }
+            if (ok) {
+                const unsigned rank = (unsigned)__popcll(same & ((1ull << lane) - 1ull));
+                const unsigned at = mine[digit] + rank;
+                if (rank == 0) mine[digit] = at + (unsigned)__popcll(same);       // (a wave's LDS accesses keep their order: everybody has read)
+                p.key_out[at] = key[q];
+                p.pay_out[at] = pay[q];
+                if (p.w_out) p.w_out[at] = weight[q];
+            }
         }
     }
 }
