@@ -21,30 +21,36 @@ struct EmbedParams {
     int slabs;              // column slabs of a row: ceil(dim / (G * N))
 };
 
-// N elements at column c of a row of `dim`, in 32 bits; beyond the row 0
-template <typename T, int N> struct Piece {
-    RawVec<T, N> r;
-    __device__ __forceinline__ void load(const T *row, int c, int dim) {
-        if (c + N <= dim) r = vec_load<T, N>(row + c);
-        else {
-#pragma unroll
-            for (int j = 0; j < N; ++j) r.v[j] = c + j < dim ? row[c + j] : (T)0.f;
-        }
-    }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int j = 0; j < N; ++j) r.v[j] = (T)0.f;
-    }
+// The columns of a lane: N of them from c on.  The last lane of a row moves back to the row's last N columns instead of taking fewer (it
+// repeats what the lane before it computes, to the same bits), so that every access is a whole vector; only rows shorter than N differ.
+template <int N> struct Columns {
+    int own;           // first column that is this lane's alone
+    int c;
+    bool active, whole;
+    __device__ __forceinline__ Columns(int first, int dim) : own(first), c(dim >= N && first > dim - N ? dim - N : first), active(first < dim), whole(dim >= N) {}
 };
-template <typename T, int N> __device__ __forceinline__ void store_piece(T *row, int c, int dim, const float *v) {
+template <typename T, int N> __device__ __forceinline__ RawVec<T, N> piece_load(const T *row, const Columns<N> &l, int dim) {
+    if (l.whole) return vec_load<T, N>(row + l.c);
+    RawVec<T, N> r;
+#pragma unroll
+    for (int j = 0; j < N; ++j) r.v[j] = j < dim ? row[j] : (T)0.f;
+    return r;
+}
+template <typename T, int N> __device__ __forceinline__ RawVec<T, N> piece_zero() {
+    RawVec<T, N> r;
+#pragma unroll
+    for (int j = 0; j < N; ++j) r.v[j] = (T)0.f;
+    return r;
+}
+template <typename T, int N> __device__ __forceinline__ void piece_store(T *row, const Columns<N> &l, int dim, const float *v) {
     RawVec<T, N> o;
 #pragma unroll
     for (int j = 0; j < N; ++j) o.v[j] = (T)v[j];
-    if (c + N <= dim) vec_store<T, N>(row + c, o);
+    if (l.whole) vec_store<T, N>(row + l.c, o);
     else {
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            if (c + j < dim) row[c + j] = o.v[j];
+            if (j < dim) row[j] = o.v[j];
     }
 }
 
@@ -58,24 +64,24 @@ template <typename T, typename I, int G> __global__ __launch_bounds__(256) void 
     const int lane = threadIdx.x & (G - 1);
     const i64 item = (i64)blockIdx.x * (256 / G) + threadIdx.x / G;
     const i64 row = item / p.slabs * U;
-    const int c = ((int)(item % p.slabs) * G + lane) * N;
-    if (row >= p.n_rows || c >= p.dim) return;
-    Piece<T, N> x[U];
+    const Columns<N> cols(((int)(item % p.slabs) * G + lane) * N, p.dim);
+    if (row >= p.n_rows || !cols.active) return;
+    RawVec<T, N> x[U];
     i64 id[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) id[u] = row + u < p.n_rows ? (i64)((const I *)p.indices)[row + u] : -1;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        if (id[u] >= 0 && id[u] < p.n_vocab) x[u].load((const T *)p.in + id[u] * p.ld_in, c, p.dim);
-        else x[u].zero();
+        if (id[u] >= 0 && id[u] < p.n_vocab) x[u] = piece_load<T, N>((const T *)p.in + id[u] * p.ld_in, cols, p.dim);
+        else x[u] = piece_zero<T, N>();
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
         if (row + u < p.n_rows) {
             float v[N];
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = up(x[u].r.v[j]) * p.scale;
-            store_piece<T, N>((T *)p.out + (row + u) * p.ld_out, c, p.dim, v);
+            for (int j = 0; j < N; ++j) v[j] = up(x[u].v[j]) * p.scale;
+            piece_store<T, N>((T *)p.out + (row + u) * p.ld_out, cols, p.dim, v);
         }
 }
 
@@ -88,8 +94,7 @@ template <typename T, typename I, int G> __global__ __launch_bounds__(256) void 
     const i64 item = (i64)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const i64 row = item / p.slabs;
     if (row >= p.n_rows) return;
-    const int c = ((int)(item % p.slabs) * G + (lane & (G - 1))) * N;
-    const bool active = c < p.dim;
+    const Columns<N> cols(((int)(item % p.slabs) * G + (lane & (G - 1))) * N, p.dim);
     const I *ids = (const I *)p.indices;
     const i64 b = max((i64)0, (i64)((const I *)p.indptr)[row]), e = min(p.nnz, (i64)((const I *)p.indptr)[row + 1]);
     float acc[N];
@@ -105,33 +110,33 @@ template <typename T, typename I, int G> __global__ __launch_bounds__(256) void 
             weight = p.data ? p.data[i + lane] : 1.f;
         }
         for (int j = 0; j < n; j += S * U) {
-            Piece<T, N> x[U];
+            RawVec<T, N> x[U];
             float w[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int at = j + u * S + sub;
                 const int id = S == 1 ? __builtin_amdgcn_readlane(mine, j + u) : __shfl(mine, at, 64);
                 w[u] = __int_as_float(S == 1 ? __builtin_amdgcn_readlane(__float_as_int(weight), j + u) : __shfl(__float_as_int(weight), at, 64));
-                if (id >= 0 && active) x[u].load((const T *)p.in + (i64)id * p.ld_in, c, p.dim);
+                if (id >= 0 && cols.active) x[u] = piece_load<T, N>((const T *)p.in + (i64)id * p.ld_in, cols, p.dim);
                 else {
-                    x[u].zero();
+                    x[u] = piece_zero<T, N>();
                     w[u] = 0.f;
                 }
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int k = 0; k < N; ++k) acc[k] = __fmaf_rn(w[u], up(x[u].r.v[k]), acc[k]);
+                for (int k = 0; k < N; ++k) acc[k] = __fmaf_rn(w[u], up(x[u].v[k]), acc[k]);
         }
     }
 #pragma unroll
     for (int d = G; d < 64; d <<= 1)
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[k] += __shfl_xor(acc[k], d, 64);
-    if (sub == 0 && active) {
+    if (sub == 0 && cols.active) {
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[k] *= p.scale;
-        store_piece<T, N>((T *)p.out + row * p.ld_out, c, p.dim, acc);
+        piece_store<T, N>((T *)p.out + row * p.ld_out, cols, p.dim, acc);
     }
 }
 
@@ -352,16 +357,22 @@ struct ReduceParams {
     float scale;
 };
 
-template <typename TO, int N> __device__ __forceinline__ void write_row(const ReduceParams &p, unsigned key, int c, float *acc) {
+template <typename TO, int N> __device__ __forceinline__ void write_row(const ReduceParams &p, unsigned key, const Columns<N> &cols, float *acc) {
     TO *row = (TO *)p.out + (i64)key * p.ld_out;
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] *= p.scale;
-    if (p.accumulate) {
+    if (p.accumulate && (cols.c != cols.own || !cols.whole)) {       // (columns that another lane writes as well are added to once)
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            if (c + j < p.dim) acc[j] += up(row[c + j]);
+            if (cols.c + j >= cols.own && cols.c + j < p.dim) row[cols.c + j] = (TO)(acc[j] + up(row[cols.c + j]));
+        return;
     }
-    store_piece<TO, N>(row, c, p.dim, acc);
+    if (p.accumulate) {
+        const RawVec<TO, N> was = vec_load<TO, N>(row + cols.c);
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += up(was.v[j]);
+    }
+    piece_store<TO, N>(row, cols, p.dim, acc);
 }
 
 // One group of G lanes per chunk of the sorted entries and slab of columns: runs of equal ids are summed as they come.  A run that
@@ -373,8 +384,7 @@ template <typename T, typename TO, int G> __global__ __launch_bounds__(256) void
     if (G == 64) item = (i64)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const i64 ch = item / p.slabs;
     if (ch >= p.chunks) return;
-    const int c = ((int)(item % p.slabs) * G + lane) * N;
-    const bool active = c < p.dim;
+    const Columns<N> cols(((int)(item % p.slabs) * G + lane) * N, p.dim);
     const i64 b = ch * p.chunk, e = min(p.n, b + p.chunk);
     const unsigned none = (unsigned)p.n_vocab;
     const unsigned prev = b > 0 ? p.key[b - 1] : none, next = e < p.n ? p.key[e] : none;
@@ -384,12 +394,12 @@ template <typename T, typename TO, int G> __global__ __launch_bounds__(256) void
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
     auto flush = [&](bool last) {
-        if (run == none || !active) return;
+        if (run == none || !cols.active) return;
         float *slot = nullptr;
         if (head) slot = p.part + (2 * ch) * p.dim;
         else if (last && e < p.n && next == run) slot = p.part + (2 * ch + 1) * p.dim;
-        if (slot) store_piece<float, N>(slot, c, p.dim, acc);
-        else write_row<TO, N>(p, run, c, acc);
+        if (slot) piece_store<float, N>(slot, cols, p.dim, acc);
+        else write_row<TO, N>(p, run, cols, acc);
     };
     for (i64 i = b; i < e; i += G) {                           // G entries at once, a lane each
         const int n = (int)min((i64)G, e - i);
@@ -405,7 +415,7 @@ template <typename T, typename TO, int G> __global__ __launch_bounds__(256) void
         }
         if (key == (int)none) from = -1;
         for (int j = 0; j < n; j += U) {
-            Piece<T, N> x[U];
+            RawVec<T, N> x[U];
             float w[U];
             unsigned k[U];
 #pragma unroll
@@ -413,9 +423,9 @@ template <typename T, typename TO, int G> __global__ __launch_bounds__(256) void
                 k[u] = (unsigned)group_lane<G>(key, j + u);
                 const int r = group_lane<G>(from, j + u);
                 w[u] = __int_as_float(group_lane<G>(__float_as_int(weight), j + u));
-                if (r >= 0 && active) x[u].load((const T *)p.in + (i64)r * p.ld_in, c, p.dim);
+                if (r >= 0 && cols.active) x[u] = piece_load<T, N>((const T *)p.in + (i64)r * p.ld_in, cols, p.dim);
                 else {
-                    x[u].zero();
+                    x[u] = piece_zero<T, N>();
                     w[u] = 0.f;
                 }
             }
@@ -430,7 +440,7 @@ template <typename T, typename TO, int G> __global__ __launch_bounds__(256) void
                     for (int q = 0; q < N; ++q) acc[q] = 0.f;
                 }
 #pragma unroll
-                for (int q = 0; q < N; ++q) acc[q] = __fmaf_rn(w[u], up(x[u].r.v[q]), acc[q]);
+                for (int q = 0; q < N; ++q) acc[q] = __fmaf_rn(w[u], up(x[u].v[q]), acc[q]);
             }
         }
     }
@@ -445,8 +455,7 @@ template <typename TO, int N, int G> __global__ __launch_bounds__(256) void sp_e
     __shared__ int ends;
     const int tid = threadIdx.x, lane = tid & (G - 1), g = tid / G;
     const i64 ch = blockIdx.x / p.slabs;
-    const int c = ((int)(blockIdx.x % p.slabs) * G + lane) * N;
-    const bool active = c < p.dim;
+    const Columns<N> cols(((int)(blockIdx.x % p.slabs) * G + lane) * N, p.dim);
     const i64 b = ch * p.chunk, e = b + p.chunk;               // (there is a chunk behind this one: it is full, and key[e] exists)
     const unsigned run = p.key[e - 1];
     if (run == (unsigned)p.n_vocab || p.key[e] != run) return;                              // nothing goes on behind it
@@ -471,33 +480,29 @@ template <typename TO, int N, int G> __global__ __launch_bounds__(256) void sp_e
     float acc[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
-    if (active) {
+    if (cols.active) {
         for (i64 k = k0; k < k1; k += U) {
-            Piece<float, N> x[U];
+            RawVec<float, N> x[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (k + u < k1) x[u].load(p.part + (2 * (k + u)) * p.dim, c, p.dim);
-                else x[u].zero();
-            }
+            for (int u = 0; u < U; ++u) x[u] = k + u < k1 ? piece_load<float, N>(p.part + (2 * (k + u)) * p.dim, cols, p.dim) : piece_zero<float, N>();
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int j = 0; j < N; ++j) acc[j] += x[u].r.v[j];
+                for (int j = 0; j < N; ++j) acc[j] += x[u].v[j];
         }
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) sums[g][lane * N + j] = acc[j];
     __syncthreads();
-    if (g != 0 || !active) return;
-    Piece<float, N> x;
-    x.load(p.part + (2 * ch + 1) * p.dim, c, p.dim);
+    if (g != 0 || !cols.active) return;
+    const RawVec<float, N> x = piece_load<float, N>(p.part + (2 * ch + 1) * p.dim, cols, p.dim);
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = x.r.v[j];
+    for (int j = 0; j < N; ++j) acc[j] = x.v[j];
     const int parts = (int)min((i64)GROUPS, (count + share - 1) / share);
     for (int q = 0; q < parts; ++q)
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] += sums[q][lane * N + j];
-    write_row<TO, N>(p, run, c, acc);
+    write_row<TO, N>(p, run, cols, acc);
 }
 
 }  // namespace
