@@ -78,20 +78,17 @@ int check_embed(const sp_embed_args *a) {
     return SP_OK;
 }
 
-// lanes of a group: the fewest that cover a row with N elements each, 8 .. 64; columns beyond 64 lanes make further slabs
-int group_of(i64 dim, int n) {
-    const i64 lanes = ceil_div(dim, n);
-    int g = 8;
-    while (g < 64 && g < lanes) g *= 2;
-    return g;
-}
-template <typename F> int with_group(int g, F f) {
-    switch (g) {
-    case 8: return f(std::integral_constant<int, 8>());
-    case 16: return f(std::integral_constant<int, 16>());
-    case 32: return f(std::integral_constant<int, 32>());
-    default: return f(std::integral_constant<int, 64>());
-    }
+// Calls f with the lanes of a group and the elements of a lane: 16 bytes a lane, or one element where a row has fewer; the fewest lanes that
+// cover a row, 8 .. 64 (columns beyond 64 lanes make further slabs).
+template <typename T, typename F> int with_group(i64 dim, F f) {
+    constexpr int N = VecOf<T>::N;
+    using Wide = std::integral_constant<int, N>;
+    if (dim < N) return f(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
+    const i64 lanes = ceil_div(dim, N);
+    if (lanes <= 8) return f(std::integral_constant<int, 8>(), Wide());
+    if (lanes <= 16) return f(std::integral_constant<int, 16>(), Wide());
+    if (lanes <= 32) return f(std::integral_constant<int, 32>(), Wide());
+    return f(std::integral_constant<int, 64>(), Wide());
 }
 
 EmbedParams embed_params(const sp_embed_args *a) {
@@ -102,20 +99,28 @@ EmbedParams embed_params(const sp_embed_args *a) {
     return p;
 }
 
+constexpr int FILL_WGS = 512;      // workgroups that clear rows
+
 int run_embed(const sp_embed_args *a) {
     hipStream_t stream = (hipStream_t)a->stream;
     return with_type(a->dtype, [&](auto tag) {
         using T = decltype(tag);
-        constexpr int N = VecOf<T>::N;
-        return with_group(group_of(a->dim, N), [&](auto gc) {
-            constexpr int G = decltype(gc)::value;
+        if (a->n_vocab == 0) {                                 // every id is outside
+            FillParams fill{};
+            fill.out = a->out; fill.n_rows = a->n_rows; fill.dim = a->dim; fill.ld = a->n_rows > 1 ? a->ld_out : a->dim; fill.bytes = (int)sizeof(T); fill.parts = 1;
+            hipLaunchKernelGGL(sp_fill_kernel<SORT_NT>, dim3(FILL_WGS), dim3(SORT_NT), 0, stream, fill);
+            HIP_TRY(hipGetLastError());
+            return (int)SP_OK;
+        }
+        return with_group<T>(a->dim, [&](auto gc, auto nc) {
+            constexpr int G = decltype(gc)::value, N = decltype(nc)::value;
             EmbedParams p = embed_params(a);
             p.slabs = (int)ceil_div(a->dim, G * N);
-            const i64 blocks = a->indptr ? ceil_div(a->n_rows * p.slabs, 4) : ceil_div(ceil_div(a->n_rows, LOOKUP_ROWS) * p.slabs, 256 / G);
+            const i64 blocks = a->indptr ? ceil_div(a->n_rows * p.slabs, 4) : ceil_div(a->n_rows * p.slabs, 256 / G);
             if (blocks > I32_MAX) return fail(SP_EINVAL, "too many rows for one launch");
             auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p); };
-            if (a->indptr) a->index64 ? launch(sp_embed_rows_kernel<T, i64, G>) : launch(sp_embed_rows_kernel<T, int, G>);
-            else a->index64 ? launch(sp_embed_lookup_kernel<T, i64, G>) : launch(sp_embed_lookup_kernel<T, int, G>);
+            if (a->indptr) a->index64 ? launch(sp_embed_rows_kernel<T, i64, G, N>) : launch(sp_embed_rows_kernel<T, int, G, N>);
+            else a->index64 ? launch(sp_embed_lookup_kernel<T, i64, G, N>) : launch(sp_embed_lookup_kernel<T, int, G, N>);
             HIP_TRY(hipGetLastError());
             return (int)SP_OK;
         });
@@ -124,7 +129,7 @@ int run_embed(const sp_embed_args *a) {
 
 // workspace of the gradient: two copies of the sorted entries (the passes alternate), the digit counts, the partial sums
 constexpr i64 REDUCE_CHUNKS = 4096;      // groups that sum sorted entries: about four waves per SIMD at one slab of 64 lanes
-constexpr int FILL_WGS = 512, SORT_WGS = 512;
+constexpr int SORT_WGS = 512;
 struct GradLayout {
     int wgs, sort_chunk, passes, bits, chunk;
     i64 chunks;
@@ -161,17 +166,17 @@ GradLayout grad_layout(const sp_embed_args *a) {
 
 template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a) {
     hipStream_t stream = (hipStream_t)a->stream;
-    constexpr int N = VecOf<T>::N;
     FillParams fill{};
     if (!a->accumulate) {
         fill.out = a->out;
         fill.n_rows = a->n_vocab; fill.dim = a->dim; fill.ld = a->n_vocab > 1 ? a->ld_out : a->dim; fill.bytes = (int)sizeof(TO);
     }
-    if (a->nnz == 0 && fill.out) {
+    const bool entries = a->nnz > 0 && a->n_rows > 0;         // (without rows every entry is in none)
+    if (!entries && fill.out) {
         fill.parts = 1;
         hipLaunchKernelGGL(sp_fill_kernel<SORT_NT>, dim3(FILL_WGS * 2), dim3(SORT_NT), 0, stream, fill);
     }
-    if (a->nnz > 0) {
+    if (entries) {
         const GradLayout L = grad_layout(a);
         unsigned char *ws = (unsigned char *)a->workspace;
         SortParams s{};
@@ -203,13 +208,13 @@ template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a)
         r.part = (float *)(ws + L.part);
         r.n = a->nnz; r.n_vocab = a->n_vocab; r.n_rows = a->n_rows; r.ld_in = a->ld_src; r.ld_out = a->ld_out;
         r.chunks = L.chunks; r.chunk = L.chunk; r.dim = (int)a->dim; r.accumulate = a->accumulate; r.scale = a->scale;
-        TRY(with_group(group_of(a->dim, N), [&](auto gc) {
-            constexpr int G = decltype(gc)::value;
+        TRY(with_group<T>(a->dim, [&](auto gc, auto nc) {
+            constexpr int G = decltype(gc)::value, N = decltype(nc)::value;
             r.slabs = (int)ceil_div(a->dim, G * N);
             const i64 blocks = ceil_div(L.chunks * r.slabs, 256 / G);
             if (L.chunks * r.slabs > I32_MAX) return fail(SP_EINVAL, "too many entries for one launch");
-            hipLaunchKernelGGL((sp_embed_reduce_kernel<T, TO, G>), dim3((unsigned)blocks), dim3(256), 0, stream, r);
-            if (L.chunks > 1) hipLaunchKernelGGL((sp_embed_join_kernel<TO, N, G>), dim3((unsigned)((L.chunks - 1) * r.slabs)), dim3(256), 0, stream, r);
+            hipLaunchKernelGGL((sp_embed_reduce_kernel<T, TO, G, N>), dim3((unsigned)blocks), dim3(256), 0, stream, r);
+            if (L.chunks > 1) hipLaunchKernelGGL((sp_embed_join_kernel<TO, G, N>), dim3((unsigned)((L.chunks - 1) * r.slabs)), dim3(256), 0, stream, r);
             return (int)SP_OK;
         }));
     }

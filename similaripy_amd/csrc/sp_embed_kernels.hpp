@@ -21,74 +21,50 @@ struct EmbedParams {
     int slabs;              // column slabs of a row: ceil(dim / (G * N))
 };
 
-// The columns of a lane: N of them from c on.  The last lane of a row moves back to the row's last N columns instead of taking fewer (it
-// repeats what the lane before it computes, to the same bits), so that every access is a whole vector; only rows shorter than N differ.
+// The columns of a lane: N of them from c on, of rows of at least N.  The last lane of a row moves back to the row's last N columns instead
+// of taking fewer (it repeats what the lane before it computes, to the same bits), and lanes beyond it read the same ones: every access is
+// a whole vector and none is behind a branch.  Rows shorter than a vector of 16 bytes are served with N = 1.
 template <int N> struct Columns {
     int own;           // first column that is this lane's alone
     int c;
-    bool active, whole;
-    __device__ __forceinline__ Columns(int first, int dim) : own(first), c(dim >= N && first > dim - N ? dim - N : first), active(first < dim), whole(dim >= N) {}
+    bool active;
+    __device__ __forceinline__ Columns(int first, int dim) : own(first), c(first > dim - N ? dim - N : first), active(first < dim) {}
 };
-template <typename T, int N> __device__ __forceinline__ RawVec<T, N> piece_load(const T *row, const Columns<N> &l, int dim) {
-    if (l.whole) return vec_load<T, N>(row + l.c);
-    RawVec<T, N> r;
-#pragma unroll
-    for (int j = 0; j < N; ++j) r.v[j] = j < dim ? row[j] : (T)0.f;
-    return r;
-}
-template <typename T, int N> __device__ __forceinline__ RawVec<T, N> piece_zero() {
-    RawVec<T, N> r;
-#pragma unroll
-    for (int j = 0; j < N; ++j) r.v[j] = (T)0.f;
-    return r;
-}
-template <typename T, int N> __device__ __forceinline__ void piece_store(T *row, const Columns<N> &l, int dim, const float *v) {
+template <typename T, int N> __device__ __forceinline__ void put(T *p, const float *v) {
     RawVec<T, N> o;
 #pragma unroll
     for (int j = 0; j < N; ++j) o.v[j] = (T)v[j];
-    if (l.whole) vec_store<T, N>(row + l.c, o);
-    else {
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (j < dim) row[j] = o.v[j];
-    }
+    vec_store<T, N>(p, o);
 }
 
 // value of lane `at` of the group of G lanes
 template <int G> __device__ __forceinline__ int group_lane(int v, int at) { return G == 64 ? __builtin_amdgcn_readlane(v, at) : __shfl(v, at, G); }
 
-constexpr int LOOKUP_ROWS = 1;       // rows of a group (16 k rows of 2 KB: 14.4 us with 1, 19 with 2, 20 with 4: more waves beat more loads per wave)
-// Lookup: one group of G lanes per LOOKUP_ROWS rows and slab of G * N columns.
-template <typename T, typename I, int G> __global__ __launch_bounds__(256) void sp_embed_lookup_kernel(EmbedParams p) {
-    constexpr int N = VecOf<T>::N, U = LOOKUP_ROWS;
+// Lookup: one group of G lanes per row and slab of G * N columns.  (16 k rows of 2 KB: 14.4 us with one row per group, 19 with two, 20 with
+// four: more waves beat more loads per wave.)
+template <typename T, typename I, int G, int N> __global__ __launch_bounds__(256) void sp_embed_lookup_kernel(EmbedParams p) {
     const int lane = threadIdx.x & (G - 1);
     const i64 item = (i64)blockIdx.x * (256 / G) + threadIdx.x / G;
-    const i64 row = item / p.slabs * U;
+    const i64 row = item / p.slabs;
     const Columns<N> cols(((int)(item % p.slabs) * G + lane) * N, p.dim);
     if (row >= p.n_rows || !cols.active) return;
-    RawVec<T, N> x[U];
-    i64 id[U];
+    const i64 id = (i64)((const I *)p.indices)[row];
+    float v[N];
+    if (id >= 0 && id < p.n_vocab) {
+        const RawVec<T, N> x = vec_load<T, N>((const T *)p.in + id * p.ld_in + cols.c);
 #pragma unroll
-    for (int u = 0; u < U; ++u) id[u] = row + u < p.n_rows ? (i64)((const I *)p.indices)[row + u] : -1;
+        for (int j = 0; j < N; ++j) v[j] = up(x.v[j]) * p.scale;
+    } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (id[u] >= 0 && id[u] < p.n_vocab) x[u] = piece_load<T, N>((const T *)p.in + id[u] * p.ld_in, cols, p.dim);
-        else x[u] = piece_zero<T, N>();
+        for (int j = 0; j < N; ++j) v[j] = 0.f;
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (row + u < p.n_rows) {
-            float v[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[j] = up(x[u].v[j]) * p.scale;
-            piece_store<T, N>((T *)p.out + (row + u) * p.ld_out, cols, p.dim, v);
-        }
+    put<T, N>((T *)p.out + row * p.ld_out + cols.c, v);
 }
 
 // Bags: one wave per row and slab.  Its 64 / G groups take the row's entries in turn; 64 ids and weights are read at once, a lane each, and
-// U rows of the table are on their way per group.
-template <typename T, typename I, int G> __global__ __launch_bounds__(256) void sp_embed_rows_kernel(EmbedParams p) {
-    constexpr int N = VecOf<T>::N, S = 64 / G, U = 8;
+// U rows of the table are on their way per group (an id outside the table reads row 0 and adds nothing).
+template <typename T, typename I, int G, int N> __global__ __launch_bounds__(256) void sp_embed_rows_kernel(EmbedParams p) {
+    constexpr int S = 64 / G, U = 8;
     static_assert(S * U <= 64, "a round stays inside the 64 entries read at once");
     const int lane = threadIdx.x & 63, sub = lane / G;
     const i64 item = (i64)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -111,22 +87,20 @@ template <typename T, typename I, int G> __global__ __launch_bounds__(256) void 
         }
         for (int j = 0; j < n; j += S * U) {
             RawVec<T, N> x[U];
-            float w[U];
+            int id[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int at = j + u * S + sub;
-                const int id = S == 1 ? __builtin_amdgcn_readlane(mine, j + u) : __shfl(mine, at, 64);
-                w[u] = __int_as_float(S == 1 ? __builtin_amdgcn_readlane(__float_as_int(weight), j + u) : __shfl(__float_as_int(weight), at, 64));
-                if (id >= 0 && cols.active) x[u] = piece_load<T, N>((const T *)p.in + (i64)id * p.ld_in, cols, p.dim);
-                else {
-                    x[u] = piece_zero<T, N>();
-                    w[u] = 0.f;
-                }
+                id[u] = S == 1 ? __builtin_amdgcn_readlane(mine, j + u) : __shfl(mine, j + u * S + sub, 64);
+                x[u] = vec_load<T, N>((const T *)p.in + (i64)max(id[u], 0) * p.ld_in + cols.c);
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                const float w = __int_as_float(S == 1 ? __builtin_amdgcn_readlane(__float_as_int(weight), j + u) : __shfl(__float_as_int(weight), j + u * S + sub, 64));
+                if (id[u] >= 0) {
 #pragma unroll
-                for (int k = 0; k < N; ++k) acc[k] = __fmaf_rn(w[u], up(x[u].v[k]), acc[k]);
+                    for (int k = 0; k < N; ++k) acc[k] = __fmaf_rn(w, up(x[u].v[k]), acc[k]);
+                }
+            }
         }
     }
 #pragma unroll
@@ -136,7 +110,7 @@ template <typename T, typename I, int G> __global__ __launch_bounds__(256) void 
     if (sub == 0 && cols.active) {
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[k] *= p.scale;
-        piece_store<T, N>((T *)p.out + row * p.ld_out, cols, p.dim, acc);
+        put<T, N>((T *)p.out + row * p.ld_out + cols.c, acc);
     }
 }
 
@@ -358,27 +332,29 @@ struct ReduceParams {
 };
 
 template <typename TO, int N> __device__ __forceinline__ void write_row(const ReduceParams &p, unsigned key, const Columns<N> &cols, float *acc) {
-    TO *row = (TO *)p.out + (i64)key * p.ld_out;
+    TO *row = (TO *)p.out + (i64)key * p.ld_out + cols.c;
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] *= p.scale;
-    if (p.accumulate && (cols.c != cols.own || !cols.whole)) {       // (columns that another lane writes as well are added to once)
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (cols.c + j >= cols.own && cols.c + j < p.dim) row[cols.c + j] = (TO)(acc[j] + up(row[cols.c + j]));
-        return;
-    }
     if (p.accumulate) {
-        const RawVec<TO, N> was = vec_load<TO, N>(row + cols.c);
+        if (cols.c != cols.own) {                              // (columns that another lane writes as well are added to once, by that lane)
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (cols.c + j >= cols.own) row[j] = (TO)(acc[j] + up(row[j]));
+            return;
+        }
+        const RawVec<TO, N> was = vec_load<TO, N>(row);
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] += up(was.v[j]);
     }
-    piece_store<TO, N>(row, cols, p.dim, acc);
+    put<TO, N>(row, acc);
 }
+
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }      // vmcnt(0)
 
 // One group of G lanes per chunk of the sorted entries and slab of columns: runs of equal ids are summed as they come.  A run that
 // lies inside the chunk is a row of the gradient and is written; one that began before or goes on behind it leaves its sum in `part`.
-template <typename T, typename TO, int G> __global__ __launch_bounds__(256) void sp_embed_reduce_kernel(ReduceParams p) {
-    constexpr int N = VecOf<T>::N, U = 8;
+template <typename T, typename TO, int G, int N> __global__ __launch_bounds__(256) void sp_embed_reduce_kernel(ReduceParams p) {
+    constexpr int U = 8;
     const int lane = threadIdx.x & (G - 1);
     i64 item = (i64)blockIdx.x * (256 / G) + threadIdx.x / G;
     if (G == 64) item = (i64)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -386,61 +362,56 @@ template <typename T, typename TO, int G> __global__ __launch_bounds__(256) void
     if (ch >= p.chunks) return;
     const Columns<N> cols(((int)(item % p.slabs) * G + lane) * N, p.dim);
     const i64 b = ch * p.chunk, e = min(p.n, b + p.chunk);
-    const unsigned none = (unsigned)p.n_vocab;
-    const unsigned prev = b > 0 ? p.key[b - 1] : none, next = e < p.n ? p.key[e] : none;
-    unsigned run = p.key[b];
+    const int none = (int)p.n_vocab;
+    const int prev = b > 0 ? (int)p.key[b - 1] : none, next = e < p.n ? (int)p.key[e] : none;
+    int run = group_lane<G>((int)p.key[b], 0);
     bool head = b > 0 && run == prev;
     float acc[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
     auto flush = [&](bool last) {
         if (run == none || !cols.active) return;
-        float *slot = nullptr;
-        if (head) slot = p.part + (2 * ch) * p.dim;
-        else if (last && e < p.n && next == run) slot = p.part + (2 * ch + 1) * p.dim;
-        if (slot) piece_store<float, N>(slot, cols, p.dim, acc);
-        else write_row<TO, N>(p, run, cols, acc);
+        const bool tail = last && next == run;                 // (next is `none` behind the last entry)
+        if (head || tail) put<float, N>(p.part + (2 * ch + (head ? 0 : 1)) * p.dim + cols.c, acc);
+        else write_row<TO, N>(p, (unsigned)run, cols, acc);
     };
     for (i64 i = b; i < e; i += G) {                           // G entries at once, a lane each
         const int n = (int)min((i64)G, e - i);
-        int key = (int)none, from = -1;
+        int key = none, from = -1;
         float weight = 0.f;
         if (lane < n) {
             key = (int)p.key[i + lane];
             const unsigned r = p.pay[i + lane];
-            if ((i64)r < p.n_rows) {
-                from = (int)r;
-                weight = p.w ? p.w[i + lane] : 1.f;
-            }
+            from = key != none && (i64)r < p.n_rows ? (int)r : -1;
+            weight = p.w ? p.w[i + lane] : 1.f;
         }
-        if (key == (int)none) from = -1;
         for (int j = 0; j < n; j += U) {
             RawVec<T, N> x[U];
-            float w[U];
-            unsigned k[U];
+            int r[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                k[u] = (unsigned)group_lane<G>(key, j + u);
-                const int r = group_lane<G>(from, j + u);
-                w[u] = __int_as_float(group_lane<G>(__float_as_int(weight), j + u));
-                if (r >= 0 && cols.active) x[u] = piece_load<T, N>((const T *)p.in + (i64)r * p.ld_in, cols, p.dim);
-                else {
-                    x[u] = piece_zero<T, N>();
-                    w[u] = 0.f;
-                }
+                r[u] = group_lane<G>(from, j + u);
+                x[u] = vec_load<T, N>((const T *)p.in + (i64)max(r[u], 0) * p.ld_in + cols.c);
             }
+            // Loads and stores of a wave are counted together: once a row has been written behind a branch, waiting for a load that is still
+            // on its way means waiting for the store as well.  So all rows of the batch are waited for here.
+            loads_done();
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (j + u >= n) break;
-                if (k[u] != run) {
+                const int k = group_lane<G>(key, j + u);
+                if (k != run) {
                     flush(false);
-                    run = k[u];
+                    run = k;
                     head = false;
 #pragma unroll
                     for (int q = 0; q < N; ++q) acc[q] = 0.f;
                 }
+                if (r[u] >= 0) {
+                    const float w = __int_as_float(group_lane<G>(__float_as_int(weight), j + u));
 #pragma unroll
-                for (int q = 0; q < N; ++q) acc[q] = __fmaf_rn(w[u], up(x[u].v[q]), acc[q]);
+                    for (int q = 0; q < N; ++q) acc[q] = __fmaf_rn(w, up(x[u].v[q]), acc[q]);
+                }
             }
         }
     }
@@ -449,7 +420,7 @@ template <typename T, typename TO, int G> __global__ __launch_bounds__(256) void
 
 // Runs over several chunks: the workgroup of the chunk in which a run begins adds up its parts and writes the row.  All threads look how
 // far the run goes, 256 chunks at once; the 256 / G groups then sum contiguous shares of the parts, which are joined in their order.
-template <typename TO, int N, int G> __global__ __launch_bounds__(256) void sp_embed_join_kernel(ReduceParams p) {
+template <typename TO, int G, int N> __global__ __launch_bounds__(256) void sp_embed_join_kernel(ReduceParams p) {
     constexpr int GROUPS = 256 / G, U = 8;
     __shared__ float sums[GROUPS][G * N];
     __shared__ int ends;
@@ -480,22 +451,23 @@ template <typename TO, int N, int G> __global__ __launch_bounds__(256) void sp_e
     float acc[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
-    if (cols.active) {
+    {
         for (i64 k = k0; k < k1; k += U) {
             RawVec<float, N> x[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) x[u] = k + u < k1 ? piece_load<float, N>(p.part + (2 * (k + u)) * p.dim, cols, p.dim) : piece_zero<float, N>();
+            for (int u = 0; u < U; ++u) x[u] = vec_load<float, N>(p.part + (2 * min(k + u, k1 - 1)) * p.dim + cols.c);
 #pragma unroll
             for (int u = 0; u < U; ++u)
+                if (k + u < k1)
 #pragma unroll
-                for (int j = 0; j < N; ++j) acc[j] += x[u].v[j];
+                    for (int j = 0; j < N; ++j) acc[j] += x[u].v[j];
         }
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) sums[g][lane * N + j] = acc[j];
     __syncthreads();
     if (g != 0 || !cols.active) return;
-    const RawVec<float, N> x = piece_load<float, N>(p.part + (2 * ch + 1) * p.dim, cols, p.dim);
+    const RawVec<float, N> x = vec_load<float, N>(p.part + (2 * ch + 1) * p.dim + cols.c);
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = x.v[j];
     const int parts = (int)min((i64)GROUPS, (count + share - 1) / share);

@@ -157,6 +157,8 @@ def test_embed_rows_outside_indptr_are_not_read():
     assert dense.embed_rows(table, ids, indptr)[:, 0].tolist() == [3.0, 0.0, 2.0]
     g = dense.embed_rows_grad(torch.tensor([[1.0], [10.0], [100.0]], device="cuda").repeat(1, 8), ids, 4, indptr)
     assert g[0, 0].item() == 203.0 and (g[1:] == 0).all()
+    nobody = torch.zeros(1, dtype=torch.int32, device="cuda")                    # no rows at all, though there are entries
+    assert (dense.embed_rows_grad(torch.ones(0, 8, device="cuda"), ids, 4, nobody) == 0).all() and dense.embed_rows(table, ids, nobody).shape == (0, 8)
     indptr = torch.tensor([2, 4], dtype=torch.int32, device="cuda")              # entries before the first row and behind the last belong to none
     assert dense.embed_rows(table, ids, indptr)[0, 0].item() == 2.0
     assert dense.embed_rows_grad(torch.ones(1, 8, device="cuda"), ids, 4, indptr)[0, 0].item() == 2.0
