@@ -132,6 +132,7 @@ constexpr i64 REDUCE_CHUNKS = 4096;      // groups that sum sorted entries: abou
 constexpr int SORT_WGS = 512;
 struct GradLayout {
     int wgs, sort_chunk, passes, bits, chunk;
+    bool small;                                                  // sorted by one workgroup
     i64 chunks;
     size_t key[2], pay[2], w[2], rows, hist, digits, part, total;
 };
@@ -144,6 +145,7 @@ GradLayout grad_layout(const sp_embed_args *a) {
     L.wgs = (int)ceil_div(n, L.sort_chunk);
     int kb = 1;                                                  // bits of the keys 0 .. n_vocab
     while (kb < 31 && (1ll << kb) <= a->n_vocab) ++kb;
+    L.small = n <= SMALL_MAX && kb + SMALL_INDEX_BITS <= 32;
     L.passes = (kb + 8) / 9;
     L.bits = (kb + L.passes - 1) / L.passes;
     const i64 per = ceil_div(n, REDUCE_CHUNKS);
@@ -188,7 +190,17 @@ template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a)
         s.fill = fill;
         s.fill.parts = 2 * L.passes;
         s.entry_row = a->indptr ? (unsigned *)(ws + L.rows) : nullptr;
-        for (int pass = 0; pass < L.passes; ++pass) {
+        if (L.small) {
+            s.fill.parts = 1;
+            s.key_out = (unsigned *)(ws + L.key[0]);
+            s.pay_out = (unsigned *)(ws + L.pay[0]);
+            s.w_out = a->data ? (float *)(ws + L.w[0]) : nullptr;
+            const dim3 grid(1 + (fill.out ? FILL_WGS : 0));
+            if (a->index64) hipLaunchKernelGGL(sp_sort_small_kernel<i64>, grid, dim3(SMALL_NT), 0, stream, s, L.passes);
+            else hipLaunchKernelGGL(sp_sort_small_kernel<int>, grid, dim3(SMALL_NT), 0, stream, s, L.passes);
+            s.key_in = s.key_out; s.pay_in = s.pay_out; s.w_in = s.w_out;
+        }
+        for (int pass = 0; pass < (L.small ? 0 : L.passes); ++pass) {
             const int to = pass & 1;
             s.shift = pass * L.bits;
             s.key_out = (unsigned *)(ws + L.key[to]);

@@ -319,6 +319,107 @@ template <typename I> __global__ __launch_bounds__(SORT_NT) void sp_sort_move_ke
     }
 }
 
+// the CSR row of entry i; n_rows for an entry that no row holds
+template <typename I> __device__ __forceinline__ i64 row_of(const void *indptr, i64 n_rows, i64 i) {
+    i64 lo = 0, hi = n_rows;                                   // first r with indptr[r + 1] > i
+    while (lo < hi) {
+        const i64 mid = (lo + hi) >> 1;
+        if ((i64)((const I *)indptr)[mid + 1] > i) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo < n_rows && (i64)((const I *)indptr)[lo] > i ? n_rows : lo;
+}
+
+// Up to 8192 entries are sorted by one workgroup, in one launch, while the others clear the gradient: an entry is its key and its index
+// in one word, 8 words per thread in registers, moved through LDS once per pass.  Gradient of n lookups into 84 433 rows of 1024 bf16, this
+// way / by the launches above: n = 64 33 / 41 us, 1024 35 / 47, 4096 36 / 48, 8192 41 / 50, 16 384 82 / 55; into 2000 rows, where there is
+// little to clear beside it: 1024 19 / 28, 4096 26 / 30, 8192 37 / 33.
+constexpr int SMALL_NT = 1024, SMALL_WAVES = SMALL_NT / 64, SMALL_PER = 8, SMALL_MAX = SMALL_NT * SMALL_PER, SMALL_INDEX_BITS = 13;
+static_assert(SMALL_MAX == 1 << SMALL_INDEX_BITS, "an index fits its bits");
+
+template <typename I> __global__ __launch_bounds__(SMALL_NT) void sp_sort_small_kernel(SortParams p, int passes) {
+    __shared__ unsigned buf[SMALL_MAX];
+    __shared__ unsigned off[SMALL_WAVES][SORT_BINS];
+    __shared__ unsigned wsum[SORT_BINS / 64];
+    if (blockIdx.x > 0) {
+        if (p.fill.out) fill_share(p.fill, blockIdx.x - 1, gridDim.x - 1);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = (int)p.n;
+    const int rounds = (n + SMALL_NT - 1) / SMALL_NT, first = wave * rounds * 64 + lane;      // a wave's entries are consecutive
+    const unsigned mask = (1u << p.bits) - 1u;
+    unsigned v[SMALL_PER];
+#pragma unroll
+    for (int q = 0; q < SMALL_PER; ++q) {
+        const int i = first + q * 64;
+        if (q < rounds && i < n) v[q] = sort_key<I>(p, i) << SMALL_INDEX_BITS | (unsigned)i;
+    }
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = SMALL_INDEX_BITS + pass * p.bits;
+        for (int i = tid; i < SMALL_WAVES * SORT_BINS; i += SMALL_NT) (&off[0][0])[i] = 0u;
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < SMALL_PER; ++q)
+            if (q < rounds && first + q * 64 < n) atomicAdd(&off[wave][(v[q] >> shift) & mask], 1u);
+        __syncthreads();
+        unsigned inc = 0, all = 0;
+        if (tid < SORT_BINS) {                                 // a thread per digit: entries of smaller digits, then of the waves before
+            for (int w = 0; w < SMALL_WAVES; ++w) all += off[w][tid];
+            inc = all;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const unsigned o = __shfl_up(inc, d, 64);
+                if (lane >= d) inc += o;
+            }
+            if (lane == 63) wsum[wave] = inc;
+        }
+        __syncthreads();
+        if (tid < SORT_BINS) {
+            unsigned base = inc - all;
+            for (int w = 0; w < wave; ++w) base += wsum[w];
+            for (int w = 0; w < SMALL_WAVES; ++w) {
+                const unsigned c = off[w][tid];
+                off[w][tid] = base;
+                base += c;
+            }
+        }
+        __syncthreads();
+        volatile unsigned *mine = off[wave];
+#pragma unroll
+        for (int q = 0; q < SMALL_PER; ++q) {
+            if (q >= rounds) break;
+            const bool ok = first + q * 64 < n;
+            const unsigned digit = ok ? (v[q] >> shift) & mask : 0u;
+            u64 same = __ballot(ok);
+            for (int k = 0; k < p.bits; ++k) {
+                const u64 set = __ballot((digit >> k) & 1u);
+                same &= (digit >> k) & 1u ? set : ~set;
+            }
+            if (ok) {
+                const unsigned rank = (unsigned)__popcll(same & ((1ull << lane) - 1ull));
+                const unsigned at = mine[digit] + rank;
+                if (rank == 0) mine[digit] = at + (unsigned)__popcll(same);       // (as in the launches above)
+                buf[at] = v[q];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < SMALL_PER; ++q)
+            if (q < rounds && first + q * 64 < n) v[q] = buf[first + q * 64];
+        __syncthreads();
+    }
+#pragma unroll
+    for (int q = 0; q < SMALL_PER; ++q) {
+        const int i = first + q * 64;
+        if (q < rounds && i < n) {
+            const unsigned from = v[q] & (SMALL_MAX - 1);
+            p.key_out[i] = v[q] >> SMALL_INDEX_BITS;
+            p.pay_out[i] = p.indptr ? (unsigned)row_of<I>(p.indptr, p.n_rows, from) : from;
+            if (p.w_out) p.w_out[i] = p.w_in[from];
+        }
+    }
+}
+
 struct ReduceParams {
     const void *in;
     void *out;
