@@ -307,6 +307,7 @@ DistillParams distill_params(const sp_distill_args *a) {
 }
 
 constexpr i64 SCAN_WGS = 1024, GRAD_WGS = 2048;
+constexpr i64 LDS_BYTES = 163840;   // of a CU
 constexpr i64 FUSED_ROWS = 256;      // from as many rows on a workgroup per row fills the card
 
 int launch_scan(const sp_distill_args *a, DistillParams p, hipStream_t stream) {
@@ -448,9 +449,19 @@ int sp_distill_loss_grad(const sp_distill_args *a) {
     }
     return with_type(a->dtype, [&](auto tag) {
         using T = decltype(tag);
-        hipLaunchKernelGGL((sp_distill_loss_grad_kernel<T, DI_NT>), dim3((unsigned)a->n_rows), dim3(DI_NT), (size_t)a->k * 12, stream, p);
-        HIP_TRY(hipGetLastError());
-        return (int)SP_OK;
+        // the row in registers and LDS: by two workgroups of 512 threads per CU if it fits half of them, else by one of 1024
+        const i64 vecs = a->n_cols / VecOf<T>::N, lists = ((i64)a->k * 12 + 15) / 16 * 16;
+        const i64 half = (LDS_BYTES / 2 - lists - 1024) / 16;
+        auto launch = [&](auto kernel, int nt, i64 stage) {
+            p.stage = (int)(vecs - (i64)ROW_VECS * nt < 0 ? 0 : vecs - (i64)ROW_VECS * nt < stage ? vecs - (i64)ROW_VECS * nt : stage);
+            const size_t lds = (size_t)(lists + (i64)p.stage * 16);
+            HIP_TRY(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+            hipLaunchKernelGGL(kernel, dim3((unsigned)a->n_rows), dim3(nt), lds, stream, p);
+            HIP_TRY(hipGetLastError());
+            return (int)SP_OK;
+        };
+        if (vecs <= (i64)ROW_VECS * 512 + half) return launch(sp_distill_loss_grad_kernel<T, 512>, 512, half);
+        return launch(sp_distill_loss_grad_kernel<T, 1024>, 1024, (LDS_BYTES - lists - 1024) / 16);
     });
 }
 

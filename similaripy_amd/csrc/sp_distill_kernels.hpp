@@ -27,6 +27,7 @@ struct DistillParams {
     int splits;                        // workgroups of a row
     i64 chunk;                         // columns of one of them (a multiple of the vector)
     float *part;                       // [n_rows, splits, 2] maximum, sum
+    int stage;                         // vectors of a row that the one-call kernel keeps in LDS
 };
 
 // maximum and sum of exp2((z - max) c) of some columns
@@ -66,9 +67,10 @@ template <int NT> __device__ __forceinline__ MaxSum block_join(MaxSum a, float c
     a = wave_join(a, c);
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
     __syncthreads();
-    a = sh[0];
+    constexpr int W = NT / 64;
+    a = sh[threadIdx.x & (W - 1)];
 #pragma unroll
-    for (int w = 1; w < NT / 64; ++w) a = join(a, sh[w], c);
+    for (int d = W / 2; d > 0; d >>= 1) a = join(a, MaxSum{__shfl_xor(a.m, d, 64), __shfl_xor(a.s, d, 64)}, c);
     return a;
 }
 
@@ -85,6 +87,11 @@ template <int N> __device__ __forceinline__ void add_vec(Running &a, const float
 #pragma unroll
     for (int j = 0; j < N; ++j) s += exp2_fast(__fmaf_rn(z[j], c, -off));
     a = {m, off, s};
+}
+
+// (a maximum whose m c leaves float32 has no sum here: it is nothing next to a larger one, and the row is summed again otherwise)
+__device__ __forceinline__ MaxSum finish(const Running &a, float c) {
+    return {a.m, a.m == NEG_INF || !off_fits(a.m, c) ? (a.s != a.s ? a.s : 0.f) : a.s * exp2_fast(-__fmaf_rn(a.m, c, -a.off))};
 }
 
 // maximum and sum over columns [c0, c1) of a row, by the NT threads of the workgroup (each its share)
@@ -115,20 +122,21 @@ template <typename T, int NT> __device__ __forceinline__ MaxSum thread_columns(c
             const float v = up(z[i + j]);
             add_vec<1>(a, &v, c);
         }
-    // (a maximum whose m c leaves float32 has no sum here: it is nothing next to a larger one, and scan_columns sums again otherwise)
-    return {a.m, a.m == NEG_INF || !off_fits(a.m, c) ? (a.s != a.s ? a.s : 0.f) : a.s * exp2_fast(-__fmaf_rn(a.m, c, -a.off))};
+    return finish(a, c);
 }
 
-// the same for the workgroup: the result is everybody's
+// columns summed once more, with an exponent that fits; a.m is their maximum
+template <typename T, int NT> __device__ __forceinline__ MaxSum rescan(const T *z, i64 c0, i64 c1, MaxSum a, float c, MaxSum *sh) {
+    const Exponent x = exponent_of(a.m, c);
+    a.s = 0.f;
+    for (i64 i = c0 + threadIdx.x; i < c1; i += NT) a.s += exp2_fast(__fmaf_rn(up(z[i]), x.c, -x.off));
+    __syncthreads();
+    return block_join<NT>(a, c, sh);
+}
+// thread_columns for the workgroup: the result is everybody's
 template <typename T, int NT> __device__ __forceinline__ MaxSum scan_columns(const T *z, i64 c0, i64 c1, float c, MaxSum *sh) {
     MaxSum a = block_join<NT>(thread_columns<T, NT>(z, c0, c1, c), c, sh);
-    if (!off_fits(a.m, c)) {                                    // (uniform) summed once more, with an exponent that fits
-        const Exponent x = exponent_of(a.m, c);
-        a.s = 0.f;
-        for (i64 i = c0 + threadIdx.x; i < c1; i += NT) a.s += exp2_fast(__fmaf_rn(up(z[i]), x.c, -x.off));
-        __syncthreads();
-        a = block_join<NT>(a, c, sh);
-    }
+    if (!off_fits(a.m, c)) a = rescan<T, NT>(z, c0, c1, a, c, sh);      // (uniform)
     return a;
 }
 
@@ -224,9 +232,26 @@ __device__ __forceinline__ MaxSum join_parts(const DistillParams &p, i64 row) {
 // rows in several pieces: one wave joins them
 template <typename T> __global__ __launch_bounds__(64) void sp_distill_join_kernel(DistillParams p) { finish_loss<T>(p, blockIdx.x, join_parts(p, blockIdx.x)); }
 
+// the listed columns of [c0, c1) once more, with their probabilities taken off; a column listed several times is written by its first entry
+template <typename T, int NT, typename F>
+__device__ __forceinline__ void write_listed(const DistillParams &p, T *d, i64 c0, i64 c1, F one, float gt, const int *scol, const float *sprob, const float *sz) {
+    for (int j = threadIdx.x; j < p.k; j += NT) {
+        const int c = scol[j];
+        if (c < c0 || c >= c1) continue;
+        float prob = 0.f;
+        bool first = true;
+        for (int i = 0; i < p.k; ++i)
+            if (scol[i] == c) {
+                first = first && i >= j;
+                prob += sprob[i];
+            }
+        if (first) d[c] = (T)(one(sz[j]) - gt * prob);
+    }
+}
+
 // The gradient of columns [c0, c1) of a row by the NT threads of a workgroup: g tau P q everywhere, then the listed columns once
 // more with their probabilities taken off.  scol / sprob hold the list; sz [k] is scratch: the listed scores are kept before
-// anything is written, so `grad` may be `student`.  A column listed several times is written by its first entry.  A row whose list
+// anything is written, so `grad` may be `student`.  A row whose list
 // has no mass gets zeros, whatever its scores hold (a padded row of a batch).
 template <typename T, int NT>
 __device__ __forceinline__ void grad_columns(const DistillParams &p, i64 row, i64 c0, i64 c1, MaxSum a, float mass, float gt, const int *scol, const float *sprob, float *sz) {
@@ -275,18 +300,7 @@ __device__ __forceinline__ void grad_columns(const DistillParams &p, i64 row, i6
     for (int j = 0; j < N; ++j)
         if (i + j < c1) d[i + j] = (T)one(up(z[i + j]));
     __syncthreads();
-    for (int j = tid; j < p.k; j += NT) {
-        const int c = scol[j];
-        if (c < c0 || c >= c1) continue;
-        float prob = 0.f;
-        bool first = true;
-        for (int i2 = 0; i2 < p.k; ++i2)
-            if (scol[i2] == c) {
-                first = first && i2 >= j;
-                prob += sprob[i2];
-            }
-        if (first) d[c] = (T)(one(sz[j]) - gt * prob);
-    }
+    write_listed<T, NT>(p, d, c0, c1, one, gt, scol, sprob, sz);
 }
 
 extern __shared__ int distill_list[];      // [k] columns, [k] probabilities, [k] scores
@@ -306,25 +320,98 @@ template <typename T, int NT> __global__ __launch_bounds__(NT) void sp_distill_g
     grad_columns<T, NT>(p, row, c0, c1, a, mass, gt, scol, sprob, sz);
 }
 
-// loss and gradient of a row by one workgroup: the second reading of the row finds it in the caches
-template <typename T, int NT> __global__ __launch_bounds__(NT) void sp_distill_loss_grad_kernel(DistillParams p) {
+// what the compiler has derived from a vector is to be derived again
+template <typename T, int N> __device__ __forceinline__ void forget(RawVec<T, N> &x) {
+    typedef unsigned Quad __attribute__((ext_vector_type(4)));
+    Quad q;
+    __builtin_memcpy(&q, &x, 16);
+    asm volatile("" : "+v"(q));
+    __builtin_memcpy(&x, &q, 16);
+}
+
+// Loss and gradient of a row by one workgroup that keeps the row: ROW_VECS vectors of 16 bytes per thread in registers, `stage` more per
+// workgroup in LDS; only what is left of a still longer row is read a second time.  The sums are formed while vectors arrive, the gradient
+// while they leave; two workgroups of 512 threads share a CU where the row allows it, so that one loads while the other stores.
+constexpr int ROW_VECS = 16;
+template <typename T, int NT> __global__ __launch_bounds__(NT, 4) void sp_distill_loss_grad_kernel(DistillParams p) {
+    constexpr int N = VecOf<T>::N, M = 16 / N;                 // M vectors, 16 scores, are added at once
     __shared__ MaxSum sh[NT / 64];
-    __shared__ float mass;
+    __shared__ float mass_of_row;
     int *scol = distill_list;
     float *sprob = (float *)(distill_list + p.k), *sz = sprob + p.k;
+    RawVec<T, N> *stage = (RawVec<T, N> *)(distill_list + (3 * p.k + 3) / 4 * 4);
     const i64 row = blockIdx.x;
+    const int tid = threadIdx.x, n_cols = (int)p.n_cols, vecs = n_cols / N;
+    const int kept = min(vecs, ROW_VECS * NT + p.stage);       // vectors that are not read again
     const T *z = (const T *)p.student + row * p.ld_student;
-    const MaxSum a = scan_columns<T, NT>(z, 0, p.n_cols, p.c, sh);
-    if (threadIdx.x < 64) {
+    T *d = (T *)p.grad + row * p.ld_grad;
+
+    RawVec<T, N> x[ROW_VECS];
+#pragma unroll
+    for (int q = 0; q < ROW_VECS; ++q) {
+        const int j = q * NT + tid;
+        if (j < vecs) x[q] = vec_load<T, N>(z + (i64)j * N);
+        else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[q].v[e] = (T)NEG_INF;          // (adds nothing)
+        }
+    }
+    Running run{NEG_INF, NEG_INF, 0.f};
+    for (int j = ROW_VECS * NT + tid; j < vecs; j += NT) {
+        const RawVec<T, N> y = vec_load<T, N>(z + (i64)j * N);
+        if (j < kept) stage[j - ROW_VECS * NT] = y;
+        float v[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = up(y.v[e]);
+        add_vec<N>(run, v, p.c);
+    }
+    const int end = vecs * N + tid;                            // fewer than N columns behind the last vector
+    const float lone = end < n_cols ? up(z[end]) : NEG_INF;
+    add_vec<1>(run, &lone, p.c);
+#pragma unroll
+    for (int q = 0; q < ROW_VECS; q += M) {
+        if (q * NT >= vecs) break;
+        float v[16];
+#pragma unroll
+        for (int u = 0; u < M; ++u)
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[u * N + e] = up(x[q + u].v[e]);
+        add_vec<16>(run, v, p.c);
+    }
+    MaxSum a = block_join<NT>(finish(run, p.c), p.c, sh);
+    if (!off_fits(a.m, p.c)) a = rescan<T, NT>(z, 0, n_cols, a, p.c, sh);
+    if (tid < 64) {
         const ListSums l = list_sums<T, true>(p, row, z, a, scol, sprob);
-        if (threadIdx.x == 0) {
-            mass = l.mass;
+        if (tid == 0) {
+            mass_of_row = l.mass;
             if (p.loss) p.loss[row] = p.tau * p.tau * l.loss;
         }
     }
-    const float gt = (p.grad_loss ? p.grad_loss[row] : 1.f) * p.tau;
     __syncthreads();
-    grad_columns<T, NT>(p, row, 0, p.n_cols, a, mass, gt, scol, sprob, sz);
+#pragma unroll
+    for (int q = 0; q < ROW_VECS; ++q) forget(x[q]);           // (or the scores stay unpacked in registers, which there are not enough of)
+    const float mass = mass_of_row, gt = (p.grad_loss ? p.grad_loss[row] : 1.f) * p.tau;
+    for (int j = tid; j < p.k; j += NT) sz[j] = scol[j] >= 0 ? up(z[scol[j]]) : 0.f;
+    __syncthreads();                                           // (from here on `grad` is written, which may be `student`)
+    const Exponent ex = exponent_of(a.m, p.c);
+    const bool some = mass != 0.f;                             // (a row whose list has no mass gets zeros, whatever its scores hold)
+    const float coef = a.s == 0.f || !some ? 0.f : gt * mass / a.s * correction_of(a.m, ex);
+    auto one = [&](float v) { return some ? coef * exp2_fast(__fmaf_rn(v, ex.c, -ex.off)) : 0.f; };
+    auto put = [&](int j, const RawVec<T, N> &y) {
+        RawVec<T, N> o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o.v[e] = (T)one(up(y.v[e]));
+        vec_store<T, N>(d + (i64)j * N, o);
+    };
+    // (what has to be read again goes first: nothing of it has been written yet)
+    for (int j = kept + tid; j < vecs; j += NT) put(j, vec_load<T, N>(z + (i64)j * N));
+#pragma unroll
+    for (int q = 0; q < ROW_VECS; ++q)
+        if (q * NT + tid < vecs) put(q * NT + tid, x[q]);
+    for (int j = ROW_VECS * NT + tid; j < kept; j += NT) put(j, stage[j - ROW_VECS * NT]);
+    if (end < n_cols) d[end] = (T)one(lone);
+    __syncthreads();
+    write_listed<T, NT>(p, d, 0, n_cols, one, gt, scol, sprob, sz);
 }
 
 }  // namespace
