@@ -306,6 +306,8 @@ DistillParams distill_params(const sp_distill_args *a) {
     return p;
 }
 
+size_t list_bytes(const sp_distill_args *a) { return (size_t)ListLds::list_room(a->k) * 16; }
+
 constexpr i64 SCAN_WGS = 1024, GRAD_WGS = 2048;
 constexpr i64 LDS_BYTES = 163840;   // of a CU
 constexpr i64 FUSED_ROWS = 256;      // from as many rows on a workgroup per row fills the card
@@ -313,10 +315,13 @@ constexpr i64 FUSED_ROWS = 256;      // from as many rows on a workgroup per row
 int launch_scan(const sp_distill_args *a, DistillParams p, hipStream_t stream) {
     p.splits = splits_of(a, SCAN_WGS);
     p.chunk = chunk_of(a, p.splits);
+    const size_t lists = list_bytes(a);
     return with_type(a->dtype, [&](auto tag) {
         using T = decltype(tag);
-        hipLaunchKernelGGL((sp_distill_scan_kernel<T, DI_NT>), dim3((unsigned)(a->n_rows * p.splits)), dim3(DI_NT), 0, stream, p);
-        if (p.splits > 1) hipLaunchKernelGGL((sp_distill_join_kernel<T>), dim3((unsigned)a->n_rows), dim3(64), 0, stream, p);
+        HIP_TRY(hipFuncSetAttribute((const void *)sp_distill_scan_kernel<T, DI_NT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lists));
+        HIP_TRY(hipFuncSetAttribute((const void *)sp_distill_join_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lists));
+        hipLaunchKernelGGL((sp_distill_scan_kernel<T, DI_NT>), dim3((unsigned)(a->n_rows * p.splits)), dim3(DI_NT), lists, stream, p);
+        if (p.splits > 1) hipLaunchKernelGGL((sp_distill_join_kernel<T>), dim3((unsigned)a->n_rows), dim3(64), lists, stream, p);
         HIP_TRY(hipGetLastError());
         return (int)SP_OK;
     });
@@ -326,7 +331,9 @@ int launch_grad(const sp_distill_args *a, DistillParams p, hipStream_t stream) {
     p.chunk = chunk_of(a, p.splits);
     return with_type(a->dtype, [&](auto tag) {
         using T = decltype(tag);
-        hipLaunchKernelGGL((sp_distill_grad_kernel<T, DI_NT>), dim3((unsigned)(a->n_rows * p.splits)), dim3(DI_NT), (size_t)a->k * 12, stream, p);
+        const size_t lists = list_bytes(a);
+        HIP_TRY(hipFuncSetAttribute((const void *)sp_distill_grad_kernel<T, DI_NT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lists));
+        hipLaunchKernelGGL((sp_distill_grad_kernel<T, DI_NT>), dim3((unsigned)(a->n_rows * p.splits)), dim3(DI_NT), lists, stream, p);
         HIP_TRY(hipGetLastError());
         return (int)SP_OK;
     });
@@ -449,19 +456,23 @@ int sp_distill_loss_grad(const sp_distill_args *a) {
     }
     return with_type(a->dtype, [&](auto tag) {
         using T = decltype(tag);
-        // the row in registers and LDS: by two workgroups of 512 threads per CU if it fits half of them, else by one of 1024
-        const i64 vecs = a->n_cols / VecOf<T>::N, lists = ((i64)a->k * 12 + 15) / 16 * 16;
-        const i64 half = (LDS_BYTES / 2 - lists - 1024) / 16;
-        auto launch = [&](auto kernel, int nt, i64 stage) {
-            p.stage = (int)(vecs - (i64)ROW_VECS * nt < 0 ? 0 : vecs - (i64)ROW_VECS * nt < stage ? vecs - (i64)ROW_VECS * nt : stage);
+        // The row in registers and LDS, by the smallest kind of workgroup that holds all of it: 8 of 256 threads on a CU, 4 or 2 of 512, one
+        // of 1024; the last one takes longer rows as well, and reads the rest twice.
+        const i64 vecs = a->n_cols / VecOf<T>::N, lists = (i64)list_bytes(a);
+        auto launch = [&](auto kernel, i64 kept, i64 room) {
+            p.stage = (int)(vecs <= kept ? 0 : vecs - kept < room ? vecs - kept : room);
             const size_t lds = (size_t)(lists + (i64)p.stage * 16);
             HIP_TRY(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-            hipLaunchKernelGGL(kernel, dim3((unsigned)a->n_rows), dim3(nt), lds, stream, p);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)a->n_rows), dim3((unsigned)p.threads), lds, stream, p);
             HIP_TRY(hipGetLastError());
             return (int)SP_OK;
         };
-        if (vecs <= (i64)ROW_VECS * 512 + half) return launch(sp_distill_loss_grad_kernel<T, 512>, 512, half);
-        return launch(sp_distill_loss_grad_kernel<T, 1024>, 1024, (LDS_BYTES - lists - 1024) / 16);
+        auto room = [&](int wgs) { const i64 r = (LDS_BYTES / wgs - lists - 512) / 16; return r < 0 ? (i64)0 : r; };      // vectors in a share of the LDS
+        if (vecs <= 4 * 256 + room(8)) { p.threads = 256; return launch(sp_distill_loss_grad_kernel<T, 256, 4>, 4 * 256, room(8)); }
+        if (vecs <= 4 * 512 + room(4)) { p.threads = 512; return launch(sp_distill_loss_grad_kernel<T, 512, 4>, 4 * 512, room(4)); }
+        if (vecs <= 16 * 512 + room(2)) { p.threads = 512; return launch(sp_distill_loss_grad_kernel<T, 512, 16>, 16 * 512, room(2)); }
+        p.threads = 1024;
+        return launch(sp_distill_loss_grad_kernel<T, 1024, 16>, 16 * 1024, room(1));
     });
 }
 

@@ -27,7 +27,7 @@ struct DistillParams {
     int splits;                        // workgroups of a row
     i64 chunk;                         // columns of one of them (a multiple of the vector)
     float *part;                       // [n_rows, splits, 2] maximum, sum
-    int stage;                         // vectors of a row that the one-call kernel keeps in LDS
+    int threads, stage;                // the one-call kernel: threads of a workgroup, vectors of a row that it keeps in LDS
 };
 
 // maximum and sum of exp2((z - max) c) of some columns
@@ -140,68 +140,132 @@ template <typename T, int NT> __device__ __forceinline__ MaxSum scan_columns(con
     return a;
 }
 
-struct ListSums {
-    float mass;       // P
-    float loss;       // sum p_j (log p_j - log q[c_j]) when asked for, else 0
+// A row's list in LDS: columns (-1: not in the list), probabilities, the student's scores there, probabilities with the entries of equal
+// columns added up.  Room for k rounded up to whole vectors of 4; the slots behind the k-th are not in the list.
+struct ListLds {
+    int *col;
+    float *prob, *z, *sum;
+    __device__ __forceinline__ ListLds(int *mem, int k) : col(mem), prob((float *)(mem + list_room(k))), z((float *)(mem + 2 * list_room(k))), sum((float *)(mem + 3 * list_room(k))) {}
+    static __host__ __device__ constexpr int list_room(int k) { return (k + 3) / 4 * 4; }
 };
-// The teacher's list of a row, by the 64 lanes of one wave.  scol / sp (NULL or [k] in LDS): the columns (-1: not in the list) and
-// probabilities for the gradient.  a: the row's maximum and sum (read with LOSS only); log q is taken from score - maximum, so that the
-// type's lowest value as a mask stays finite.
-template <typename T, bool LOSS>
-__device__ __forceinline__ ListSums list_sums(const DistillParams &p, i64 row, const T *z, MaxSum a, int *scol, float *sprob) {
-    const int lane = threadIdx.x & 63;
+// The teacher's list of a row, by the 64 lanes of one wave, with S = sum p_j log p_j and P = sum p_j.  Nothing here depends on the row's
+// maximum and sum.  256 entries are requested at once, then the student's scores at all of their columns.
+struct ListSums {
+    float mass, plogp;
+};
+template <typename T> __device__ __forceinline__ ListSums list_sums(const DistillParams &p, i64 row, const T *z, const ListLds &list) {
+    constexpr int R = 4;
+    const int lane = threadIdx.x & 63, room = ListLds::list_room(p.k);
     int n = p.counts ? p.counts[row] : p.k;
     n = n < 0 ? 0 : n > p.k ? p.k : n;
     const i64 base = row * p.k;
-    const float high = a.m == NEG_INF ? 0.f : a.m, logs = LOSS ? logf(a.s) : 0.f;
-    float top = NEG_INF, shift = 0.f;
-    if (p.teacher_lse) shift = -p.teacher_lse[row];
-    else {
-        for (int j = lane; j < n; j += 64) {
-            const i64 col = load_index(p.cols, p.cols64, base + j);
-            if (col >= 0 && col < p.n_cols) top = fmaxf(top, load_scalar(p.values, p.values_dtype, base + j));
+    float top = NEG_INF;
+    for (int j0 = lane; j0 < room; j0 += 64 * R) {
+        i64 col[R];
+        float t[R], zc[R];
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const int j = j0 + 64 * u;
+            col[u] = -1;
+            t[u] = NEG_INF;
+            if (j < n) {
+                col[u] = load_index(p.cols, p.cols64, base + j);
+                t[u] = load_scalar(p.values, p.values_dtype, base + j);
+            }
         }
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const bool in = col[u] >= 0 && col[u] < p.n_cols;
+            zc[u] = 0.f;
+            if (in) zc[u] = up(z[col[u]]);
+            else {
+                col[u] = -1;
+                t[u] = NEG_INF;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const int j = j0 + 64 * u;
+            if (j < room) {
+                list.col[j] = (int)col[u];
+                list.prob[j] = t[u];
+                list.z[j] = zc[u];
+            }
+            top = fmaxf(top, t[u]);
+        }
+    }
+    float shift;
+    if (p.teacher_lse) {
+        shift = -p.teacher_lse[row];
+        top = 0.f;
+    } else {
         top = wave_max(top);
         float sum = 0.f;
-        for (int j = lane; j < n; j += 64) {
-            const i64 col = load_index(p.cols, p.cols64, base + j);
-            if (col >= 0 && col < p.n_cols && top != NEG_INF) sum += exp2_fast((load_scalar(p.values, p.values_dtype, base + j) - top) * p.inv_tau * LOG2E);
-        }
+        for (int j = lane; j < p.k; j += 64)
+            if (list.col[j] >= 0 && top != NEG_INF) sum += exp2_fast((list.prob[j] - top) * p.inv_tau * LOG2E);
         sum = wave_sum(sum);
         shift = sum > 0.f || sum != sum ? -logf(sum) : NEG_INF;       // (nothing in the list, or -inf only: all p_j are 0)
     }
     ListSums r{0.f, 0.f};
-    for (int j = lane; j < p.k; j += 64) {
+    for (int j = lane; j < room; j += 64) {
         float prob = 0.f;
-        int at = -1;
-        if (j < n) {
-            const i64 col = load_index(p.cols, p.cols64, base + j);
-            if (col >= 0 && col < p.n_cols) {
-                const float t = load_scalar(p.values, p.values_dtype, base + j);
-                const float logp = p.teacher_lse ? __fmaf_rn(t, p.inv_tau, shift) : top == NEG_INF ? NEG_INF : __fmaf_rn(t - top, p.inv_tau, shift);
-                prob = exp2_fast(logp * LOG2E);
-                at = (int)col;
-                r.mass += prob;
-                if (LOSS && prob != 0.f) {
-                    const float zc = up(z[col]);
-                    r.loss += prob * (logp - (zc == NEG_INF ? NEG_INF : __fmaf_rn(zc - high, p.inv_tau, -logs)));
-                }
-            }
+        if (list.col[j] >= 0) {
+            const float logp = top == NEG_INF ? NEG_INF : __fmaf_rn(list.prob[j] - top, p.inv_tau, shift);
+            prob = exp2_fast(logp * LOG2E);
+            r.mass += prob;
+            if (prob != 0.f) r.plogp += prob * logp;
         }
-        if (scol) {
-            scol[j] = at;
-            sprob[j] = prob;
-        }
+        list.prob[j] = prob;
     }
     r.mass = wave_sum(r.mass);
-    if (LOSS) r.loss = wave_sum(r.loss);
+    r.plogp = wave_sum(r.plogp);
     return r;
 }
+// tau^2 sum p_j (log p_j - log q[c_j]) by the same wave, log q = (z - m) / tau - log s: taken from score - maximum, so that the type's lowest
+// value as a mask stays finite
+__device__ __forceinline__ float list_loss(const DistillParams &p, ListSums l, MaxSum a, const ListLds &list) {
+    const float high = a.m == NEG_INF ? 0.f : a.m, logs = logf(a.s);
+    float cross = 0.f;
+    for (int j = threadIdx.x & 63; j < p.k; j += 64)
+        if (list.prob[j] != 0.f) cross += list.prob[j] * (list.z[j] == NEG_INF ? NEG_INF : __fmaf_rn(list.z[j] - high, p.inv_tau, -logs));
+    return p.tau * p.tau * (l.plogp - wave_sum(cross));
+}
+// Entries of the same column become one: the first one keeps their sum, the others leave the list.  By all NT threads, between barriers;
+// four columns are read per access, the same ones by all lanes.
+template <int NT> __device__ __forceinline__ void merge_listed(int k, const ListLds &list) {
+    const int4 *col4 = (const int4 *)list.col;
+    for (int j = threadIdx.x; j < k; j += NT) {
+        const int c = list.col[j];
+        int first = j;
+        unsigned same = 0;                                     // how many entries name the column
+#pragma unroll 4
+        for (int i = 0; i < ListLds::list_room(k) / 4; ++i) {
+            const int4 q = col4[i];
+            const unsigned hits = (unsigned)(q.x == c) | (unsigned)(q.y == c) << 1 | (unsigned)(q.z == c) << 2 | (unsigned)(q.w == c) << 3;
+            if (hits) {
+                if (same == 0) first = 4 * i + __builtin_ctz(hits);
+                same += __popc(hits);
+            }
+        }
+        float prob = list.prob[j];
+        if (same > 1 && first == j) {                          // (hardly ever: added up in the order of the list)
+            prob = 0.f;
+            for (int i = j; i < k; ++i)
+                if (list.col[i] == c) prob += list.prob[i];
+        }
+        list.sum[j] = first == j ? prob : -1.f;                // (probabilities are not negative; NaN stays)
+    }
+}
+
+// (16 bytes aligned: the list's columns and the one-call kernel's vectors are read as such)
+extern __shared__ __align__(16) int distill_list[];
 
 template <typename T> __device__ __forceinline__ void finish_loss(const DistillParams &p, i64 row, MaxSum a) {
     if (p.loss) {
-        const ListSums l = list_sums<T, true>(p, row, (const T *)p.student + row * p.ld_student, a, nullptr, nullptr);
-        if ((threadIdx.x & 63) == 0) p.loss[row] = p.tau * p.tau * l.loss;
+        const ListLds list(distill_list, p.k);
+        const ListSums l = list_sums<T>(p, row, (const T *)p.student + row * p.ld_student, list);
+        const float loss = list_loss(p, l, a, list);
+        if ((threadIdx.x & 63) == 0) p.loss[row] = loss;
     }
     if (p.stats && (threadIdx.x & 63) == 0) {
         p.stats[2 * row] = a.m;
@@ -232,29 +296,21 @@ __device__ __forceinline__ MaxSum join_parts(const DistillParams &p, i64 row) {
 // rows in several pieces: one wave joins them
 template <typename T> __global__ __launch_bounds__(64) void sp_distill_join_kernel(DistillParams p) { finish_loss<T>(p, blockIdx.x, join_parts(p, blockIdx.x)); }
 
-// the listed columns of [c0, c1) once more, with their probabilities taken off; a column listed several times is written by its first entry
+// the listed columns of [c0, c1) once more, with their probabilities taken off
 template <typename T, int NT, typename F>
-__device__ __forceinline__ void write_listed(const DistillParams &p, T *d, i64 c0, i64 c1, F one, float gt, const int *scol, const float *sprob, const float *sz) {
+__device__ __forceinline__ void write_listed(const DistillParams &p, T *d, i64 c0, i64 c1, F one, float gt, const ListLds &list) {
     for (int j = threadIdx.x; j < p.k; j += NT) {
-        const int c = scol[j];
-        if (c < c0 || c >= c1) continue;
-        float prob = 0.f;
-        bool first = true;
-        for (int i = 0; i < p.k; ++i)
-            if (scol[i] == c) {
-                first = first && i >= j;
-                prob += sprob[i];
-            }
-        if (first) d[c] = (T)(one(sz[j]) - gt * prob);
+        const int c = list.col[j];
+        if (c >= c0 && c < c1 && !(list.sum[j] < 0.f)) d[c] = (T)(one(list.z[j]) - gt * list.sum[j]);
     }
 }
 
 // The gradient of columns [c0, c1) of a row by the NT threads of a workgroup: g tau P q everywhere, then the listed columns once
-// more with their probabilities taken off.  scol / sprob hold the list; sz [k] is scratch: the listed scores are kept before
+// more with their probabilities taken off.  The list keeps the scores at its columns: they have been read before
 // anything is written, so `grad` may be `student`.  A row whose list
 // has no mass gets zeros, whatever its scores hold (a padded row of a batch).
 template <typename T, int NT>
-__device__ __forceinline__ void grad_columns(const DistillParams &p, i64 row, i64 c0, i64 c1, MaxSum a, float mass, float gt, const int *scol, const float *sprob, float *sz) {
+__device__ __forceinline__ void grad_columns(const DistillParams &p, i64 row, i64 c0, i64 c1, MaxSum a, float mass, float gt, const ListLds &list) {
     constexpr int N = VecOf<T>::N, U = 4;
     const int tid = threadIdx.x;
     const T *z = (const T *)p.student + row * p.ld_student;
@@ -271,11 +327,6 @@ __device__ __forceinline__ void grad_columns(const DistillParams &p, i64 row, i6
     }
     const Exponent x = exponent_of(a.m, p.c);
     const float coef = a.s == 0.f ? 0.f : gt * mass / a.s * correction_of(a.m, x);       // (a row of -inf only has q = 0)
-    for (int j = tid; j < p.k; j += NT) {
-        const int c = scol[j];
-        sz[j] = c >= c0 && c < c1 ? up(z[c]) : 0.f;
-    }
-    __syncthreads();
     auto one = [&](float v) { return coef * exp2_fast(__fmaf_rn(v, x.c, -x.off)); };
     i64 i = c0 + (i64)tid * N;
     for (; i + (U - 1) * NT * N + N <= c1; i += U * NT * N) {
@@ -300,24 +351,23 @@ __device__ __forceinline__ void grad_columns(const DistillParams &p, i64 row, i6
     for (int j = 0; j < N; ++j)
         if (i + j < c1) d[i + j] = (T)one(up(z[i + j]));
     __syncthreads();
-    write_listed<T, NT>(p, d, c0, c1, one, gt, scol, sprob, sz);
+    write_listed<T, NT>(p, d, c0, c1, one, gt, list);
 }
-
-extern __shared__ int distill_list[];      // [k] columns, [k] probabilities, [k] scores
 
 template <typename T, int NT> __global__ __launch_bounds__(NT) void sp_distill_grad_kernel(DistillParams p) {
     __shared__ float mass;
-    int *scol = distill_list;
-    float *sprob = (float *)(distill_list + p.k), *sz = sprob + p.k;
+    const ListLds list(distill_list, p.k);
     const i64 row = blockIdx.x / p.splits, c0 = (blockIdx.x % p.splits) * p.chunk, c1 = min(p.n_cols, c0 + p.chunk);
     if (threadIdx.x < 64) {
-        const ListSums l = list_sums<T, false>(p, row, nullptr, MaxSum{0.f, 1.f}, scol, sprob);
+        const ListSums l = list_sums<T>(p, row, (const T *)p.student + row * p.ld_student, list);
         if (threadIdx.x == 0) mass = l.mass;
     }
     const MaxSum a{p.stats[2 * row], p.stats[2 * row + 1]};
     const float gt = (p.grad_loss ? p.grad_loss[row] : 1.f) * p.tau;
     __syncthreads();
-    grad_columns<T, NT>(p, row, c0, c1, a, mass, gt, scol, sprob, sz);
+    merge_listed<NT>(p.k, list);
+    __syncthreads();
+    grad_columns<T, NT>(p, row, c0, c1, a, mass, gt, list);
 }
 
 // what the compiler has derived from a vector is to be derived again
@@ -329,26 +379,29 @@ template <typename T, int N> __device__ __forceinline__ void forget(RawVec<T, N>
     __builtin_memcpy(&x, &q, 16);
 }
 
-// Loss and gradient of a row by one workgroup that keeps the row: ROW_VECS vectors of 16 bytes per thread in registers, `stage` more per
+// Loss and gradient of a row by one workgroup that keeps the row: RV vectors of 16 bytes per thread in registers, `stage` more per
 // workgroup in LDS; only what is left of a still longer row is read a second time.  The sums are formed while vectors arrive, the gradient
-// while they leave; two workgroups of 512 threads share a CU where the row allows it, so that one loads while the other stores.
-constexpr int ROW_VECS = 16;
-template <typename T, int NT> __global__ __launch_bounds__(NT, 4) void sp_distill_loss_grad_kernel(DistillParams p) {
+// while they leave; several workgroups share a CU where the row allows it, so that one loads while another stores.
+template <typename T, int NT, int RV> __global__ __launch_bounds__(NT, RV <= 4 ? 8 : 4) void sp_distill_loss_grad_kernel(DistillParams p) {
     constexpr int N = VecOf<T>::N, M = 16 / N;                 // M vectors, 16 scores, are added at once
     __shared__ MaxSum sh[NT / 64];
     __shared__ float mass_of_row;
-    int *scol = distill_list;
-    float *sprob = (float *)(distill_list + p.k), *sz = sprob + p.k;
-    RawVec<T, N> *stage = (RawVec<T, N> *)(distill_list + (3 * p.k + 3) / 4 * 4);
+    const ListLds list(distill_list, p.k);
+    RawVec<T, N> *stage = (RawVec<T, N> *)(distill_list + 4 * ListLds::list_room(p.k));
     const i64 row = blockIdx.x;
     const int tid = threadIdx.x, n_cols = (int)p.n_cols, vecs = n_cols / N;
-    const int kept = min(vecs, ROW_VECS * NT + p.stage);       // vectors that are not read again
+    const int kept = min(vecs, RV * NT + p.stage);             // vectors that are not read again
     const T *z = (const T *)p.student + row * p.ld_student;
     T *d = (T *)p.grad + row * p.ld_grad;
 
-    RawVec<T, N> x[ROW_VECS];
+    ListSums l{0.f, 0.f};
+    if (tid < 64) {                                            // (one wave is a little late; what it does is in nobody's way then)
+        l = list_sums<T>(p, row, z, list);
+        if (tid == 0) mass_of_row = l.mass;
+    }
+    RawVec<T, N> x[RV];
 #pragma unroll
-    for (int q = 0; q < ROW_VECS; ++q) {
+    for (int q = 0; q < RV; ++q) {
         const int j = q * NT + tid;
         if (j < vecs) x[q] = vec_load<T, N>(z + (i64)j * N);
         else {
@@ -357,9 +410,9 @@ template <typename T, int NT> __global__ __launch_bounds__(NT, 4) void sp_distil
         }
     }
     Running run{NEG_INF, NEG_INF, 0.f};
-    for (int j = ROW_VECS * NT + tid; j < vecs; j += NT) {
+    for (int j = RV * NT + tid; j < vecs; j += NT) {
         const RawVec<T, N> y = vec_load<T, N>(z + (i64)j * N);
-        if (j < kept) stage[j - ROW_VECS * NT] = y;
+        if (j < kept) stage[j - RV * NT] = y;
         float v[N];
 #pragma unroll
         for (int e = 0; e < N; ++e) v[e] = up(y.v[e]);
@@ -369,7 +422,7 @@ template <typename T, int NT> __global__ __launch_bounds__(NT, 4) void sp_distil
     const float lone = end < n_cols ? up(z[end]) : NEG_INF;
     add_vec<1>(run, &lone, p.c);
 #pragma unroll
-    for (int q = 0; q < ROW_VECS; q += M) {
+    for (int q = 0; q < RV; q += M) {
         if (q * NT >= vecs) break;
         float v[16];
 #pragma unroll
@@ -380,19 +433,15 @@ template <typename T, int NT> __global__ __launch_bounds__(NT, 4) void sp_distil
     }
     MaxSum a = block_join<NT>(finish(run, p.c), p.c, sh);
     if (!off_fits(a.m, p.c)) a = rescan<T, NT>(z, 0, n_cols, a, p.c, sh);
-    if (tid < 64) {
-        const ListSums l = list_sums<T, true>(p, row, z, a, scol, sprob);
-        if (tid == 0) {
-            mass_of_row = l.mass;
-            if (p.loss) p.loss[row] = p.tau * p.tau * l.loss;
-        }
+    if (tid < 64 && p.loss) {
+        const float loss = list_loss(p, l, a, list);
+        if (tid == 0) p.loss[row] = loss;
     }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < ROW_VECS; ++q) forget(x[q]);           // (or the scores stay unpacked in registers, which there are not enough of)
-    const float mass = mass_of_row, gt = (p.grad_loss ? p.grad_loss[row] : 1.f) * p.tau;
-    for (int j = tid; j < p.k; j += NT) sz[j] = scol[j] >= 0 ? up(z[scol[j]]) : 0.f;
+    merge_listed<NT>(p.k, list);
     __syncthreads();                                           // (from here on `grad` is written, which may be `student`)
+#pragma unroll
+    for (int q = 0; q < RV; ++q) forget(x[q]);                 // (or the scores stay unpacked in registers, which there are not enough of)
+    const float mass = mass_of_row, gt = (p.grad_loss ? p.grad_loss[row] : 1.f) * p.tau;
     const Exponent ex = exponent_of(a.m, p.c);
     const bool some = mass != 0.f;                             // (a row whose list has no mass gets zeros, whatever its scores hold)
     const float coef = a.s == 0.f || !some ? 0.f : gt * mass / a.s * correction_of(a.m, ex);
@@ -406,12 +455,12 @@ template <typename T, int NT> __global__ __launch_bounds__(NT, 4) void sp_distil
     // (what has to be read again goes first: nothing of it has been written yet)
     for (int j = kept + tid; j < vecs; j += NT) put(j, vec_load<T, N>(z + (i64)j * N));
 #pragma unroll
-    for (int q = 0; q < ROW_VECS; ++q)
+    for (int q = 0; q < RV; ++q)
         if (q * NT + tid < vecs) put(q * NT + tid, x[q]);
-    for (int j = ROW_VECS * NT + tid; j < kept; j += NT) put(j, stage[j - ROW_VECS * NT]);
+    for (int j = RV * NT + tid; j < kept; j += NT) put(j, stage[j - RV * NT]);
     if (end < n_cols) d[end] = (T)one(lone);
     __syncthreads();
-    write_listed<T, NT>(p, d, 0, n_cols, one, gt, scol, sprob, sz);
+    write_listed<T, NT>(p, d, 0, n_cols, one, gt, list);
 }
 
 }  // namespace
