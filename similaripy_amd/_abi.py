@@ -531,10 +531,16 @@ def call_col_sums(args: SpCsrColsumsArgs) -> None:
         raise HipLibraryError(f"sp_csr_col_sums_f32 failed ({rc}): {last_error()}")
 
 
+_dense_fns = {}      # entries of include/sp_dense.h that have been called
+
+
 def call_dense(symbol: str, args) -> int:
     """One entry of include/sp_dense.h: 0, or the bytes a workspace query answers."""
+    fn = _dense_fns.get(symbol)
+    if fn is None:
+        fn = _dense_fns[symbol] = getattr(load(), symbol)
     args.struct_size = C.sizeof(args)
-    rc = getattr(load(), symbol)(C.byref(args))
+    rc = fn(C.byref(args))
     if rc < 0:
         raise HipLibraryError(f"{symbol} failed ({rc}): {last_error()}")
     return rc

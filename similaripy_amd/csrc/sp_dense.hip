@@ -306,6 +306,11 @@ DistillParams distill_params(const sp_distill_args *a) {
     return p;
 }
 
+// a kernel's limit of dynamic LDS is raised where a launch needs more than every kernel may have
+int allow_lds(const void *kernel, size_t bytes) {
+    if (bytes > 48 * 1024) HIP_TRY(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    return SP_OK;
+}
 size_t list_bytes(const sp_distill_args *a) { return (size_t)ListLds::list_room(a->k) * 16; }
 
 constexpr i64 SCAN_WGS = 1024, GRAD_WGS = 2048;
@@ -318,8 +323,8 @@ int launch_scan(const sp_distill_args *a, DistillParams p, hipStream_t stream) {
     const size_t lists = list_bytes(a);
     return with_type(a->dtype, [&](auto tag) {
         using T = decltype(tag);
-        HIP_TRY(hipFuncSetAttribute((const void *)sp_distill_scan_kernel<T, DI_NT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lists));
-        HIP_TRY(hipFuncSetAttribute((const void *)sp_distill_join_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lists));
+        TRY(allow_lds((const void *)sp_distill_scan_kernel<T, DI_NT>, lists));
+        TRY(allow_lds((const void *)sp_distill_join_kernel<T>, lists));
         hipLaunchKernelGGL((sp_distill_scan_kernel<T, DI_NT>), dim3((unsigned)(a->n_rows * p.splits)), dim3(DI_NT), lists, stream, p);
         if (p.splits > 1) hipLaunchKernelGGL((sp_distill_join_kernel<T>), dim3((unsigned)a->n_rows), dim3(64), lists, stream, p);
         HIP_TRY(hipGetLastError());
@@ -332,15 +337,17 @@ int launch_grad(const sp_distill_args *a, DistillParams p, hipStream_t stream) {
     return with_type(a->dtype, [&](auto tag) {
         using T = decltype(tag);
         const size_t lists = list_bytes(a);
-        HIP_TRY(hipFuncSetAttribute((const void *)sp_distill_grad_kernel<T, DI_NT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lists));
+        TRY(allow_lds((const void *)sp_distill_grad_kernel<T, DI_NT>, lists));
         hipLaunchKernelGGL((sp_distill_grad_kernel<T, DI_NT>), dim3((unsigned)(a->n_rows * p.splits)), dim3(DI_NT), lists, stream, p);
         HIP_TRY(hipGetLastError());
         return (int)SP_OK;
     });
 }
 
+// the row statistics between the two halves of a call that is not one kernel, and the partial ones of rows in several pieces
 i64 distill_ws_bytes(const sp_distill_args *a) {
-    return (i64)distill_stats_bytes(a) + a->n_rows * splits_of(a, SCAN_WGS) * 8;
+    const int splits = splits_of(a, SCAN_WGS);
+    return a->n_rows >= FUSED_ROWS && splits == 1 ? 0 : (i64)distill_stats_bytes(a) + a->n_rows * splits * 8;
 }
 int check_workspace(const void *ws, i64 have, i64 need) {
     if (need > 0 && (!ws || have < need)) return fail(SP_EWORKSPACE, "workspace too small: need %lld bytes, got %lld", need, ws ? have : 0ll);
@@ -462,7 +469,7 @@ int sp_distill_loss_grad(const sp_distill_args *a) {
         auto launch = [&](auto kernel, i64 kept, i64 room) {
             p.stage = (int)(vecs <= kept ? 0 : vecs - kept < room ? vecs - kept : room);
             const size_t lds = (size_t)(lists + (i64)p.stage * 16);
-            HIP_TRY(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+            TRY(allow_lds((const void *)kernel, lds));
             hipLaunchKernelGGL(kernel, dim3((unsigned)a->n_rows), dim3((unsigned)p.threads), lds, stream, p);
             HIP_TRY(hipGetLastError());
             return (int)SP_OK;

@@ -40,8 +40,12 @@ _INT = (torch.int32, torch.int64)
 
 # ---- argument checks ---------------------------------------------------------------------------------------------------------
 
+# (the checks of one operand are one condition on the way through: a small call's time is mostly this file's)
+
 def _dense(name: str, t, ndim: int = 2):
     """A dense operand: a supported type on a HIP device, rows contiguous."""
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _DT and t.dim() == ndim and (ndim == 1 or t.stride(1) == 1 or t.shape[1] <= 1):
+        return t
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if t.dtype not in _DT:
@@ -50,9 +54,7 @@ def _dense(name: str, t, ndim: int = 2):
         raise ValueError(f"{name} must have {ndim} dimension(s), got shape {tuple(t.shape)}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a HIP device (similaripy_amd has no CPU fallback), got {t.device}")
-    if ndim == 2 and t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name} must have contiguous rows (stride 1 in its last dimension), got strides {t.stride()}")
-    return t
+    raise ValueError(f"{name} must have contiguous rows (stride 1 in its last dimension), got strides {t.stride()}")
 
 
 def _same_device(name: str, t, device) -> None:
@@ -62,15 +64,18 @@ def _same_device(name: str, t, device) -> None:
 
 def _ints(name: str, t, device, dtypes=_INT):
     """An index operand, contiguous."""
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.device == device:
+        return t if t.is_contiguous() else t.contiguous()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, got {t.dtype}")
-    _same_device(name, t, device)
-    return t if t.is_contiguous() else t.contiguous()
+    raise ValueError(f"{name} is on {t.device}, the other operands are on {device}")
 
 
 def _floats(name: str, t, device, numel: int, dtype=torch.float32):
+    if isinstance(t, torch.Tensor) and t.dtype == dtype and t.numel() == numel and t.device == device and not t.requires_grad:
+        return t if t.is_contiguous() else t.contiguous()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if t.dtype != dtype:
@@ -78,9 +83,9 @@ def _floats(name: str, t, device, numel: int, dtype=torch.float32):
     if t.numel() != numel:
         raise ValueError(f"{name} must have {numel} elements, got shape {tuple(t.shape)}")
     _same_device(name, t, device)
-    if t.requires_grad and torch.is_grad_enabled():
+    if torch.is_grad_enabled():
         raise ValueError(f"{name} has no gradient here: detach it")
-    return t if t.is_contiguous() else t.contiguous()
+    return t.contiguous()
 
 
 def _ld(t) -> int:
@@ -117,15 +122,17 @@ def _extent(t):
     return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
 
 
+# torch's own way to a stream's handle costs as much as a launch; torch.compile's generated code uses this one
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
-def _no_grad_here(name: str, *tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t.requires_grad:
-                raise ValueError(f"{name} builds no autograd graph: detach its inputs or call it under torch.no_grad()")
+def _no_grad_here(name: str, t) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} builds no autograd graph: detach its inputs or call it under torch.no_grad()")
 
 
 def _not_capturing(name: str, instead: str) -> None:
@@ -259,8 +266,9 @@ def _pattern(name: str, csr, device, keep):
         return _NO_PATTERN
     if not isinstance(csr, (tuple, list)) or len(csr) != 2:
         raise TypeError(f"{name} must be a pair (indptr, indices)")
-    indices = _ints(f"{name} indices", csr[1], device)
-    indptr = _ints(f"{name} indptr", csr[0], device, (indices.dtype,))
+    indptr, indices = csr
+    indices = _ints(name, indices, device)
+    indptr = _ints(name, indptr, device, (indices.dtype,))
     if indptr.dim() != 1 or indptr.numel() < 1 or indices.dim() != 1:
         raise ValueError(f"{name}: indptr and indices must have 1 dimension, indptr at least one element")
     keep += (indptr, indices)
@@ -311,9 +319,8 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
     h = _pattern("history", history, device, keep)
     f = _pattern("filter_cols", filter_cols, device, keep)
     t = _pattern("target_cols", target_cols, device, keep)
-    for name, v in (("repetition", repetition),):
-        if not isinstance(v, torch.Tensor) and not float(v) > 0.0:
-            raise ValueError(f"{name} must be positive, got {v}")
+    if not isinstance(repetition, torch.Tensor) and not float(repetition) > 0.0:
+        raise ValueError(f"repetition must be positive, got {repetition}")
     rep, rep_all = _per_row("repetition", repetition, device, n, keep)
     pres, pres_all = _per_row("presence", presence, device, n, keep)
     freq, freq_all = _per_row("frequency", frequency, device, n, keep)
@@ -354,7 +361,7 @@ def _distill_args(student, cols, values, counts, temperature, teacher_lse):
     if cols.numel() % max(1, n) or (n == 0 and cols.numel()):
         raise ValueError(f"cols must hold the same number of slots for each of the {n} rows, got shape {tuple(cols.shape)}")
     k = cols.numel() // n if n else 0
-    if cols.dim() != 1 and tuple(cols.shape) != (n, k) and n:
+    if n and cols.dim() != 1 and cols.shape != (n, k):
         raise ValueError(f"cols must have shape ({n}, k) or ({n} * k,), got {tuple(cols.shape)}")
     if k > _abi.SP_DISTILL_KMAX:
         raise ValueError(f"lists of {k} slots: at most {_abi.SP_DISTILL_KMAX} are supported")
@@ -380,8 +387,11 @@ def _distill_args(student, cols, values, counts, temperature, teacher_lse):
 
 
 def _workspace(a, device):
-    ws = torch.empty(_abi.call_dense("sp_distill_workspace_bytes", a), dtype=torch.uint8, device=device)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    need = _abi.call_dense("sp_distill_workspace_bytes", a)
+    if not need:
+        return None
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need
     return ws
 
 
