@@ -129,7 +129,7 @@ int run_embed(const sp_embed_args *a) {
 
 // workspace of the gradient: two copies of the sorted entries (the passes alternate), the digit counts, the partial sums
 constexpr i64 REDUCE_CHUNKS = 4096;      // groups that sum sorted entries: about four waves per SIMD at one slab of 64 lanes
-constexpr int SORT_WGS = 512;
+constexpr int DIRECT_WGS = 512;
 struct GradLayout {
     int wgs, sort_chunk, passes, bits, chunk;
     bool small;                                                  // sorted by one workgroup
@@ -139,9 +139,10 @@ struct GradLayout {
 GradLayout grad_layout(const sp_embed_args *a) {
     GradLayout L{};
     const i64 n = a->nnz;
-    // chunks of 1024 entries, or more of them once that makes more than SORT_WGS workgroups
-    L.sort_chunk = (int)(ceil_div(ceil_div(n, SORT_WGS), SORT_NT) * SORT_NT);
-    if (L.sort_chunk < 1024) L.sort_chunk = 1024;
+    if (n <= DIRECT_MAX) return L;                               // no sort, no workspace
+    // chunks for one workgroup per CU, of 1024 .. SORT_CHUNK entries
+    i64 chunk = ceil_div(ceil_div(n, 256), SORT_NT) * SORT_NT;
+    L.sort_chunk = (int)(chunk < 1024 ? 1024 : chunk > SORT_CHUNK ? SORT_CHUNK : chunk);
     L.wgs = (int)ceil_div(n, L.sort_chunk);
     int kb = 1;                                                  // bits of the keys 0 .. n_vocab
     while (kb < 31 && (1ll << kb) <= a->n_vocab) ++kb;
@@ -177,6 +178,25 @@ template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a)
     if (!entries && fill.out) {
         fill.parts = 1;
         hipLaunchKernelGGL(sp_fill_kernel<SORT_NT>, dim3(FILL_WGS * 2), dim3(SORT_NT), 0, stream, fill);
+    }
+    if (entries && a->nnz <= DIRECT_MAX) {
+        DirectParams d{};
+        ReduceParams &r = d.r;
+        r.in = a->src; r.out = a->out; r.n = a->nnz; r.n_vocab = a->n_vocab; r.n_rows = a->n_rows; r.ld_in = a->ld_src; r.ld_out = a->ld_out;
+        r.dim = (int)a->dim; r.accumulate = a->accumulate; r.scale = a->scale;
+        d.indices = a->indices; d.indptr = a->indptr; d.data = a->data;
+        const i64 per = ceil_div(a->n_vocab, DIRECT_WGS);
+        d.per = (int)(per < DIRECT_IDS ? per : DIRECT_IDS);
+        return with_group<T>(a->dim, [&](auto gc, auto nc) {
+            constexpr int G = decltype(gc)::value, N = decltype(nc)::value;
+            r.slabs = (int)ceil_div(a->dim, G * N);
+            const i64 blocks = ceil_div(a->n_vocab, d.per) * r.slabs;
+            if (blocks > I32_MAX) return fail(SP_EINVAL, "too many rows for one launch");
+            auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, d); };
+            a->index64 ? launch(sp_embed_grad_direct_kernel<T, TO, i64, G, N>) : launch(sp_embed_grad_direct_kernel<T, TO, int, G, N>);
+            HIP_TRY(hipGetLastError());
+            return (int)SP_OK;
+        });
     }
     if (entries) {
         const GradLayout L = grad_layout(a);

@@ -121,6 +121,7 @@ template <typename T, typename I, int G, int N> __global__ __launch_bounds__(256
 // An entry carries its row of the gradient and its weight.  The rows of a CSR's entries are written out beside the first count.
 
 constexpr int SORT_NT = 512, SORT_WAVES = SORT_NT / 64, SORT_BINS = 512;
+constexpr int SORT_PER = 9, SORT_CHUNK = SORT_NT * SORT_PER;    // entries of a thread, most of a workgroup: 54 KB of LDS
 constexpr int SORT_DIRECT = 32;      // up to so many workgroups the moving launch adds up the counts itself
 
 // The rows of the gradient that no entry names are 0: all of it is cleared, by workgroups behind those of the sort's launches, which leave
@@ -234,9 +235,14 @@ __global__ __launch_bounds__(1024) void sp_sort_prefix_kernel(unsigned *hist, un
 }
 static_assert(SORT_NT == SORT_BINS, "a thread per digit");
 
+// Entries go to their places by way of LDS, where the chunk is laid out in the order of its digits: neighbours there are neighbours in
+// memory, so that what a wave writes are runs (scattered one by one, 1.2 M entries took 24 us a pass).
 template <typename I> __global__ __launch_bounds__(SORT_NT) void sp_sort_move_kernel(SortParams p) {
     __shared__ unsigned off[SORT_WAVES][SORT_BINS];
-    __shared__ unsigned wsum[SORT_WAVES];
+    __shared__ unsigned delta[SORT_BINS];                      // global place - place in the chunk, of a digit
+    __shared__ unsigned wsum[2][SORT_WAVES];
+    __shared__ unsigned skey[SORT_CHUNK], spay[SORT_CHUNK];
+    __shared__ float sweight[SORT_CHUNK];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const unsigned mask = (1u << p.bits) - 1u;
     // consecutive chunks go to one XCD (workgroups are dealt to the eight in turn): what they write next to each other meets in its L2
@@ -247,6 +253,21 @@ template <typename I> __global__ __launch_bounds__(SORT_NT) void sp_sort_move_ke
     }
     const int wg = (int)(blockIdx.x % 8) * per_xcd + (int)blockIdx.x / 8;
     if (wg >= p.wgs) return;
+    // the wave's part, consecutive entries, all of it requested at once
+    const int n = (int)min((i64)p.chunk, p.n - (i64)wg * p.chunk), per = p.chunk / SORT_WAVES, rounds = per / 64;
+    const int first = wave * per + lane;
+    const i64 chunk0 = (i64)wg * p.chunk;
+    unsigned key[SORT_PER], pay[SORT_PER];
+    float weight[SORT_PER];
+#pragma unroll
+    for (int q = 0; q < SORT_PER; ++q) {
+        const int j = first + q * 64;
+        if (q < rounds && j < n) {
+            key[q] = sort_key<I>(p, chunk0 + j);
+            pay[q] = p.key_in ? p.pay_in[chunk0 + j] : p.entry_row ? p.entry_row[chunk0 + j] : (unsigned)(chunk0 + j);
+            if (p.w_out) weight[q] = p.w_in[chunk0 + j];
+        }
+    }
     for (int w = 0; w < SORT_WAVES; ++w) off[w][tid] = 0;
     // entries of digit `tid` before this workgroup: those of smaller digits anywhere, and of its own in the workgroups before
     unsigned before = 0, all = 0;
@@ -263,59 +284,66 @@ template <typename I> __global__ __launch_bounds__(SORT_NT) void sp_sort_move_ke
         before = p.hist[(i64)wg * SORT_BINS + tid];
         all = p.total[tid];
     }
-    unsigned inc = all;
+    __syncthreads();
+    // digits of every wave's part
+#pragma unroll
+    for (int q = 0; q < SORT_PER; ++q)
+        if (q < rounds && first + q * 64 < n) atomicAdd(&off[wave][(key[q] >> p.shift) & mask], 1u);
+    __syncthreads();
+    unsigned here = 0;
+    for (int w = 0; w < SORT_WAVES; ++w) here += off[w][tid];
+    unsigned inc_all = all, inc_here = here;                   // prefix sums over the digits, of all entries and of the chunk's
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const unsigned o = __shfl_up(inc, d, 64);
-        if (lane >= d) inc += o;
+        const unsigned o = __shfl_up(inc_all, d, 64), q = __shfl_up(inc_here, d, 64);
+        if (lane >= d) {
+            inc_all += o;
+            inc_here += q;
+        }
     }
-    if (lane == 63) wsum[wave] = inc;
+    if (lane == 63) {
+        wsum[0][wave] = inc_all;
+        wsum[1][wave] = inc_here;
+    }
     __syncthreads();
-    unsigned base = before + inc - all;
-    for (int w = 0; w < wave; ++w) base += wsum[w];
-    // digits of every wave's part
-    const int per = p.chunk / SORT_WAVES;
-    const i64 b = (i64)wg * p.chunk + (i64)wave * per, e = min(p.n, b + per);
-    for (i64 i = b + lane; i < e; i += 64) atomicAdd(&off[wave][(sort_key<I>(p, i) >> p.shift) & mask], 1u);
-    __syncthreads();
+    unsigned place = before + inc_all - all, local = inc_here - here;
+    for (int w = 0; w < wave; ++w) {
+        place += wsum[0][w];
+        local += wsum[1][w];
+    }
+    delta[tid] = place - local;
     for (int w = 0; w < SORT_WAVES; ++w) {
         const unsigned n = off[w][tid];
-        off[w][tid] = base;
-        base += n;
+        off[w][tid] = local;
+        local += n;
     }
     __syncthreads();
     volatile unsigned *mine = off[wave];
-    constexpr int Q = 4;                                       // 64 entries each, requested together
-    for (i64 i0 = b; i0 < e; i0 += 64 * Q) {
-        unsigned key[Q], pay[Q];
-        float weight[Q];
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-            const i64 i = i0 + q * 64 + lane;
-            if (i < e) {
-                key[q] = sort_key<I>(p, i);
-                pay[q] = p.key_in ? p.pay_in[i] : p.entry_row ? p.entry_row[i] : (unsigned)i;
-                if (p.w_out) weight[q] = p.w_in[i];
-            }
+    for (int q = 0; q < SORT_PER; ++q) {
+        if (q >= rounds) break;
+        const bool ok = first + q * 64 < n;
+        const unsigned digit = ok ? (key[q] >> p.shift) & mask : 0u;
+        u64 same = __ballot(ok);
+        for (int k = 0; k < p.bits; ++k) {
+            const u64 set = __ballot((digit >> k) & 1u);
+            same &= (digit >> k) & 1u ? set : ~set;
         }
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-            const bool ok = i0 + q * 64 + lane < e;
-            const unsigned digit = ok ? (key[q] >> p.shift) & mask : 0u;
-            u64 same = __ballot(ok);
-            for (int k = 0; k < p.bits; ++k) {
-                const u64 set = __ballot((digit >> k) & 1u);
-                same &= (digit >> k) & 1u ? set : ~set;
-            }
-            if (ok) {
-                const unsigned rank = (unsigned)__popcll(same & ((1ull << lane) - 1ull));
-                const unsigned at = mine[digit] + rank;
-                if (rank == 0) mine[digit] = at + (unsigned)__popcll(same);       // (a wave's LDS accesses keep their order: everybody has read)
-                p.key_out[at] = key[q];
-                p.pay_out[at] = pay[q];
-                if (p.w_out) p.w_out[at] = weight[q];
-            }
+        if (ok) {
+            const unsigned rank = (unsigned)__popcll(same & ((1ull << lane) - 1ull));
+            const unsigned at = mine[digit] + rank;
+            if (rank == 0) mine[digit] = at + (unsigned)__popcll(same);       // (a wave's LDS accesses keep their order: everybody has read)
+            skey[at] = key[q];
+            spay[at] = pay[q];
+            if (p.w_out) sweight[at] = weight[q];
         }
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += SORT_NT) {
+        const unsigned k = skey[i], at = (unsigned)i + delta[(k >> p.shift) & mask];
+        p.key_out[at] = k;
+        p.pay_out[at] = spay[i];
+        if (p.w_out) p.w_out[at] = sweight[i];
     }
 }
 
@@ -517,6 +545,101 @@ template <typename T, typename TO, int G, int N> __global__ __launch_bounds__(25
         }
     }
     flush(true);
+}
+
+// Up to 1024 entries need no sort at all: a workgroup owns DIRECT_IDS ids or fewer (and a slab of columns), looks through all entries, keeps
+// those of its ids in their order, sums each id's and clears the rows that have none.  One launch, no workspace.  Gradient of n lookups
+// into 84 433 rows of 1024 bf16, this way / by the sort above: n = 64 24 / 33 us, 512 27 / 36, 1024 28 / 35, 2048 36 / 35; into 2000 rows:
+// 8.8 / 18, 10 / 19, 16 / 20, 31 / 20 (what a popular id has is summed by one group).
+constexpr int DIRECT_MAX = 1024, DIRECT_IDS = 2048, DIRECT_NONE = 0x7FFFFFFF;
+struct DirectParams {
+    ReduceParams r;              // in, out, n, n_vocab, ld_in, ld_out, n_rows, dim, slabs, accumulate, scale
+    const void *indices, *indptr;
+    const float *data;
+    int per;                     // ids of a workgroup
+};
+template <typename T, typename TO, typename I, int G, int N> __global__ __launch_bounds__(256) void sp_embed_grad_direct_kernel(DirectParams d) {
+    constexpr int GROUPS = 256 / G, U = 8, Q = DIRECT_MAX / 256;
+    __shared__ int key[DIRECT_MAX], from[DIRECT_MAX], first[DIRECT_IDS];
+    __shared__ float weight[DIRECT_MAX];
+    __shared__ int wsum[4];
+    const ReduceParams &p = d.r;
+    const int tid = threadIdx.x, lane = tid & 63, gl = tid & (G - 1), g = tid / G, n = (int)p.n;
+    const i64 v0 = (i64)(blockIdx.x / p.slabs) * d.per;
+    const int width = (int)min((i64)d.per, p.n_vocab - v0);
+    const Columns<N> cols(((int)(blockIdx.x % p.slabs) * G + gl) * N, p.dim);
+    int mine[Q], count = 0;                                    // a thread's entries are consecutive: their order is the threads'
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int i = tid * Q + q;
+        const i64 id = i < n ? (i64)((const I *)d.indices)[i] - v0 : -1;
+        mine[q] = id >= 0 && id < width ? (int)id : -1;
+        count += mine[q] >= 0;
+    }
+    for (int i = tid; i < width; i += 256) first[i] = DIRECT_NONE;
+    int at = count;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+        const int o = __shfl_up(at, k, 64);
+        if (lane >= k) at += o;
+    }
+    if (lane == 63) wsum[tid >> 6] = at;
+    __syncthreads();
+    at -= count;
+    for (int w = 0; w < (tid >> 6); ++w) at += wsum[w];
+    const int m = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+        if (mine[q] >= 0) {
+            key[at] = mine[q];
+            from[at] = tid * Q + q;
+            atomicMin(&first[mine[q]], at);
+            ++at;
+        }
+    __syncthreads();
+    for (int e = tid; e < m; e += 256) {
+        const int i = from[e];
+        const i64 r = d.indptr ? row_of<I>(d.indptr, p.n_rows, i) : i;
+        weight[e] = d.data ? d.data[i] : 1.f;
+        from[e] = r < p.n_rows ? (int)r : -1;
+    }
+    __syncthreads();
+    for (int e = g; e < m; e += GROUPS) {
+        const int k = key[e];
+        if (first[k] != e) continue;
+        float acc[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) acc[q] = 0.f;
+        for (int f0 = e; f0 < m; f0 += G) {                    // G entries looked at together; the id's own ones in their order
+            const u64 all = __ballot(f0 + gl < m && key[min(f0 + gl, m - 1)] == k);
+            u64 hits = G == 64 ? all : (all >> (lane & ~(G - 1))) & ((1ull << (G & 63)) - 1ull);
+            while (hits) {
+                RawVec<T, N> x[U];
+                int r[U], f[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    f[u] = hits ? f0 + __builtin_ctzll(hits) : f0;
+                    r[u] = hits ? from[f[u]] : -1;
+                    hits &= hits - 1ull;                       // (0 stays 0)
+                    x[u] = vec_load<T, N>((const T *)p.in + (i64)max(r[u], 0) * p.ld_in + cols.c);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (r[u] >= 0) {
+                        const float w = weight[f[u]];
+#pragma unroll
+                        for (int q = 0; q < N; ++q) acc[q] = __fmaf_rn(w, up(x[u].v[q]), acc[q]);
+                    }
+            }
+        }
+        if (cols.active) write_row<TO, N>(p, (unsigned)(v0 + k), cols, acc);
+    }
+    if (p.accumulate || !cols.active) return;
+    RawVec<TO, N> zero;
+#pragma unroll
+    for (int q = 0; q < N; ++q) zero.v[q] = (TO)0.f;
+    for (int i = g; i < width; i += GROUPS)
+        if (first[i] == DIRECT_NONE) vec_store<TO, N>((TO *)p.out + (v0 + i) * p.ld_out + cols.c, zero);
 }
 
 // Runs over several chunks: the workgroup of the chunk in which a run begins adds up its parts and writes the row.  All threads look how

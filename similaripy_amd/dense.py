@@ -250,8 +250,10 @@ def embed_rows_grad(grad: torch.Tensor, indices: torch.Tensor, n_vocab: int, ind
         raise ValueError(f"the result must be {grad.dtype} or float32, got {dtype}")
     res = _out("out", out, (n_vocab, dim), dtype, grad.device, (grad, False))
     a = _embed_args(grad, res, indices, indptr, data, n_rows, n_vocab, dim, float(scale), 1 if accumulate else 0)
-    ws = torch.empty(_abi.call_dense("sp_embed_rows_grad_workspace_bytes", a), dtype=torch.uint8, device=grad.device)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    need = _abi.call_dense("sp_embed_rows_grad_workspace_bytes", a)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=grad.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
     _abi.call_dense("sp_embed_rows_grad", a)
     return res
 

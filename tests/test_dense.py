@@ -166,6 +166,7 @@ def test_embed_rows_outside_indptr_are_not_read():
 
 GRADS = [  # n, vocab, mean entries of a row (0: lookup), share of bad ids
     (1, 1, 0, 0.0), (1, 700, 0, 0.0), (2, 3, 0, 0.5), (777, 50, 0, 0.05), (5000, 3, 0, 0.0), (9001, 70_000, 0, 0.01),
+    (1024, 90_000, 0, 0.1), (1025, 5000, 0, 0.1), (1000, 5, 0, 0.2), (8192, 2000, 0, 0.0), (8193, 2000, 0, 0.0), (60, 3000, 15, 0.1),
     (1, 40, 5, 0.0), (300, 511, 30, 0.1), (300, 512, 30, 0.1), (64, 300_000, 20, 0.0), (900, 7, 60, 0.0),
 ]
 
@@ -767,9 +768,9 @@ def test_c_entries_refuse():
         a.n_rows = -1
         assert _c(symbol, a)[0] == -1
     e = _abi.SpEmbedArgs()
-    e.n_rows, e.nnz, e.dim, e.n_vocab = 4, 3, 2, 5
+    e.n_rows, e.nnz, e.dim, e.n_vocab = 4000, 3999, 2, 5
     assert "nnz must equal n_rows" in _c("sp_embed_rows", e)[1]
-    e.nnz = 4
+    e.nnz = 4000
     assert "NULL indices" in _c("sp_embed_rows", e)[1]
     e.indices = 64
     assert "NULL table" in _c("sp_embed_rows", e)[1]
