@@ -99,6 +99,8 @@ EmbedParams embed_params(const sp_embed_args *a) {
     return p;
 }
 
+constexpr i64 L2_BYTES = 4 << 20;     // of an XCD
+constexpr i64 FEW_BAGS = 8192;        // one wave each does not fill the card
 constexpr int FILL_WGS = 512;      // workgroups that clear rows
 
 int run_embed(const sp_embed_args *a) {
@@ -112,18 +114,35 @@ int run_embed(const sp_embed_args *a) {
             HIP_TRY(hipGetLastError());
             return (int)SP_OK;
         }
-        return with_group<T>(a->dim, [&](auto gc, auto nc) {
+        auto run = [&](auto gc, auto nc, int by_xcd) {
             constexpr int G = decltype(gc)::value, N = decltype(nc)::value;
             EmbedParams p = embed_params(a);
             p.slabs = (int)ceil_div(a->dim, G * N);
-            const i64 blocks = a->indptr ? ceil_div(a->n_rows * p.slabs, 4) : ceil_div(a->n_rows * p.slabs, 256 / G);
+            p.by_xcd = by_xcd;
+            const i64 fours = ceil_div(a->n_rows, 4);          // bags: a workgroup takes four rows of a slab
+            const i64 blocks = !a->indptr ? ceil_div(a->n_rows * p.slabs, 256 / G) : by_xcd ? ceil_div(fours, 8 / p.slabs) * 8 : fours * p.slabs;
             if (blocks > I32_MAX) return fail(SP_EINVAL, "too many rows for one launch");
             auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p); };
             if (a->indptr) a->index64 ? launch(sp_embed_rows_kernel<T, i64, G, N>) : launch(sp_embed_rows_kernel<T, int, G, N>);
             else a->index64 ? launch(sp_embed_lookup_kernel<T, i64, G, N>) : launch(sp_embed_lookup_kernel<T, int, G, N>);
             HIP_TRY(hipGetLastError());
             return (int)SP_OK;
-        });
+        };
+        // Slabs of whole cache lines, one per XCD or per two or four of them: for a table beyond the L2 of an XCD whose rows are wide and from
+        // which more rows are taken than it has, and for few bags.
+        constexpr int N = VecOf<T>::N;
+        const i64 row_bytes = a->dim * (i64)sizeof(T), lanes = a->dim / N;
+        const bool large = a->nnz >= a->n_vocab && a->n_vocab * row_bytes > L2_BYTES && row_bytes >= 1024;
+        if (a->indptr && (large || a->n_rows <= FEW_BAGS) && a->ld_src * (i64)sizeof(T) % 128 == 0 && (uintptr_t)a->src % 128 == 0) {
+            int slabs = 8;
+            while (slabs > 1 && row_bytes % (128 * slabs) != 0) slabs /= 2;
+            const std::integral_constant<int, N> n;
+            if (slabs > 1 && lanes == 8 * slabs) return run(std::integral_constant<int, 8>(), n, 1);
+            if (slabs > 1 && lanes == 16 * slabs) return run(std::integral_constant<int, 16>(), n, 1);
+            if (slabs > 1 && lanes == 32 * slabs) return run(std::integral_constant<int, 32>(), n, 1);
+            if (slabs > 1 && lanes == 64 * slabs) return run(std::integral_constant<int, 64>(), n, 1);
+        }
+        return with_group<T>(a->dim, [&](auto gc, auto nc) { return run(gc, nc, 0); });
     });
 }
 

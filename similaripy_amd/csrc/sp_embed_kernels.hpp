@@ -19,6 +19,7 @@ struct EmbedParams {
     int dim, index64, accumulate;
     float scale;
     int slabs;              // column slabs of a row: ceil(dim / (G * N))
+    int by_xcd;             // bags: slab s is the work of the XCDs s, s + slabs, .. (slabs divides 8)
 };
 
 // The columns of a lane: N of them from c on, of rows of at least N.  The last lane of a row moves back to the row's last N columns instead
@@ -61,16 +62,29 @@ template <typename T, typename I, int G, int N> __global__ __launch_bounds__(256
     put<T, N>((T *)p.out + row * p.ld_out + cols.c, v);
 }
 
-// Bags: one wave per row and slab.  Its 64 / G groups take the row's entries in turn; 64 ids and weights are read at once, a lane each, and
+// Bags: one wave per row and slab.  What bounds it is the lines of the table that the L2 of an XCD (4 MB) does not hold and the latency of
+// the others: 65 536 bags of 64 out of 100 000 rows of 512 B (Zipf 0.9) read 2.1 GB, half of it past L2, in 184 us.  A large table of wide
+// rows is cut by columns, so that each XCD works on one slab only and holds that many times more rows of it; few rows are cut so that
+// there are waves enough.  (16 384 bags, rows of 2 KB: 245 -> 182 us with eight slabs; 4000 bags, rows of 512 B: 60 -> 27 with four; 65 536
+// bags: 512 B 186 -> 179, 256 B 103 -> 106, a table of 10 MB 142 -> 154, which is why those stay whole.)
+// A wave's 64 / G groups take the row's entries in turn; 64 ids and weights are read at once, a lane each, and
 // U rows of the table are on their way per group (an id outside the table reads row 0 and adds nothing).
 template <typename T, typename I, int G, int N> __global__ __launch_bounds__(256) void sp_embed_rows_kernel(EmbedParams p) {
     constexpr int S = 64 / G, U = 8;
     static_assert(S * U <= 64, "a round stays inside the 64 entries read at once");
-    const int lane = threadIdx.x & 63, sub = lane / G;
-    const i64 item = (i64)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const i64 row = item / p.slabs;
+    const int lane = threadIdx.x & 63, sub = lane / G, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    i64 row;
+    int slab;
+    if (p.by_xcd) {                                            // workgroups are dealt to the eight XCDs in turn
+        const int xcd = (int)(blockIdx.x % 8);
+        slab = xcd % p.slabs;
+        row = ((i64)(blockIdx.x / 8) * (8 / p.slabs) + xcd / p.slabs) * 4 + wave;
+    } else {
+        slab = (int)(blockIdx.x % p.slabs);
+        row = (i64)(blockIdx.x / p.slabs) * 4 + wave;
+    }
     if (row >= p.n_rows) return;
-    const Columns<N> cols(((int)(item % p.slabs) * G + (lane & (G - 1))) * N, p.dim);
+    const Columns<N> cols((slab * G + (lane & (G - 1))) * N, p.dim);
     const I *ids = (const I *)p.indices;
     const i64 b = max((i64)0, (i64)((const I *)p.indptr)[row]), e = min(p.nnz, (i64)((const I *)p.indptr)[row + 1]);
     float acc[N];
@@ -103,14 +117,29 @@ template <typename T, typename I, int G, int N> __global__ __launch_bounds__(256
             }
         }
     }
+    // The groups' sums: while a lane holds several columns, two groups share them out (each sends the half it gives up); then they add.
+    int first = 0;
+    bool mine_alone = true;
 #pragma unroll
-    for (int d = G; d < 64; d <<= 1)
+    for (int d = G, held = N; d < 64; d <<= 1, held = held > 1 ? held / 2 : 1) {
+        const bool upper = (lane & d) != 0;
+        if (held > 1) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += __shfl_xor(acc[k], d, 64);
-    if (sub == 0 && cols.active) {
+            for (int k = 0; k < held / 2; ++k) {
+                const float give = upper ? acc[k] : acc[k + held / 2], keep = upper ? acc[k + held / 2] : acc[k];
+                acc[k] = keep + __shfl_xor(give, d, 64);
+            }
+            first += upper ? held / 2 : 0;
+        } else {
+            acc[0] += __shfl_xor(acc[0], d, 64);
+            mine_alone = mine_alone && !upper;
+        }
+    }
+    if (mine_alone && cols.active) {
+        constexpr int LEFT = N > S ? N / S : 1;
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] *= p.scale;
-        put<T, N>((T *)p.out + row * p.ld_out + cols.c, acc);
+        for (int k = 0; k < LEFT; ++k) acc[k] *= p.scale;
+        put<T, LEFT>((T *)p.out + row * p.ld_out + cols.c + first, acc);
     }
 }
 
