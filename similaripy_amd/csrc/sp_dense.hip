@@ -350,8 +350,6 @@ int allow_lds(const void *kernel, size_t bytes) {
     if (bytes > 48 * 1024) HIP_TRY(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     return SP_OK;
 }
-size_t list_bytes(const sp_distill_args *a) { return (size_t)ListLds::list_room(a->k) * 16; }
-
 constexpr i64 SCAN_WGS = 1024, GRAD_WGS = 2048;
 constexpr i64 LDS_BYTES = 163840;   // of a CU
 constexpr i64 FUSED_ROWS = 256;      // from as many rows on a workgroup per row fills the card
@@ -359,7 +357,7 @@ constexpr i64 FUSED_ROWS = 256;      // from as many rows on a workgroup per row
 int launch_scan(const sp_distill_args *a, DistillParams p, hipStream_t stream) {
     p.splits = splits_of(a, SCAN_WGS);
     p.chunk = chunk_of(a, p.splits);
-    const size_t lists = list_bytes(a);
+    const size_t lists = (size_t)ListLds::loss_bytes(a->k);
     return with_type(a->dtype, [&](auto tag) {
         using T = decltype(tag);
         TRY(allow_lds((const void *)sp_distill_scan_kernel<T, DI_NT>, lists));
@@ -375,7 +373,7 @@ int launch_grad(const sp_distill_args *a, DistillParams p, hipStream_t stream) {
     p.chunk = chunk_of(a, p.splits);
     return with_type(a->dtype, [&](auto tag) {
         using T = decltype(tag);
-        const size_t lists = list_bytes(a);
+        const size_t lists = (size_t)ListLds::grad_bytes(a->k, DI_NT);
         TRY(allow_lds((const void *)sp_distill_grad_kernel<T, DI_NT>, lists));
         hipLaunchKernelGGL((sp_distill_grad_kernel<T, DI_NT>), dim3((unsigned)(a->n_rows * p.splits)), dim3(DI_NT), lists, stream, p);
         HIP_TRY(hipGetLastError());
@@ -504,21 +502,24 @@ int sp_distill_loss_grad(const sp_distill_args *a) {
         using T = decltype(tag);
         // The row in registers and LDS, by the smallest kind of workgroup that holds all of it: 8 of 256 threads on a CU, 4 or 2 of 512, one
         // of 1024; the last one takes longer rows as well, and reads the rest twice.
-        const i64 vecs = a->n_cols / VecOf<T>::N, lists = (i64)list_bytes(a);
-        auto launch = [&](auto kernel, i64 kept, i64 room) {
-            p.stage = (int)(vecs <= kept ? 0 : vecs - kept < room ? vecs - kept : room);
-            const size_t lds = (size_t)(lists + (i64)p.stage * 16);
+        const i64 vecs = a->n_cols / VecOf<T>::N;
+        auto room = [&](int nt, int wgs) {                     // vectors in a share of the LDS
+            const i64 r = (LDS_BYTES / wgs - ListLds::grad_bytes(a->k, nt) - 512) / 16;
+            return r < 0 ? (i64)0 : r;
+        };
+        auto launch = [&](auto kernel, int nt, int rv, int wgs) {
+            const i64 more = vecs - (i64)nt * rv;
+            p.stage = (int)(more < 0 ? 0 : more < room(nt, wgs) ? more : room(nt, wgs));
+            const size_t lds = (size_t)(ListLds::grad_bytes(a->k, nt) + (i64)p.stage * 16);
             TRY(allow_lds((const void *)kernel, lds));
-            hipLaunchKernelGGL(kernel, dim3((unsigned)a->n_rows), dim3((unsigned)p.threads), lds, stream, p);
+            hipLaunchKernelGGL(kernel, dim3((unsigned)a->n_rows), dim3((unsigned)nt), lds, stream, p);
             HIP_TRY(hipGetLastError());
             return (int)SP_OK;
         };
-        auto room = [&](int wgs) { const i64 r = (LDS_BYTES / wgs - lists - 512) / 16; return r < 0 ? (i64)0 : r; };      // vectors in a share of the LDS
-        if (vecs <= 4 * 256 + room(8)) { p.threads = 256; return launch(sp_distill_loss_grad_kernel<T, 256, 4>, 4 * 256, room(8)); }
-        if (vecs <= 4 * 512 + room(4)) { p.threads = 512; return launch(sp_distill_loss_grad_kernel<T, 512, 4>, 4 * 512, room(4)); }
-        if (vecs <= 16 * 512 + room(2)) { p.threads = 512; return launch(sp_distill_loss_grad_kernel<T, 512, 16>, 16 * 512, room(2)); }
-        p.threads = 1024;
-        return launch(sp_distill_loss_grad_kernel<T, 1024, 16>, 16 * 1024, room(1));
+        if (vecs <= 4 * 256 + room(256, 8)) return launch(sp_distill_loss_grad_kernel<T, 256, 4>, 256, 4, 8);
+        if (vecs <= 4 * 512 + room(512, 4)) return launch(sp_distill_loss_grad_kernel<T, 512, 4>, 512, 4, 4);
+        if (vecs <= 16 * 512 + room(512, 2)) return launch(sp_distill_loss_grad_kernel<T, 512, 16>, 512, 16, 2);
+        return launch(sp_distill_loss_grad_kernel<T, 1024, 16>, 1024, 16, 1);
     });
 }
 

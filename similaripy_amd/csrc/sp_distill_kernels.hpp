@@ -27,7 +27,7 @@ struct DistillParams {
     int splits;                        // workgroups of a row
     i64 chunk;                         // columns of one of them (a multiple of the vector)
     float *part;                       // [n_rows, splits, 2] maximum, sum
-    int threads, stage;                // the one-call kernel: threads of a workgroup, vectors of a row that it keeps in LDS
+    int stage;                         // vectors of a row that the one-call kernel keeps in LDS
 };
 
 // maximum and sum of exp2((z - max) c) of some columns
@@ -140,13 +140,16 @@ template <typename T, int NT> __device__ __forceinline__ MaxSum scan_columns(con
     return a;
 }
 
-// A row's list in LDS: columns (-1: not in the list), probabilities, the student's scores there, probabilities with the entries of equal
-// columns added up.  Room for k rounded up to whole vectors of 4; the slots behind the k-th are not in the list.
+// A row's list in LDS: columns (-1: not in the list), probabilities, the student's scores there; for the gradient also the entries of
+// every thread, those whose columns it writes, as a chain from head[thread] over next.
 struct ListLds {
     int *col;
-    float *prob, *z, *sum;
-    __device__ __forceinline__ ListLds(int *mem, int k) : col(mem), prob((float *)(mem + list_room(k))), z((float *)(mem + 2 * list_room(k))), sum((float *)(mem + 3 * list_room(k))) {}
-    static __host__ __device__ constexpr int list_room(int k) { return (k + 3) / 4 * 4; }
+    float *prob, *z;
+    int *next, *head;
+    __device__ __forceinline__ ListLds(int *mem, int k) : col(mem), prob((float *)(mem + room(k))), z((float *)(mem + 2 * room(k))), next(mem + 3 * room(k)), head(mem + 4 * room(k)) {}
+    static __host__ __device__ constexpr int room(int k) { return (k + 3) / 4 * 4; }
+    static __host__ __device__ constexpr int loss_bytes(int k) { return 12 * room(k); }
+    static __host__ __device__ constexpr int grad_bytes(int k, int threads) { return 16 * room(k) + 4 * threads; }
 };
 // The teacher's list of a row, by the 64 lanes of one wave, with S = sum p_j log p_j and P = sum p_j.  Nothing here depends on the row's
 // maximum and sum.  256 entries are requested at once, then the student's scores at all of their columns.
@@ -155,12 +158,12 @@ struct ListSums {
 };
 template <typename T> __device__ __forceinline__ ListSums list_sums(const DistillParams &p, i64 row, const T *z, const ListLds &list) {
     constexpr int R = 4;
-    const int lane = threadIdx.x & 63, room = ListLds::list_room(p.k);
+    const int lane = threadIdx.x & 63;
     int n = p.counts ? p.counts[row] : p.k;
     n = n < 0 ? 0 : n > p.k ? p.k : n;
     const i64 base = row * p.k;
     float top = NEG_INF;
-    for (int j0 = lane; j0 < room; j0 += 64 * R) {
+    for (int j0 = lane; j0 < p.k; j0 += 64 * R) {
         i64 col[R];
         float t[R], zc[R];
 #pragma unroll
@@ -186,7 +189,7 @@ template <typename T> __device__ __forceinline__ ListSums list_sums(const Distil
 #pragma unroll
         for (int u = 0; u < R; ++u) {
             const int j = j0 + 64 * u;
-            if (j < room) {
+            if (j < p.k) {
                 list.col[j] = (int)col[u];
                 list.prob[j] = t[u];
                 list.z[j] = zc[u];
@@ -207,7 +210,7 @@ template <typename T> __device__ __forceinline__ ListSums list_sums(const Distil
         shift = sum > 0.f || sum != sum ? -logf(sum) : NEG_INF;       // (nothing in the list, or -inf only: all p_j are 0)
     }
     ListSums r{0.f, 0.f};
-    for (int j = lane; j < room; j += 64) {
+    for (int j = lane; j < p.k; j += 64) {
         float prob = 0.f;
         if (list.col[j] >= 0) {
             const float logp = top == NEG_INF ? NEG_INF : __fmaf_rn(list.prob[j] - top, p.inv_tau, shift);
@@ -230,34 +233,46 @@ __device__ __forceinline__ float list_loss(const DistillParams &p, ListSums l, M
         if (list.prob[j] != 0.f) cross += list.prob[j] * (list.z[j] == NEG_INF ? NEG_INF : __fmaf_rn(list.z[j] - high, p.inv_tau, -logs));
     return p.tau * p.tau * (l.plogp - wave_sum(cross));
 }
-// Entries of the same column become one: the first one keeps their sum, the others leave the list.  By all NT threads, between barriers;
-// four columns are read per access, the same ones by all lanes.
-template <int NT> __device__ __forceinline__ void merge_listed(int k, const ListLds &list) {
-    const int4 *col4 = (const int4 *)list.col;
-    for (int j = threadIdx.x; j < k; j += NT) {
+// The chains, by the wave that has made the list: column c of [c0, c1) is in the chain of the thread that writes it with the row, vector by
+// vector ((c - c0) / N) % NT, from column `tail` on one by one.  (What a thread writes twice ends as the later of its two stores: no barrier
+// lies between the row's vectors and the listed columns.)
+template <int NT, int N> __device__ __forceinline__ void chain_listed(int k, i64 c0, i64 c1, i64 tail, const ListLds &list) {
+    const int lane = threadIdx.x & 63;
+    for (int i = lane; i < NT; i += 64) list.head[i] = -1;
+    for (int j = lane; j < k; j += 64) {
         const int c = list.col[j];
-        int first = j;
-        unsigned same = 0;                                     // how many entries name the column
-#pragma unroll 4
-        for (int i = 0; i < ListLds::list_room(k) / 4; ++i) {
-            const int4 q = col4[i];
-            const unsigned hits = (unsigned)(q.x == c) | (unsigned)(q.y == c) << 1 | (unsigned)(q.z == c) << 2 | (unsigned)(q.w == c) << 3;
-            if (hits) {
-                if (same == 0) first = 4 * i + __builtin_ctz(hits);
-                same += __popc(hits);
+        if (c >= c0 && c < c1) list.next[j] = atomicExch(&list.head[c >= tail ? (int)(c - tail) : (int)((unsigned)(c - c0) / N % NT)], j);
+    }
+}
+// The listed columns of this thread once more, with their probabilities taken off.  Entries of the same column are in the same chain; the
+// first one of the list writes their sum, added up in the order of the list.
+template <typename T, typename F> __device__ __forceinline__ void write_listed(int k, T *d, F one, float gt, const ListLds &list) {
+    const int head = list.head[threadIdx.x];
+    for (int j = head; j >= 0; j = list.next[j]) {
+        const int c = list.col[j];
+        bool first = true, again = false;
+        for (int i = list.next[j]; i >= 0 && first; i = list.next[i])
+            if (list.col[i] == c) {
+                again = true;
+                first = i > j;
             }
-        }
+        for (int i = head; i != j && first; i = list.next[i])
+            if (list.col[i] == c) {
+                again = true;
+                first = i > j;
+            }
+        if (!first) continue;
         float prob = list.prob[j];
-        if (same > 1 && first == j) {                          // (hardly ever: added up in the order of the list)
+        if (again) {
             prob = 0.f;
             for (int i = j; i < k; ++i)
                 if (list.col[i] == c) prob += list.prob[i];
         }
-        list.sum[j] = first == j ? prob : -1.f;                // (probabilities are not negative; NaN stays)
+        d[c] = (T)(one(list.z[j]) - gt * prob);
     }
 }
 
-// (16 bytes aligned: the list's columns and the one-call kernel's vectors are read as such)
+// (16 bytes aligned: the one-call kernel's vectors are read as such)
 extern __shared__ __align__(16) int distill_list[];
 
 template <typename T> __device__ __forceinline__ void finish_loss(const DistillParams &p, i64 row, MaxSum a) {
@@ -295,15 +310,6 @@ __device__ __forceinline__ MaxSum join_parts(const DistillParams &p, i64 row) {
 
 // rows in several pieces: one wave joins them
 template <typename T> __global__ __launch_bounds__(64) void sp_distill_join_kernel(DistillParams p) { finish_loss<T>(p, blockIdx.x, join_parts(p, blockIdx.x)); }
-
-// the listed columns of [c0, c1) once more, with their probabilities taken off
-template <typename T, int NT, typename F>
-__device__ __forceinline__ void write_listed(const DistillParams &p, T *d, i64 c0, i64 c1, F one, float gt, const ListLds &list) {
-    for (int j = threadIdx.x; j < p.k; j += NT) {
-        const int c = list.col[j];
-        if (c >= c0 && c < c1 && !(list.sum[j] < 0.f)) d[c] = (T)(one(list.z[j]) - gt * list.sum[j]);
-    }
-}
 
 // The gradient of columns [c0, c1) of a row by the NT threads of a workgroup: g tau P q everywhere, then the listed columns once
 // more with their probabilities taken off.  The list keeps the scores at its columns: they have been read before
@@ -350,8 +356,7 @@ __device__ __forceinline__ void grad_columns(const DistillParams &p, i64 row, i6
     }
     for (int j = 0; j < N; ++j)
         if (i + j < c1) d[i + j] = (T)one(up(z[i + j]));
-    __syncthreads();
-    write_listed<T, NT>(p, d, c0, c1, one, gt, list);
+    write_listed(p.k, d, one, gt, list);
 }
 
 template <typename T, int NT> __global__ __launch_bounds__(NT) void sp_distill_grad_kernel(DistillParams p) {
@@ -360,13 +365,12 @@ template <typename T, int NT> __global__ __launch_bounds__(NT) void sp_distill_g
     const i64 row = blockIdx.x / p.splits, c0 = (blockIdx.x % p.splits) * p.chunk, c1 = min(p.n_cols, c0 + p.chunk);
     if (threadIdx.x < 64) {
         const ListSums l = list_sums<T>(p, row, (const T *)p.student + row * p.ld_student, list);
+        chain_listed<NT, VecOf<T>::N>(p.k, c0, c1, c1, list);
         if (threadIdx.x == 0) mass = l.mass;
     }
     const MaxSum a{p.stats[2 * row], p.stats[2 * row + 1]};
     const float gt = (p.grad_loss ? p.grad_loss[row] : 1.f) * p.tau;
-    __syncthreads();
-    merge_listed<NT>(p.k, list);
-    __syncthreads();
+    __syncthreads();                                           // (every listed score has been read: `grad` may be `student`)
     grad_columns<T, NT>(p, row, c0, c1, a, mass, gt, list);
 }
 
@@ -387,7 +391,7 @@ template <typename T, int NT, int RV> __global__ __launch_bounds__(NT, RV <= 4 ?
     __shared__ MaxSum sh[NT / 64];
     __shared__ float mass_of_row;
     const ListLds list(distill_list, p.k);
-    RawVec<T, N> *stage = (RawVec<T, N> *)(distill_list + 4 * ListLds::list_room(p.k));
+    RawVec<T, N> *stage = (RawVec<T, N> *)(distill_list + 4 * ListLds::room(p.k) + NT);
     const i64 row = blockIdx.x;
     const int tid = threadIdx.x, n_cols = (int)p.n_cols, vecs = n_cols / N;
     const int kept = min(vecs, RV * NT + p.stage);             // vectors that are not read again
@@ -397,6 +401,7 @@ template <typename T, int NT, int RV> __global__ __launch_bounds__(NT, RV <= 4 ?
     ListSums l{0.f, 0.f};
     if (tid < 64) {                                            // (one wave is a little late; what it does is in nobody's way then)
         l = list_sums<T>(p, row, z, list);
+        chain_listed<NT, N>(p.k, 0, n_cols, (i64)vecs * N, list);
         if (tid == 0) mass_of_row = l.mass;
     }
     RawVec<T, N> x[RV];
@@ -433,12 +438,7 @@ template <typename T, int NT, int RV> __global__ __launch_bounds__(NT, RV <= 4 ?
     }
     MaxSum a = block_join<NT>(finish(run, p.c), p.c, sh);
     if (!off_fits(a.m, p.c)) a = rescan<T, NT>(z, 0, n_cols, a, p.c, sh);
-    if (tid < 64 && p.loss) {
-        const float loss = list_loss(p, l, a, list);
-        if (tid == 0) p.loss[row] = loss;
-    }
-    merge_listed<NT>(p.k, list);
-    __syncthreads();                                           // (from here on `grad` is written, which may be `student`)
+    // (the barrier in block_join: the row and the listed scores have been read; from here on `grad` is written, which may be `student`)
 #pragma unroll
     for (int q = 0; q < RV; ++q) forget(x[q]);                 // (or the scores stay unpacked in registers, which there are not enough of)
     const float mass = mass_of_row, gt = (p.grad_loss ? p.grad_loss[row] : 1.f) * p.tau;
@@ -453,14 +453,18 @@ template <typename T, int NT, int RV> __global__ __launch_bounds__(NT, RV <= 4 ?
         vec_store<T, N>(d + (i64)j * N, o);
     };
     // (what has to be read again goes first: nothing of it has been written yet)
-    for (int j = kept + tid; j < vecs; j += NT) put(j, vec_load<T, N>(z + (i64)j * N));
+    for (int j = RV * NT + tid; j < vecs; j += NT)
+        if (j >= kept) put(j, vec_load<T, N>(z + (i64)j * N));
 #pragma unroll
     for (int q = 0; q < RV; ++q)
         if (q * NT + tid < vecs) put(q * NT + tid, x[q]);
     for (int j = RV * NT + tid; j < kept; j += NT) put(j, stage[j - RV * NT]);
     if (end < n_cols) d[end] = (T)one(lone);
-    __syncthreads();
-    write_listed<T, NT>(p, d, 0, n_cols, one, gt, list);
+    write_listed(p.k, d, one, gt, list);
+    if (tid < 64 && p.loss) {
+        const float loss = list_loss(p, l, a, list);
+        if (tid == 0) p.loss[row] = loss;
+    }
 }
 
 }  // namespace

@@ -552,6 +552,27 @@ def test_distill_row_of_the_lowest_value(dtype, n, v, tau):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v", [(300, 4099), (300, 4103), (5, 4103), (260, 7), (260, 40_013)])
+def test_distill_every_listed_place(dtype, n, v):
+    """Listed columns at the row's first and last places, at the borders of vectors and pieces, named once, twice and many times: each is
+    written after the vector it lies in."""
+    rng = np.random.default_rng(v)
+    k = 64
+    places = np.concatenate([np.arange(v - min(v, 12), v), np.arange(min(v, 9)), [v // 2, v // 2, v // 2 + 1], rng.integers(0, v, k)])[:k]
+    cols = torch.from_numpy(np.stack([rng.permutation(places) for _ in range(n)]).astype(np.int64))
+    cols[1] = v - 1                                                               # one column, k times
+    values = torch.from_numpy(rng.standard_normal((n, k)).astype(np.float32))
+    z = torch.from_numpy(rng.standard_normal((n, v)) * 2).to(dtype).cuda()
+    ref = distill_ref(z, cols, values, None, 1.0, None, None)
+    grad_b = distill_bounds(z, cols, 1.0, ref, None, dtype)[1]
+    loss, stats = dense.distill_loss(z, cols.cuda(), values.cuda(), return_stats=True)
+    check(dense.distill_grad(z, stats, cols.cuda(), values.cuda()), ref[2], grad_b)
+    for _ in range(3):
+        check(dense.distill_loss_grad(z, cols.cuda(), values.cuda())[1], ref[2], grad_b)
+
+
+@gpu
 def test_distill_sizes_of_nothing():
     z = torch.randn(3, 50, device="cuda")
     none = torch.zeros(3, 0, dtype=torch.int32, device="cuda")
