@@ -173,8 +173,11 @@ __device__ __forceinline__ void fill_share(const FillParams &f, int block, int b
         for (; i + 16 <= total; i += step) *(Quad *)(out + i) = zero;
         for (; i < total && i + 16 > total; i += 2) *(unsigned short *)(out + i) = 0;
     } else {
-        for (i64 r = block; r < r1 - r0; r += blocks)
-            for (i64 c = (i64)threadIdx.x * 2; c < width; c += blockDim.x * 2) *(unsigned short *)(out + r * ld + c) = 0;
+        for (i64 r = block; r < r1 - r0; r += blocks) {
+            i64 c = (i64)threadIdx.x * 16;
+            for (; c + 16 <= width; c += (i64)blockDim.x * 16) *(Quad *)(out + r * ld + c) = zero;
+            for (; c < width && c + 16 > width; c += 2) *(unsigned short *)(out + r * ld + c) = 0;
+        }
     }
 }
 template <int NT> __global__ __launch_bounds__(NT) void sp_fill_kernel(FillParams f) { fill_share(f, blockIdx.x, gridDim.x); }
