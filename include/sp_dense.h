@@ -84,7 +84,7 @@ typedef struct sp_adjust_args {
     int32_t  device;
     int32_t  dtype;            /* SP_DT_* of scores and out */
     int64_t  n_rows;
-    int64_t  n_cols;           /* < 2^31 */
+    int64_t  n_cols;           /* < 2^31 - 65536 */
     int64_t  ld_scores;        /* elements between rows */
     int64_t  ld_out;
     const void *scores;        /* [n_rows, n_cols] */
@@ -118,7 +118,7 @@ typedef struct sp_distill_args {
     int32_t  device;
     int32_t  dtype;            /* SP_DT_* of student and grad */
     int64_t  n_rows;
-    int64_t  n_cols;           /* < 2^31 */
+    int64_t  n_cols;           /* < 2^31 - 65536 */
     int64_t  ld_student;
     int64_t  ld_grad;
     int32_t  k;                /* slots of a list, 0 .. SP_DISTILL_KMAX */

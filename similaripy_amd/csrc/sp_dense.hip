@@ -56,6 +56,7 @@ struct OnDevice {
 
 i64 ceil_div(i64 a, i64 b) { return (a + b - 1) / b; }
 constexpr i64 I32_MAX = 0x7FFFFFFFLL;
+constexpr i64 COLS_MAX = I32_MAX - 65536;      // column numbers a workgroup beyond the row's end are still int32
 bool bad_dtype(int d) { return d < SP_DT_F32 || d > SP_DT_F16; }
 
 // calls f with a value of the element type
@@ -307,7 +308,7 @@ int check_distill(const sp_distill_args *a, int what) {
     if (!a || a->struct_size != sizeof(sp_distill_args)) return fail(SP_EINVAL, "sp_distill_args size mismatch");
     if (a->flags) return fail(SP_EINVAL, "flags must be 0");
     if (bad_dtype(a->dtype) || bad_dtype(a->values_dtype)) return fail(SP_EINVAL, "bad dtype");
-    if (a->n_rows < 0 || a->n_rows > I32_MAX || a->n_cols < 0 || a->n_cols > I32_MAX) return fail(SP_EINVAL, "bad shape");
+    if (a->n_rows < 0 || a->n_rows > I32_MAX || a->n_cols < 0 || a->n_cols > COLS_MAX) return fail(SP_EINVAL, "bad shape");
     if (a->k < 0 || a->k > SP_DISTILL_KMAX) return fail(SP_EINVAL, "k = %d out of range [0, %d]", a->k, SP_DISTILL_KMAX);
     if (!(a->temperature > 0.f) || a->temperature > 1e30f || a->temperature < 1e-30f) return fail(SP_EINVAL, "temperature must be positive");
     if (a->n_rows == 0) return SP_OK;
@@ -433,7 +434,7 @@ int sp_adjust_scores(const sp_adjust_args *a) {
     if (!a || a->struct_size != sizeof(sp_adjust_args)) return fail(SP_EINVAL, "sp_adjust_args size mismatch");
     if (a->flags) return fail(SP_EINVAL, "flags must be 0");
     if (bad_dtype(a->dtype) || (a->bias && bad_dtype(a->bias_dtype))) return fail(SP_EINVAL, "bad dtype");
-    if (a->n_rows < 0 || a->n_rows > I32_MAX || a->n_cols < 0 || a->n_cols > I32_MAX) return fail(SP_EINVAL, "bad shape");
+    if (a->n_rows < 0 || a->n_rows > I32_MAX || a->n_cols < 0 || a->n_cols > COLS_MAX) return fail(SP_EINVAL, "bad shape");
     TRY(check_pattern(a->history, "history"));
     TRY(check_pattern(a->filter, "filter"));
     TRY(check_pattern(a->target, "target"));
