@@ -22,6 +22,7 @@ Autograd and graph capture: inside a capture the functions that build an autogra
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -135,12 +136,23 @@ def _no_grad_here(name: str, t) -> None:
         raise ValueError(f"{name} builds no autograd graph: detach its inputs or call it under torch.no_grad()")
 
 
+def _fixed(name: str, t) -> None:
+    """An operand that gets no gradient, checked before an autograd graph is built (inside one, grad mode is off)."""
+    if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} has no gradient here: detach it")
+
+
 def _not_capturing(name: str, instead: str) -> None:
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{name} on tensors that require a gradient cannot be captured into a graph: capture {instead} on detached tensors")
 
 
 # ---- embedding rows ------------------------------------------------------------------------------------------------------------
+
+def _rows(t):
+    """All but the last dimension as one (reshape(-1, d) does not work for d = 0)."""
+    return t if t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+
 
 def _csr_of(indices, indptr, data, device):
     """(indices, indptr, data, rows, output shape without the last dimension)."""
@@ -169,6 +181,8 @@ def _embed_args(src, out, indices, indptr, data, n_rows, n_vocab, dim, scale, ac
 def _embed_forward(table, indices, indptr, data, scale, out):
     indices, indptr, data, n_rows, lead = _csr_of(indices, indptr, data, table.device)
     dim = table.shape[1]
+    if out is not None and not isinstance(out, torch.Tensor):
+        raise TypeError(f"out must be a torch.Tensor, got {type(out).__name__}")
     if out is not None and tuple(out.shape) != lead + (dim,):
         raise ValueError(f"out must have shape {lead + (dim,)}, got {tuple(out.shape)}")
     flat = None if out is None else out.view(n_rows, dim) if out.dim() != 2 else out
@@ -189,7 +203,7 @@ class _EmbedRows(torch.autograd.Function):
     def backward(ctx, grad):
         _not_capturing("embed_rows' backward pass", "embed_rows_grad")
         indices, indptr, data = ctx.saved_tensors
-        grad = grad.reshape(-1, grad.shape[-1])
+        grad = _rows(grad)
         if grad.shape[1] > 1 and grad.stride(1) != 1:
             grad = grad.contiguous()
         return embed_rows_grad(grad, indices, ctx.n_vocab, indptr, data, scale=ctx.scale), None, None, None, None
@@ -210,6 +224,8 @@ def embed_rows(table: torch.Tensor, indices: torch.Tensor, indptr: Optional[torc
     """
     _dense("table", table)
     scale = float(scale)
+    if data is not None:
+        _fixed("data", data)
     if out is None and table.requires_grad and torch.is_grad_enabled():
         _not_capturing("embed_rows", "embed_rows and embed_rows_grad")
         return _EmbedRows.apply(table, indices, indptr, data, scale)
@@ -234,7 +250,7 @@ def embed_rows_grad(grad: torch.Tensor, indices: torch.Tensor, n_vocab: int, ind
     if not isinstance(grad, torch.Tensor):
         raise TypeError(f"grad must be a torch.Tensor, got {type(grad).__name__}")
     if indptr is None and grad.dim() != 2 and grad.dim() > 0:
-        grad = grad.reshape(-1, grad.shape[-1])
+        grad = _rows(grad)
     _dense("grad", grad)
     _no_grad_here("embed_rows_grad", grad)
     indices, indptr, data, n_rows, _ = _csr_of(indices, indptr, data, grad.device)
@@ -299,7 +315,7 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
     targets      [n] int32 / int64: the row of ``history``, ``filter_cols`` and ``target_cols`` each row of scores belongs to (absolute
                  row ids, as ``target_rows`` of the similarity functions); default ``0 .. n-1``.  A row outside a pattern is empty there.
     history      (indptr, indices) of a CSR pattern: ids in any order, repeats count, ids outside the columns are passed over
-    repetition, presence, frequency   a number, or one float32 per row
+    repetition, presence, frequency   a number, or one float32 per row (repetition positive)
     bias         [n_cols] or [n, n_cols], any of the three types
     allowed      int32 words of packed bits, [words] or [n, words] with ``words = ceil(n_cols / 32)``: column c stays where bit ``c % 32``
                  of word ``c // 32`` is set
@@ -371,6 +387,8 @@ def _distill_args(student, cols, values, counts, temperature, teacher_lse):
         raise TypeError(f"values must be a torch.Tensor, got {type(values).__name__}")
     if values.dtype not in _DT:
         raise TypeError(f"values must be float32, bfloat16 or float16, got {values.dtype}")
+    if values.dim() != 1 and n and values.shape != (n, k):
+        raise ValueError(f"values must have shape ({n}, {k}) or ({n * k},), got {tuple(values.shape)}")
     values = _floats("values", values, device, cols.numel(), values.dtype)
     if counts is not None:
         counts = _ints("counts", counts, device, (torch.int32,))
@@ -444,6 +462,9 @@ def distill_loss(student: torch.Tensor, cols: torch.Tensor, values: torch.Tensor
     return_stats also return [n, 2] float32, every row's maximum ``m`` and the sum of ``exp((student - m) / temperature)``, which
                  :func:`distill_grad` takes (their log-sum-exp ``m / temperature + log(sum)`` in two parts)
     """
+    _fixed("values", values)
+    if teacher_lse is not None:
+        _fixed("teacher_lse", teacher_lse)
     if isinstance(student, torch.Tensor) and student.requires_grad and torch.is_grad_enabled():
         _not_capturing("distill_loss", "distill_loss and distill_grad, or distill_loss_grad,")
         loss, stats = _DistillLoss.apply(student, cols, values, counts, float(temperature), teacher_lse)

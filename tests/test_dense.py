@@ -650,6 +650,80 @@ def test_run_together():
 
 
 @gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements in the table, its gradient, the scores: the last rows are where they belong."""
+    vocab, dim = 2_200_000, 1024
+    table = torch.zeros(vocab, dim, dtype=torch.bfloat16, device="cuda")
+    last = torch.randn(dim, device="cuda").to(torch.bfloat16)
+    table[-1], table[0] = last, 3.0
+    ids = torch.tensor([vocab - 1, 0, vocab - 1], device="cuda")
+    assert torch.equal(dense.embed_rows(table, ids)[2], last)
+    bag = dense.embed_rows(table, ids, torch.tensor([0, 1, 3], device="cuda"))
+    assert torch.equal(bag[0], last) and torch.equal(bag[1], (last.float() + 3.0).to(torch.bfloat16))
+    for n in (3, 3000, 12_000):                                                   # without a sort, by one workgroup, by all
+        many = ids.repeat(n // 3)
+        grad = dense.embed_rows_grad(torch.ones(n, dim, dtype=torch.bfloat16, device="cuda"), many, vocab, out=table)
+        assert (grad[-1] == float(n // 3 * 2)).all() and (grad[0] == float(n // 3)).all() and grad[1:-1:100_003].abs().max() == 0
+        assert grad[-2].abs().max() == 0
+    del table, grad
+    n, v = 27_000, 80_000
+    z = torch.zeros(n, v, dtype=torch.bfloat16, device="cuda")
+    z[-1, -1], z[-1, 5] = 2.0, -1.0
+    one = (torch.tensor([0, 2], dtype=torch.int32, device="cuda"), torch.tensor([v - 1, 5], dtype=torch.int32, device="cuda"))
+    where = torch.full((n,), -1, dtype=torch.int32, device="cuda")
+    where[-1] = 0
+    out = dense.adjust_scores(z, targets=where, history=one, repetition=4.0, out=z)
+    assert out[-1, -1].item() == 0.5 and out[-1, 5].item() == -4.0 and out[-1].count_nonzero().item() == 2 and out[0].count_nonzero().item() == 0
+    cols, values = torch.full((n, 1), v - 1, dtype=torch.int32, device="cuda"), torch.ones(n, 1, device="cuda")
+    row = z[-1].double().cpu()
+    loss, stats = dense.distill_loss(z, cols, values, return_stats=True)
+    assert abs(loss[-1].item() + (row[-1] - torch.logsumexp(row, 0)).item()) < 1e-4
+    want = torch.softmax(row, 0)
+    want[-1] -= 1.0
+    for grad in (dense.distill_grad(z, stats, cols, values, out=z.clone()), dense.distill_loss_grad(z, cols, values, out=z)[1]):
+        check(grad[-1], want, 2.0 ** -8 * want.abs() + 1e-8)
+
+
+@gpu
+def test_captured_large_rows():
+    """The kernel that keeps a row in LDS beyond what every kernel may have, and the sorted gradient, replayed."""
+    n, v = 300, 90_000
+    z = torch.randn(n, v, device="cuda")
+    cols, values = torch.randint(0, v, (n, 10), device="cuda"), torch.randn(n, 10, device="cuda")
+    ids, grad = torch.randint(0, 5000, (20_000,), device="cuda"), torch.randn(20_000, 30, device="cuda")
+
+    def both():
+        return (*dense.distill_loss_grad(z, cols, values), dense.embed_rows_grad(grad, ids, 5000))
+    both()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = both()
+    for seed in range(3):
+        for t in (z, grad):
+            t.copy_(torch.randn(t.shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda"))
+        g.replay()
+        want = both()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(res, want))
+
+
+@gpu
+def test_embed_shapes_of_nothing():
+    """Rows without columns, a single id without dimensions, through the graph as well."""
+    table = torch.zeros(5, 0, device="cuda", requires_grad=True)
+    out = dense.embed_rows(table, torch.zeros(2, 3, dtype=torch.int64, device="cuda"))
+    assert out.shape == (2, 3, 0)
+    out.sum().backward()
+    assert table.grad.shape == (5, 0)
+    table = torch.arange(12.0, device="cuda").view(4, 3).requires_grad_()
+    out = dense.embed_rows(table, torch.tensor(2, device="cuda"))
+    assert out.shape == (3,)
+    out.sum().backward()
+    assert table.grad[2].tolist() == [1.0, 1.0, 1.0] and table.grad.sum().item() == 3.0
+
+
+@gpu
 def test_replayed_graphs_share_nothing():
     """Two captured graphs, replayed alternately with eager work between them, give the eager results every time."""
     rng = np.random.default_rng(4)
@@ -854,6 +928,7 @@ def test_wrong_operands_on_a_device():
     ids = torch.zeros(3, dtype=torch.int64, device="cuda")
     i32 = torch.zeros(4, dtype=torch.int32, device="cuda")
     cols, vals = torch.zeros(4, 2, dtype=torch.int32, device="cuda"), torch.zeros(4, 2, device="cuda")
+    leaf = torch.zeros(4, 6, device="cuda", requires_grad=True)
     bad = [
         lambda: dense.embed_rows(z.T, ids), lambda: dense.embed_rows(z, ids.float()), lambda: dense.embed_rows(z, ids.cpu()),
         lambda: dense.embed_rows(z, ids, i32), lambda: dense.embed_rows(z, ids, None, vals), lambda: dense.embed_rows(z, ids, ids, vals[0, :1]),
@@ -871,7 +946,10 @@ def test_wrong_operands_on_a_device():
         lambda: dense.distill_loss(z.detach(), cols, vals, i32[:3]), lambda: dense.distill_loss(z.detach(), cols, vals, temperature=0.0),
         lambda: dense.distill_loss(z.detach(), cols, vals, temperature=math.nan), lambda: dense.distill_loss(z.detach(), cols, vals.double()),
         lambda: dense.distill_loss(z.detach(), torch.zeros(4, 4097, dtype=torch.int32, device="cuda"), torch.zeros(4, 4097, device="cuda")),
-        lambda: dense.distill_loss(z.detach(), cols, vals.clone().requires_grad_()), lambda: dense.distill_grad(z.detach(), torch.zeros(4, device="cuda"), cols, vals),
+        lambda: dense.distill_loss(z.detach(), cols, vals.clone().requires_grad_()), lambda: dense.distill_loss(leaf, cols, vals.clone().requires_grad_()),
+        lambda: dense.distill_loss(leaf, cols, vals, teacher_lse=torch.zeros(4, device="cuda").requires_grad_()),
+        lambda: dense.embed_rows(leaf, ids, torch.zeros(2, dtype=torch.int64, device="cuda"), torch.zeros(3, device="cuda").requires_grad_()),
+        lambda: dense.distill_loss(z.detach(), cols, vals.T.contiguous()), lambda: dense.embed_rows(z, ids, out=[1]), lambda: dense.distill_grad(z.detach(), torch.zeros(4, device="cuda"), cols, vals),
         lambda: dense.distill_loss_grad(z.detach(), cols, vals, grad_loss=torch.zeros(3, device="cuda")), lambda: dense.distill_loss(z.detach(), cols.T, vals.T),
     ]
     for i, f in enumerate(bad):
