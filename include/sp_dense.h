@@ -16,6 +16,10 @@
  * Every pointer is device memory on `device`; every call is asynchronous on `stream`, allocates nothing, leaves the
  * calling thread's current device as it was and may be captured into a graph.  `flags` is 0 (reserved).
  * Same conventions as sp_knn.h: plain pointers and sizes, 0 or a negative SP_E* code, sp_last_error().
+ * A launch has fewer than 2^32 threads: calls of more rows than that gives (2^23 of distillation, 2^24 of scores, 2^26
+ * of embedding rows of 1 KB and more) are refused with SP_EINVAL and have to be cut by the caller.
+ * A launch has fewer than 2^32 threads: calls of more rows than that gives (2^23 of distillation, 2^24 of scores, 2^26
+ * of embedding rows of 1 KB and more) are refused with SP_EINVAL and have to be cut by the caller.
  * Sums, row statistics and list probabilities are formed in 32 bits or more whatever the type of the tensors.
  */
 #ifndef SP_DENSE_H_

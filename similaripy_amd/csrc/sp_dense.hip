@@ -57,6 +57,8 @@ struct OnDevice {
 i64 ceil_div(i64 a, i64 b) { return (a + b - 1) / b; }
 constexpr i64 I32_MAX = 0x7FFFFFFFLL;
 constexpr i64 COLS_MAX = I32_MAX - 65536;      // column numbers a workgroup beyond the row's end are still int32
+// a launch has fewer than 2^32 threads
+bool too_many(i64 blocks, int threads) { return blocks > I32_MAX || blocks * threads > 0xFFFFFFFFLL; }
 bool bad_dtype(int d) { return d < SP_DT_F32 || d > SP_DT_F16; }
 
 // calls f with a value of the element type
@@ -96,7 +98,7 @@ EmbedParams embed_params(const sp_embed_args *a) {
     EmbedParams p{};
     p.in = a->src; p.indices = a->indices; p.indptr = a->indptr; p.data = a->data; p.out = a->out;
     p.n_rows = a->n_rows; p.n_vocab = a->n_vocab; p.nnz = a->nnz; p.ld_in = a->ld_src; p.ld_out = a->ld_out;
-    p.dim = (int)a->dim; p.index64 = a->index64; p.accumulate = a->accumulate; p.scale = a->scale;
+    p.dim = (int)a->dim; p.scale = a->scale;
     return p;
 }
 
@@ -122,7 +124,7 @@ int run_embed(const sp_embed_args *a) {
             p.by_xcd = by_xcd;
             const i64 fours = ceil_div(a->n_rows, 4);          // bags: a workgroup takes four rows of a slab
             const i64 blocks = !a->indptr ? ceil_div(a->n_rows * p.slabs, 256 / G) : by_xcd ? ceil_div(fours, 8 / p.slabs) * 8 : fours * p.slabs;
-            if (blocks > I32_MAX) return fail(SP_EINVAL, "too many rows for one launch");
+            if (too_many(blocks, 256)) return fail(SP_EINVAL, "too many rows for one launch");
             auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p); };
             if (a->indptr) a->index64 ? launch(sp_embed_rows_kernel<T, i64, G, N>) : launch(sp_embed_rows_kernel<T, int, G, N>);
             else a->index64 ? launch(sp_embed_lookup_kernel<T, i64, G, N>) : launch(sp_embed_lookup_kernel<T, int, G, N>);
@@ -211,7 +213,7 @@ template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a)
             constexpr int G = decltype(gc)::value, N = decltype(nc)::value;
             r.slabs = (int)ceil_div(a->dim, G * N);
             const i64 blocks = ceil_div(a->n_vocab, d.per) * r.slabs;
-            if (blocks > I32_MAX) return fail(SP_EINVAL, "too many rows for one launch");
+            if (too_many(blocks, 256)) return fail(SP_EINVAL, "too many rows for one launch");
             auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, d); };
             a->index64 ? launch(sp_embed_grad_direct_kernel<T, TO, i64, G, N>) : launch(sp_embed_grad_direct_kernel<T, TO, int, G, N>);
             HIP_TRY(hipGetLastError());
@@ -264,7 +266,7 @@ template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a)
             constexpr int G = decltype(gc)::value, N = decltype(nc)::value;
             r.slabs = (int)ceil_div(a->dim, G * N);
             const i64 blocks = ceil_div(L.chunks * r.slabs, 256 / G);
-            if (L.chunks * r.slabs > I32_MAX) return fail(SP_EINVAL, "too many entries for one launch");
+            if (too_many(L.chunks * r.slabs, 256)) return fail(SP_EINVAL, "too many entries for one launch");
             hipLaunchKernelGGL((sp_embed_reduce_kernel<T, TO, G, N>), dim3((unsigned)blocks), dim3(256), 0, stream, r);
             if (L.chunks > 1) hipLaunchKernelGGL((sp_embed_join_kernel<TO, G, N>), dim3((unsigned)((L.chunks - 1) * r.slabs)), dim3(256), 0, stream, r);
             return (int)SP_OK;
@@ -293,7 +295,7 @@ template <typename T> int launch_adjust(AdjustParams p, bool counts, hipStream_t
     p.seg = (int)(ceil_div(ceil_div(p.n_cols, segs), 2048) * 2048);
     p.segs = (int)ceil_div(p.n_cols, p.seg);
     const i64 blocks = p.n_rows * p.segs;
-    if (blocks > I32_MAX) return fail(SP_EINVAL, "too many scores for one launch");
+    if (too_many(blocks, AD_NT)) return fail(SP_EINVAL, "too many rows for one launch");
     if (counts) hipLaunchKernelGGL((sp_adjust_kernel<T, true>), dim3((unsigned)blocks), dim3(AD_NT), 0, stream, p);
     else hipLaunchKernelGGL((sp_adjust_kernel<T, false>), dim3((unsigned)blocks), dim3(AD_NT), 0, stream, p);
     HIP_TRY(hipGetLastError());
@@ -303,6 +305,8 @@ template <typename T> int launch_adjust(AdjustParams p, bool counts, hipStream_t
 // ---- distillation ------------------------------------------------------------------------------------------------------------------
 
 enum { DISTILL_LOSS = 1, DISTILL_GRAD = 2 };
+constexpr int DI_NT = 512;                               // threads of a workgroup
+constexpr i64 SCAN_WGS = 1024, GRAD_WGS = 2048;          // workgroups that few rows are cut for
 
 int check_distill(const sp_distill_args *a, int what) {
     if (!a || a->struct_size != sizeof(sp_distill_args)) return fail(SP_EINVAL, "sp_distill_args size mismatch");
@@ -312,6 +316,7 @@ int check_distill(const sp_distill_args *a, int what) {
     if (a->k < 0 || a->k > SP_DISTILL_KMAX) return fail(SP_EINVAL, "k = %d out of range [0, %d]", a->k, SP_DISTILL_KMAX);
     if (!(a->temperature > 0.f) || a->temperature > 1e30f || a->temperature < 1e-30f) return fail(SP_EINVAL, "temperature must be positive");
     if (a->n_rows == 0) return SP_OK;
+    if (too_many(a->n_rows + GRAD_WGS, DI_NT)) return fail(SP_EINVAL, "too many rows for one launch");
     if ((a->n_cols > 0 && !a->student) || (a->k > 0 && (!a->cols || !a->values))) return fail(SP_EINVAL, "NULL pointer");
     if (what & DISTILL_GRAD) {
         if (a->n_cols > 0 && !a->grad) return fail(SP_EINVAL, "grad is NULL");
@@ -319,8 +324,6 @@ int check_distill(const sp_distill_args *a, int what) {
     }
     return SP_OK;
 }
-
-constexpr int DI_NT = 512;
 
 // Workgroups of a row: few rows are cut so that about `want` workgroups run, in pieces of at least 2048 columns.
 int splits_of(const sp_distill_args *a, i64 want) {
@@ -351,7 +354,6 @@ int allow_lds(const void *kernel, size_t bytes) {
     if (bytes > 48 * 1024) HIP_TRY(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     return SP_OK;
 }
-constexpr i64 SCAN_WGS = 1024, GRAD_WGS = 2048;
 constexpr i64 LDS_BYTES = 163840;   // of a CU
 constexpr i64 FUSED_ROWS = 256;      // from as many rows on a workgroup per row fills the card
 
@@ -460,7 +462,7 @@ int sp_adjust_scores(const sp_adjust_args *a) {
 
 int64_t sp_distill_workspace_bytes(const sp_distill_args *a) {
     if (!a || a->struct_size != sizeof(sp_distill_args)) return fail(SP_EINVAL, "sp_distill_args size mismatch");
-    if (a->n_rows < 0 || a->n_rows > I32_MAX || a->n_cols < 0 || a->n_cols > I32_MAX) return fail(SP_EINVAL, "bad shape");
+    if (a->n_rows < 0 || a->n_rows > I32_MAX || a->n_cols < 0 || a->n_cols > COLS_MAX) return fail(SP_EINVAL, "bad shape");
     return (int64_t)distill_ws_bytes(a);
 }
 

@@ -14,7 +14,9 @@ neighbourhood model's top-k lists, and to be served with the same selectors.
 The compute is hand-written HIP behind include/sp_dense.h; torch is the tensors, the streams and the autograd graph.  Calls are
 asynchronous on torch's current stream of the tensors' device; outputs and workspaces come from torch's allocator, so a call may
 be captured into a graph.  Dense tensors are float32, bfloat16 or float16 with contiguous rows (any distance between rows);
-everything is summed in float32 or wider and rounded once.  There is no CPU fallback.
+everything is summed in float32 or wider and rounded once.  There is no CPU fallback.  Rows of one call are limited by what one
+launch can have (2^23 of distillation, 2^24 of scores, 2^26 of wide embedding rows); an output that is given may share memory with
+no operand but where its function says so.
 
 Autograd and graph capture: inside a capture the functions that build an autograd graph refuse inputs that require a gradient
 (the backward pass of a captured graph would meet leaves whose gradients belong to another stream): capture the explicit
@@ -337,9 +339,9 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
     h = _pattern("history", history, device, keep)
     f = _pattern("filter_cols", filter_cols, device, keep)
     t = _pattern("target_cols", target_cols, device, keep)
-    if not isinstance(repetition, torch.Tensor) and not float(repetition) > 0.0:
-        raise ValueError(f"repetition must be positive, got {repetition}")
     rep, rep_all = _per_row("repetition", repetition, device, n, keep)
+    if rep is None and not rep_all > 0.0:
+        raise ValueError(f"repetition must be positive, got {repetition}")
     pres, pres_all = _per_row("presence", presence, device, n, keep)
     freq, freq_all = _per_row("frequency", frequency, device, n, keep)
     bptr, bdt, ldb = None, 0, 0

@@ -573,6 +573,27 @@ def test_distill_every_listed_place(dtype, n, v):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,v,k", [(torch.float32, 150_001, 3), (torch.float32, 110_003, 4096), (torch.bfloat16, 300_007, 300), (torch.float16, 131_072, 64)])
+def test_distill_rows_longer_than_a_workgroup_keeps(dtype, v, k):
+    """The one call on rows that do not fit registers and LDS (their rest is read twice), in place as well, next to the two calls."""
+    n, some = 257, [0, 100, 256]
+    gen = torch.Generator(device="cuda").manual_seed(v)
+    z = (torch.randn(n, v, generator=gen, device="cuda") * 2).to(dtype)
+    cols = torch.randint(0, v, (n, k), generator=gen, device="cuda")
+    cols[:, :2] = torch.tensor([v - 1, v - 40], device="cuda")
+    values = torch.randn(n, k, generator=gen, device="cuda")
+    ref = distill_ref(z[some], cols[some].cpu(), values[some].cpu(), None, 1.0, None, None)
+    loss_b, grad_b = distill_bounds(z[some], cols[some].cpu(), 1.0, ref, None, dtype)
+    loss, stats = dense.distill_loss(z, cols, values, return_stats=True)
+    check(loss[some], ref[0], loss_b, "loss")
+    check(dense.distill_grad(z, stats, cols, values)[some], ref[2], grad_b, "grad")
+    loss, grad = dense.distill_loss_grad(z, cols, values)
+    check(loss[some], ref[0], loss_b, "loss of the one call")
+    check(grad[some], ref[2], grad_b, "grad of the one call")
+    assert torch.equal(dense.distill_loss_grad(z, cols, values, out=z)[1], grad) and torch.equal(z, grad)
+
+
+@gpu
 def test_distill_sizes_of_nothing():
     z = torch.randn(3, 50, device="cuda")
     none = torch.zeros(3, 0, dtype=torch.int32, device="cuda")
@@ -878,7 +899,11 @@ def test_c_entries_refuse():
     e.n_vocab = 2**31 - 1
     assert _c("sp_embed_rows_grad", e)[0] == -1
     d = _abi.SpDistillArgs()
-    d.n_rows, d.n_cols, d.k = 2, 3, 4097
+    d.n_rows, d.n_cols, d.k, d.temperature = 2**23, 3, 1, 1.0                        # more threads than a launch can have
+    assert "too many rows" in _c("sp_distill_loss", d)[1]
+    d.n_rows, d.n_cols, d.k = 2, 2**31 - 1, 1
+    assert "bad shape" in _c("sp_distill_loss", d)[1]
+    d.n_rows, d.n_cols, d.k, d.temperature = 2, 3, 4097, 0.0
     assert "k = 4097" in _c("sp_distill_loss", d)[1]
     d.k = 1
     for t in (0.0, -1.0, math.nan, math.inf):
@@ -949,7 +974,7 @@ def test_wrong_operands_on_a_device():
         lambda: dense.distill_loss(z.detach(), cols, vals.clone().requires_grad_()), lambda: dense.distill_loss(leaf, cols, vals.clone().requires_grad_()),
         lambda: dense.distill_loss(leaf, cols, vals, teacher_lse=torch.zeros(4, device="cuda").requires_grad_()),
         lambda: dense.embed_rows(leaf, ids, torch.zeros(2, dtype=torch.int64, device="cuda"), torch.zeros(3, device="cuda").requires_grad_()),
-        lambda: dense.distill_loss(z.detach(), cols, vals.T.contiguous()), lambda: dense.embed_rows(z, ids, out=[1]), lambda: dense.distill_grad(z.detach(), torch.zeros(4, device="cuda"), cols, vals),
+        lambda: dense.adjust_scores(z, repetition=torch.tensor(0.0)), lambda: dense.distill_loss(z.detach(), cols, vals.T.contiguous()), lambda: dense.embed_rows(z, ids, out=[1]), lambda: dense.distill_grad(z.detach(), torch.zeros(4, device="cuda"), cols, vals),
         lambda: dense.distill_loss_grad(z.detach(), cols, vals, grad_loss=torch.zeros(3, device="cuda")), lambda: dense.distill_loss(z.detach(), cols.T, vals.T),
     ]
     for i, f in enumerate(bad):
