@@ -83,8 +83,7 @@ int check_embed(const sp_embed_args *a) {
 
 // Calls f with the lanes of a group and the elements of a lane: 16 bytes a lane, or one element where a row has fewer; the fewest lanes that
 // cover a row, 8 .. 64 (columns beyond 64 lanes make further slabs).
-template <typename T, typename F> int with_group(i64 dim, F f) {
-    constexpr int N = VecOf<T>::N;
+template <int N, typename F> int with_group(i64 dim, F f) {
     using Wide = std::integral_constant<int, N>;
     if (dim < N) return f(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
     const i64 lanes = ceil_div(dim, N);
@@ -145,12 +144,12 @@ int run_embed(const sp_embed_args *a) {
             if (slabs > 1 && lanes == 32 * slabs) return run(std::integral_constant<int, 32>(), n, 1);
             if (slabs > 1 && lanes == 64 * slabs) return run(std::integral_constant<int, 64>(), n, 1);
         }
-        return with_group<T>(a->dim, [&](auto gc, auto nc) { return run(gc, nc, 0); });
+        return with_group<VecOf<T>::N>(a->dim, [&](auto gc, auto nc) { return run(gc, nc, 0); });
     });
 }
 
 // workspace of the gradient: two copies of the sorted entries (the passes alternate), the digit counts, the partial sums
-constexpr i64 REDUCE_CHUNKS = 4096;      // groups that sum sorted entries: about four waves per SIMD at one slab of 64 lanes
+constexpr i64 REDUCE_WAVES = 4096;       // that sum sorted entries, of a slab: four per SIMD; a wave has 64 / G chunks of them
 constexpr int DIRECT_WGS = 512;
 struct GradLayout {
     int wgs, sort_chunk, passes, bits, chunk;
@@ -171,7 +170,9 @@ GradLayout grad_layout(const sp_embed_args *a) {
     L.small = n <= SMALL_MAX && kb + SMALL_INDEX_BITS <= 32;
     L.passes = (kb + 8) / 9;
     L.bits = (kb + L.passes - 1) / L.passes;
-    const i64 per = ceil_div(n, REDUCE_CHUNKS);
+    auto group_lanes = [](auto gc, auto) { return (int)decltype(gc)::value; };
+    const i64 lanes = a->dtype == SP_DT_F32 ? with_group<4>(a->dim, group_lanes) : with_group<8>(a->dim, group_lanes);
+    const i64 per = ceil_div(n, REDUCE_WAVES * 64 / lanes);
     L.chunk = (int)(per < 16 ? 16 : per);
     L.chunks = ceil_div(n, L.chunk);
     size_t at = 0;
@@ -209,7 +210,7 @@ template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a)
         d.indices = a->indices; d.indptr = a->indptr; d.data = a->data;
         const i64 per = ceil_div(a->n_vocab, DIRECT_WGS);
         d.per = (int)(per < DIRECT_IDS ? per : DIRECT_IDS);
-        return with_group<T>(a->dim, [&](auto gc, auto nc) {
+        return with_group<VecOf<T>::N>(a->dim, [&](auto gc, auto nc) {
             constexpr int G = decltype(gc)::value, N = decltype(nc)::value;
             r.slabs = (int)ceil_div(a->dim, G * N);
             const i64 blocks = ceil_div(a->n_vocab, d.per) * r.slabs;
@@ -262,13 +263,13 @@ template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a)
         r.part = (float *)(ws + L.part);
         r.n = a->nnz; r.n_vocab = a->n_vocab; r.n_rows = a->n_rows; r.ld_in = a->ld_src; r.ld_out = a->ld_out;
         r.chunks = L.chunks; r.chunk = L.chunk; r.dim = (int)a->dim; r.accumulate = a->accumulate; r.scale = a->scale;
-        TRY(with_group<T>(a->dim, [&](auto gc, auto nc) {
+        TRY(with_group<VecOf<T>::N>(a->dim, [&](auto gc, auto nc) {
             constexpr int G = decltype(gc)::value, N = decltype(nc)::value;
             r.slabs = (int)ceil_div(a->dim, G * N);
             const i64 blocks = ceil_div(L.chunks * r.slabs, 256 / G);
             if (too_many(L.chunks * r.slabs, 256)) return fail(SP_EINVAL, "too many entries for one launch");
             hipLaunchKernelGGL((sp_embed_reduce_kernel<T, TO, G, N>), dim3((unsigned)blocks), dim3(256), 0, stream, r);
-            if (L.chunks > 1) hipLaunchKernelGGL((sp_embed_join_kernel<TO, G, N>), dim3((unsigned)((L.chunks - 1) * r.slabs)), dim3(256), 0, stream, r);
+            if (L.chunks > 1) hipLaunchKernelGGL((sp_embed_join_kernel<TO, G, N>), dim3((unsigned)(ceil_div(L.chunks - 1, 256 / G) * r.slabs)), dim3(256), 0, stream, r);
             return (int)SP_OK;
         }));
     }

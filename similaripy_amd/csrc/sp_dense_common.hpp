@@ -24,16 +24,6 @@ template <typename T, int N> __device__ __forceinline__ RawVec<T, N> vec_load(co
 }
 template <typename T, int N> __device__ __forceinline__ void vec_store(T *p, const RawVec<T, N> &r) { __builtin_memcpy(p, &r, sizeof(r)); }
 
-// the same past the caches: for results that the kernel does not read again
-template <typename T, int N> __device__ __forceinline__ void vec_store_once(T *p, const RawVec<T, N> &r) {
-    static_assert(sizeof(r) == 16, "16 bytes");
-    typedef unsigned Quad __attribute__((ext_vector_type(4)));
-    typedef Quad LooseQuad __attribute__((aligned(2)));
-    Quad q;
-    __builtin_memcpy(&q, &r, 16);
-    __builtin_nontemporal_store(q, (LooseQuad *)p);
-}
-
 __device__ __forceinline__ float up(float x) { return x; }
 __device__ __forceinline__ float up(__bf16 x) { return (float)x; }
 __device__ __forceinline__ float up(_Float16 x) { return (float)x; }
@@ -45,7 +35,6 @@ __device__ __forceinline__ float load_scalar(const void *p, int dtype, i64 i) {
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }      // v_exp_f32: 1 ulp, results below 2^-126 become 0
 
 __device__ __forceinline__ float wave_max(float v) {

@@ -16,7 +16,7 @@ struct EmbedParams {
     const float *data;
     void *out;
     i64 n_rows, n_vocab, nnz, ld_in, ld_out;
-    int dim, index64, accumulate;
+    int dim;
     float scale;
     int slabs;              // column slabs of a row: ceil(dim / (G * N))
     int by_xcd;             // bags: slab s is the work of the XCDs s, s + slabs, .. (slabs divides 8)
@@ -41,8 +41,8 @@ template <typename T, int N> __device__ __forceinline__ void put(T *p, const flo
 // value of lane `at` of the group of G lanes
 template <int G> __device__ __forceinline__ int group_lane(int v, int at) { return G == 64 ? __builtin_amdgcn_readlane(v, at) : __shfl(v, at, G); }
 
-// Lookup: one group of G lanes per row and slab of G * N columns.  (16 k rows of 2 KB: 14.4 us with one row per group, 19 with two, 20 with
-// four: more waves beat more loads per wave.)
+// Lookup: one group of G lanes per row and slab of G * N columns; HBM bounds it: 16 384 rows of 2 KB, read and written, take 10.9 us
+// (6.2 TB/s, some of the rows being read twice).  More waves beat more loads per wave: with two rows per group it is a third slower, with four 40 %.
 template <typename T, typename I, int G, int N> __global__ __launch_bounds__(256) void sp_embed_lookup_kernel(EmbedParams p) {
     const int lane = threadIdx.x & (G - 1);
     const i64 item = (i64)blockIdx.x * (256 / G) + threadIdx.x / G;
@@ -148,6 +148,8 @@ template <typename T, typename I, int G, int N> __global__ __launch_bounds__(256
 // workgroups one more adds the counts up between them).  Every wave owns a contiguous part of the chunk and goes through it in order;
 // equal digits of 64 entries are ranked by their lane.  Ids outside the table take the key n_vocab and end up behind everything else.
 // An entry carries its row of the gradient and its weight.  The rows of a CSR's entries are written out beside the first count.
+// 1.2 M entries: 7 us to count, 5 to add the counts up and 18 to move them, two passes for 2^17 ids; each launch is near what a launch of
+// so little work costs.  65 536 lookups into 173 MB: 8.3 + 10.9 us a pass, in which the gradient is cleared as well.
 
 constexpr int SORT_NT = 512, SORT_WAVES = SORT_NT / 64, SORT_BINS = 512;
 constexpr int SORT_PER = 9, SORT_CHUNK = SORT_NT * SORT_PER;    // entries of a thread, most of a workgroup: 54 KB of LDS
@@ -514,6 +516,7 @@ __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70
 
 // One group of G lanes per chunk of the sorted entries and slab of columns: runs of equal ids are summed as they come.  A run that
 // lies inside the chunk is a row of the gradient and is written; one that began before or goes on behind it leaves its sum in `part`.
+// What bounds it is the gather: 1.2 M entries, each a row of 1 KB, are 1.2 GB in 55 us, 22 TB/s out of the L2s.
 template <typename T, typename TO, int G, int N> __global__ __launch_bounds__(256) void sp_embed_reduce_kernel(ReduceParams p) {
     constexpr int U = 8;
     const int lane = threadIdx.x & (G - 1);
@@ -674,28 +677,24 @@ template <typename T, typename TO, typename I, int G, int N> __global__ __launch
         if (first[i] == DIRECT_NONE) vec_store<TO, N>((TO *)p.out + (v0 + i) * p.ld_out + cols.c, zero);
 }
 
-// Runs over several chunks: the workgroup of the chunk in which a run begins adds up its parts and writes the row.  All threads look how
-// far the run goes, 256 chunks at once; the 256 / G groups then sum contiguous shares of the parts, which are joined in their order.
-template <typename TO, int G, int N> __global__ __launch_bounds__(256) void sp_embed_join_kernel(ReduceParams p) {
+// Runs over several chunks: the chunk in which a run begins adds up its parts, in their order, and writes the row.  One group of G lanes per
+// chunk and slab: the lanes look how far the run goes; up to JOIN_SHORT more chunks are the group's work, a longer run that of the whole
+// workgroup, whose groups sum contiguous shares.  (One workgroup per chunk instead costs 2 ns a chunk, 8 us at 4096 and 33 at 16 384, for the
+// launch and the latency of the keys alone.)
+constexpr int JOIN_SHORT = 8;
+template <typename TO, int G, int N> __device__ __forceinline__ void join_long(const ReduceParams &p, i64 ch, int slab, unsigned run, float (*sums)[G * N], int *ends) {
     constexpr int GROUPS = 256 / G, U = 8;
-    __shared__ float sums[GROUPS][G * N];
-    __shared__ int ends;
     const int tid = threadIdx.x, lane = tid & (G - 1), g = tid / G;
-    const i64 ch = blockIdx.x / p.slabs;
-    const Columns<N> cols(((int)(blockIdx.x % p.slabs) * G + lane) * N, p.dim);
-    const i64 b = ch * p.chunk, e = b + p.chunk;               // (there is a chunk behind this one: it is full, and key[e] exists)
-    const unsigned run = p.key[e - 1];
-    if (run == (unsigned)p.n_vocab || p.key[e] != run) return;                              // nothing goes on behind it
-    if (b > 0 && p.key[b - 1] == run) return;                                               // the run began before this chunk
-    // chunks ch + 1 .. last hold the rest of it: the first one that does not go on into the next
+    const Columns<N> cols((slab * G + lane) * N, p.dim);
+    // chunks ch + 1 .. last hold the rest of it: the first one that does not go on into the next, 256 looked at at once
     i64 last = ch + 1;
     for (;; last += 256) {
-        if (tid == 0) ends = 256;
+        if (tid == 0) *ends = 256;
         __syncthreads();
         const i64 k = last + tid;
-        if (k + 1 >= p.chunks || p.key[(k + 1) * p.chunk] != run) atomicMin(&ends, tid);
+        if (k + 1 >= p.chunks || p.key[(k + 1) * p.chunk] != run) atomicMin(ends, tid);
         __syncthreads();
-        const int first = ends;
+        const int first = *ends;
         __syncthreads();
         if (first < 256) {
             last += first;
@@ -707,30 +706,73 @@ template <typename TO, int G, int N> __global__ __launch_bounds__(256) void sp_e
     float acc[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
-    {
-        for (i64 k = k0; k < k1; k += U) {
-            RawVec<float, N> x[U];
+    for (i64 k = k0; k < k1; k += U) {
+        RawVec<float, N> x[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) x[u] = vec_load<float, N>(p.part + (2 * min(k + u, k1 - 1)) * p.dim + cols.c);
+        for (int u = 0; u < U; ++u) x[u] = vec_load<float, N>(p.part + (2 * min(k + u, k1 - 1)) * p.dim + cols.c);
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (k + u < k1)
+        for (int u = 0; u < U; ++u)
+            if (k + u < k1)
 #pragma unroll
-                    for (int j = 0; j < N; ++j) acc[j] += x[u].v[j];
-        }
+                for (int j = 0; j < N; ++j) acc[j] += x[u].v[j];
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) sums[g][lane * N + j] = acc[j];
     __syncthreads();
-    if (g != 0 || !cols.active) return;
-    const RawVec<float, N> x = vec_load<float, N>(p.part + (2 * ch + 1) * p.dim + cols.c);
+    if (g == 0 && cols.active) {
+        const RawVec<float, N> x = vec_load<float, N>(p.part + (2 * ch + 1) * p.dim + cols.c);
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] = x.v[j];
-    const int parts = (int)min((i64)GROUPS, (count + share - 1) / share);
-    for (int q = 0; q < parts; ++q)
+        for (int j = 0; j < N; ++j) acc[j] = x.v[j];
+        const int parts = (int)min((i64)GROUPS, (count + share - 1) / share);
+        for (int q = 0; q < parts; ++q)
 #pragma unroll
-        for (int j = 0; j < N; ++j) acc[j] += sums[q][lane * N + j];
-    write_row<TO, N>(p, run, cols, acc);
+            for (int j = 0; j < N; ++j) acc[j] += sums[q][lane * N + j];
+        write_row<TO, N>(p, run, cols, acc);
+    }
+    __syncthreads();
+}
+template <typename TO, int G, int N> __global__ __launch_bounds__(256) void sp_embed_join_kernel(ReduceParams p) {
+    constexpr int GROUPS = 256 / G;
+    __shared__ float sums[GROUPS][G * N];
+    __shared__ unsigned long_run[GROUPS];                      // n_vocab: none
+    __shared__ int ends;
+    const int tid = threadIdx.x, lane = tid & (G - 1), g = tid / G;
+    const unsigned none = (unsigned)p.n_vocab;
+    const int slab = (int)(blockIdx.x % p.slabs);
+    const i64 ch0 = (i64)(blockIdx.x / p.slabs) * GROUPS, ch = ch0 + g;
+    if (lane == 0) long_run[g] = none;
+    if (ch + 1 < p.chunks) {                                   // (the chunk is full then, and there is an entry behind it)
+        const i64 e = (ch + 1) * p.chunk, k = ch + 1 + min(lane, JOIN_SHORT - 1);
+        const unsigned run = p.key[e - 1], next = p.key[e], before = ch > 0 ? p.key[e - p.chunk - 1] : none;
+        const unsigned beyond = k + 1 < p.chunks ? p.key[(k + 1) * p.chunk] : none;
+        if (run != none && next == run && before != run) {     // it goes on behind the chunk, and began in it
+            const u64 all = __ballot(lane < JOIN_SHORT && beyond != run);
+            const unsigned ends_at = (unsigned)((all >> (tid & 63 & ~(G - 1))) & ((1u << JOIN_SHORT) - 1u));
+            if (ends_at == 0u) {
+                if (lane == 0) long_run[g] = run;
+            } else {
+                const int more = __builtin_ctz(ends_at) + 1;   // chunks ch + 1 .. ch + more
+                const Columns<N> cols((slab * G + lane) * N, p.dim);
+                RawVec<float, N> x[JOIN_SHORT], mine = vec_load<float, N>(p.part + (2 * ch + 1) * p.dim + cols.c);
+#pragma unroll
+                for (int u = 0; u < JOIN_SHORT; ++u) x[u] = vec_load<float, N>(p.part + 2 * (ch + 1 + min(u, more - 1)) * p.dim + cols.c);
+                float acc[N];
+#pragma unroll
+                for (int j = 0; j < N; ++j) acc[j] = mine.v[j];
+#pragma unroll
+                for (int u = 0; u < JOIN_SHORT; ++u)
+                    if (u < more)
+#pragma unroll
+                        for (int j = 0; j < N; ++j) acc[j] += x[u].v[j];
+                if (cols.active) write_row<TO, N>(p, run, cols, acc);
+            }
+        }
+    }
+    __syncthreads();
+    for (int q = 0; q < GROUPS; ++q) {
+        const unsigned run = long_run[q];
+        if (run != none) join_long<TO, G, N>(p, ch0 + q, slab, run, sums, &ends);
+    }
 }
 
 }  // namespace
