@@ -103,7 +103,20 @@ EmbedParams embed_params(const sp_embed_args *a) {
 
 constexpr i64 L2_BYTES = 4 << 20;     // of an XCD
 constexpr i64 FEW_BAGS = 8192;        // one wave each does not fill the card
-constexpr int FILL_WGS = 512;      // workgroups that clear rows
+constexpr int FILL_WGS = 512;         // workgroups that clear rows
+
+// A gather of wide rows may be cut by columns into slabs of whole cache lines, each the work of one XCD or of two or four, so that an XCD's L2
+// holds that many times more rows of its slab.  Slabs of a row: 8, 4 or 2 where they are equal and their lanes a power of two, 1 otherwise.
+template <typename T> int line_slabs(i64 dim, i64 ld) {
+    const i64 bytes = dim * (i64)sizeof(T), lanes = dim / VecOf<T>::N;
+    if (ld * (i64)sizeof(T) % 128 != 0) return 1;
+    for (int slabs = 8; slabs > 1; slabs /= 2)
+        if (bytes % (128 * slabs) == 0) {
+            const i64 g = lanes / slabs;
+            return g <= 64 && (g & (g - 1)) == 0 ? slabs : 1;
+        }
+    return 1;
+}
 
 int run_embed(const sp_embed_args *a) {
     hipStream_t stream = (hipStream_t)a->stream;
@@ -130,20 +143,11 @@ int run_embed(const sp_embed_args *a) {
             HIP_TRY(hipGetLastError());
             return (int)SP_OK;
         };
-        // Slabs of whole cache lines, one per XCD or per two or four of them: for a table beyond the L2 of an XCD whose rows are wide and from
-        // which more rows are taken than it has, and for few bags.
-        constexpr int N = VecOf<T>::N;
-        const i64 row_bytes = a->dim * (i64)sizeof(T), lanes = a->dim / N;
+        // by XCD: a table beyond the L2 of one from which more rows are taken than it has, and few bags
+        const i64 row_bytes = a->dim * (i64)sizeof(T);
         const bool large = a->nnz >= a->n_vocab && a->n_vocab * row_bytes > L2_BYTES && row_bytes >= 1024;
-        if (a->indptr && (large || a->n_rows <= FEW_BAGS) && a->ld_src * (i64)sizeof(T) % 128 == 0 && (uintptr_t)a->src % 128 == 0) {
-            int slabs = 8;
-            while (slabs > 1 && row_bytes % (128 * slabs) != 0) slabs /= 2;
-            const std::integral_constant<int, N> n;
-            if (slabs > 1 && lanes == 8 * slabs) return run(std::integral_constant<int, 8>(), n, 1);
-            if (slabs > 1 && lanes == 16 * slabs) return run(std::integral_constant<int, 16>(), n, 1);
-            if (slabs > 1 && lanes == 32 * slabs) return run(std::integral_constant<int, 32>(), n, 1);
-            if (slabs > 1 && lanes == 64 * slabs) return run(std::integral_constant<int, 64>(), n, 1);
-        }
+        const int slabs = a->indptr && (large || a->n_rows <= FEW_BAGS) && (uintptr_t)a->src % 128 == 0 ? line_slabs<T>(a->dim, a->ld_src) : 1;
+        if (slabs > 1) return with_group<VecOf<T>::N>(a->dim / slabs, [&](auto gc, auto nc) { return run(gc, nc, 1); });
         return with_group<VecOf<T>::N>(a->dim, [&](auto gc, auto nc) { return run(gc, nc, 0); });
     });
 }
@@ -153,6 +157,7 @@ constexpr i64 REDUCE_WAVES = 4096;       // that sum sorted entries, of a slab: 
 constexpr int DIRECT_WGS = 512;
 struct GradLayout {
     int wgs, sort_chunk, passes, bits, chunk;
+    int slabs;                                                   // of a row that are cut for the XCDs (1: not cut)
     bool small;                                                  // sorted by one workgroup
     i64 chunks;
     size_t key[2], pay[2], w[2], rows, hist, digits, part, total;
@@ -170,8 +175,13 @@ GradLayout grad_layout(const sp_embed_args *a) {
     L.small = n <= SMALL_MAX && kb + SMALL_INDEX_BITS <= 32;
     L.passes = (kb + 8) / 9;
     L.bits = (kb + L.passes - 1) / L.passes;
+    // by XCD: rows of the gradient beyond the L2 of one, each taken many times.  (8192 rows of 144 entries, cut / whole: 4 KB 384 / 595 us, 2 KB
+    // 249 / 280, 1 KB 190 / 142; 30 000 rows of 8 entries: 244 / 248, 143 / 138, 90 / 87.)
+    const i64 row_bytes = a->dim * (a->dtype == SP_DT_F32 ? 4 : 2);
+    const bool large = a->nnz >= 16 * a->n_rows && a->n_rows * row_bytes > L2_BYTES && row_bytes >= 2048;
+    L.slabs = !large ? 1 : a->dtype == SP_DT_F32 ? line_slabs<float>(a->dim, a->ld_src) : line_slabs<__bf16>(a->dim, a->ld_src);
     auto group_lanes = [](auto gc, auto) { return (int)decltype(gc)::value; };
-    const i64 lanes = a->dtype == SP_DT_F32 ? with_group<4>(a->dim, group_lanes) : with_group<8>(a->dim, group_lanes);
+    const i64 lanes = a->dtype == SP_DT_F32 ? with_group<4>(a->dim / L.slabs, group_lanes) : with_group<8>(a->dim / L.slabs, group_lanes);
     const i64 per = ceil_div(n, REDUCE_WAVES * 64 / lanes);
     L.chunk = (int)(per < 16 ? 16 : per);
     L.chunks = ceil_div(n, L.chunk);
@@ -263,13 +273,14 @@ template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a)
         r.part = (float *)(ws + L.part);
         r.n = a->nnz; r.n_vocab = a->n_vocab; r.n_rows = a->n_rows; r.ld_in = a->ld_src; r.ld_out = a->ld_out;
         r.chunks = L.chunks; r.chunk = L.chunk; r.dim = (int)a->dim; r.accumulate = a->accumulate; r.scale = a->scale;
-        TRY(with_group<VecOf<T>::N>(a->dim, [&](auto gc, auto nc) {
-            constexpr int G = decltype(gc)::value, N = decltype(nc)::value;
+        TRY(with_group<VecOf<T>::N>(a->dim / L.slabs, [&](auto gc, auto nc) {
+            constexpr int G = decltype(gc)::value, N = decltype(nc)::value, GROUPS = 256 / G;
             r.slabs = (int)ceil_div(a->dim, G * N);
-            const i64 blocks = ceil_div(L.chunks * r.slabs, 256 / G);
+            r.by_xcd = L.slabs > 1;
+            const i64 blocks = r.by_xcd ? ceil_div(ceil_div(L.chunks, GROUPS), 8 / r.slabs) * 8 : ceil_div(L.chunks * r.slabs, GROUPS);
             if (too_many(L.chunks * r.slabs, 256)) return fail(SP_EINVAL, "too many entries for one launch");
             hipLaunchKernelGGL((sp_embed_reduce_kernel<T, TO, G, N>), dim3((unsigned)blocks), dim3(256), 0, stream, r);
-            if (L.chunks > 1) hipLaunchKernelGGL((sp_embed_join_kernel<TO, G, N>), dim3((unsigned)(ceil_div(L.chunks - 1, 256 / G) * r.slabs)), dim3(256), 0, stream, r);
+            if (L.chunks > 1) hipLaunchKernelGGL((sp_embed_join_kernel<TO, G, N>), dim3((unsigned)(ceil_div(L.chunks - 1, GROUPS) * r.slabs)), dim3(256), 0, stream, r);
             return (int)SP_OK;
         }));
     }

@@ -148,8 +148,8 @@ template <typename T, typename I, int G, int N> __global__ __launch_bounds__(256
 // workgroups one more adds the counts up between them).  Every wave owns a contiguous part of the chunk and goes through it in order;
 // equal digits of 64 entries are ranked by their lane.  Ids outside the table take the key n_vocab and end up behind everything else.
 // An entry carries its row of the gradient and its weight.  The rows of a CSR's entries are written out beside the first count.
-// 1.2 M entries: 7 us to count, 5 to add the counts up and 18 to move them, two passes for 2^17 ids; each launch is near what a launch of
-// so little work costs.  65 536 lookups into 173 MB: 8.3 + 10.9 us a pass, in which the gradient is cleared as well.
+// 1.2 M entries: 7 us to count, 5 to add the counts up and 17 to move them, two passes for 2^17 ids: latency of launches with one workgroup on a
+// CU, not bandwidth (28 MB a pass).  16 384 lookups into 173 MB: 8.3 + 10.9 us a pass, in which the gradient is cleared as well.
 
 constexpr int SORT_NT = 512, SORT_WAVES = SORT_NT / 64, SORT_BINS = 512;
 constexpr int SORT_PER = 9, SORT_CHUNK = SORT_NT * SORT_PER;    // entries of a thread, most of a workgroup: 54 KB of LDS
@@ -491,6 +491,7 @@ struct ReduceParams {
     i64 n, n_vocab, ld_in, ld_out, n_rows;
     i64 chunks;
     int chunk, dim, slabs, accumulate;
+    int by_xcd;                 // slab s is the work of the XCDs s, s + slabs, .. (slabs divides 8)
     float scale;
 };
 
@@ -516,15 +517,25 @@ __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70
 
 // One group of G lanes per chunk of the sorted entries and slab of columns: runs of equal ids are summed as they come.  A run that
 // lies inside the chunk is a row of the gradient and is written; one that began before or goes on behind it leaves its sum in `part`.
-// What bounds it is the gather: 1.2 M entries, each a row of 1 KB, are 1.2 GB in 55 us, 22 TB/s out of the L2s.
+// What bounds it is the gather: 1.2 M entries, each a row of 516 bytes, are 0.61 GB in 54 us, 11 TB/s out of the L2s (47 us with four times the
+// waves, which the joins then lose again).
 template <typename T, typename TO, int G, int N> __global__ __launch_bounds__(256) void sp_embed_reduce_kernel(ReduceParams p) {
     constexpr int U = 8;
     const int lane = threadIdx.x & (G - 1);
-    i64 item = (i64)blockIdx.x * (256 / G) + threadIdx.x / G;
-    if (G == 64) item = (i64)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const i64 ch = item / p.slabs;
+    const int g = G == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : (int)threadIdx.x / G;
+    i64 ch;
+    int slab;
+    if (p.by_xcd) {                                            // (as in the bags)
+        const int xcd = (int)(blockIdx.x % 8);
+        slab = xcd % p.slabs;
+        ch = ((i64)(blockIdx.x / 8) * (8 / p.slabs) + xcd / p.slabs) * (256 / G) + g;
+    } else {
+        const i64 item = (i64)blockIdx.x * (256 / G) + g;
+        slab = (int)(item % p.slabs);
+        ch = item / p.slabs;
+    }
     if (ch >= p.chunks) return;
-    const Columns<N> cols(((int)(item % p.slabs) * G + lane) * N, p.dim);
+    const Columns<N> cols((slab * G + lane) * N, p.dim);
     const i64 b = ch * p.chunk, e = min(p.n, b + p.chunk);
     const int none = (int)p.n_vocab;
     const int prev = b > 0 ? (int)p.key[b - 1] : none, next = e < p.n ? (int)p.key[e] : none;

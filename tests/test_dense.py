@@ -240,6 +240,35 @@ def test_embed_grad_accumulate_and_layouts(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,rows,dim", [(torch.float32, 2200, 512), (torch.bfloat16, 2300, 1024), (torch.float16, 1100, 2048), (torch.float32, 1100, 1024),
+                                            (torch.float32, 3000, 384), (torch.float32, 1500, 768), (torch.bfloat16, 900, 4096)])
+def test_embed_grad_wide_rows(dtype, rows, dim):
+    """Rows beyond the L2 of an XCD, cut by columns where they can be; short runs, runs over a few chunks of the sorted entries and over many."""
+    rng = np.random.default_rng(dim + rows)
+    n, vocab = rows * 17, 70
+    ids = np.concatenate([rng.integers(0, vocab, n // 2), np.minimum(rng.zipf(1.3, n - n // 2) - 1, vocab)])      # the id `vocab` is outside
+    ids = torch.from_numpy(rng.permutation(ids).astype(np.int32))
+    indptr = torch.from_numpy(np.sort(np.concatenate([[0], rng.integers(0, n + 1, rows - 1), [n]])).astype(np.int32))
+    data = torch.from_numpy(rng.random(n).astype(np.float32) + 0.5)
+    grad = torch.from_numpy(rng.standard_normal((rows, dim)).astype(np.float32)).to(dtype)
+    row = torch.repeat_interleave(torch.arange(rows), indptr.long().diff())
+    at = torch.where(ids < vocab, ids, vocab).long()
+    terms = data.double()[:, None] * grad.double()[row]
+    want = torch.zeros(vocab + 1, dim, dtype=torch.float64).index_add_(0, at, terms)[:vocab]
+    mag = torch.zeros(vocab + 1, dim, dtype=torch.float64).index_add_(0, at, terms.abs())[:vocab]
+    most = int(torch.bincount(at).max())
+    # `most` fused additions and the joins' at most as many more, each rounding a sum no larger than mag
+    e = 2 * most * U * mag
+    args = (ids.cuda(), vocab, indptr.cuda(), data.cuda())
+    got = dense.embed_rows_grad(grad.cuda(), *args)
+    check(got, want, e + half_step(dtype) * (want.abs() + e) + tiny(dtype))
+    assert torch.equal(got, dense.embed_rows_grad(grad.cuda(), *args))
+    wide = dense.embed_rows_grad(grad.cuda(), *args, dtype=torch.float32)
+    check(wide, want, e + half_step(torch.float32) * (want.abs() + e))
+    assert torch.equal(wide.to(dtype), got)
+
+
+@gpu
 def test_embed_autograd():
     """The graph's gradient is embed_rows_grad's, also through a broadcast sum, for a table used twice, and against differences."""
     rng = np.random.default_rng(3)
