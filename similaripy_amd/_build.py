@@ -1,8 +1,7 @@
 """In-tree build of libsimilaripy_hip.so (hipcc, gfx950 only).
 
 The shared object is written next to the sources (``similaripy_amd/lib/``): it is
-git-ignored but travels with the gpurun snapshot, and the round-end driver can see
-that it is the library the Python process actually loaded.
+git-ignored, and it is the library that the Python process loads.
 """
 from __future__ import annotations
 

@@ -393,11 +393,27 @@ template <typename I> __device__ __forceinline__ i64 row_of(const void *indptr, 
 }
 
 // Up to 8192 entries are sorted by one workgroup, in one launch, while the others clear the gradient: an entry is its key and its index
-// in one word, 8 words per thread in registers, moved through LDS once per pass.  Gradient of n lookups into 84 433 rows of 1024 bf16, this
-// way / by the launches above: n = 64 33 / 41 us, 1024 35 / 47, 4096 36 / 48, 8192 41 / 50, 16 384 82 / 55; into 2000 rows, where there is
-// little to clear beside it: 1024 19 / 28, 4096 26 / 30, 8192 37 / 33.
+// in one word, 8 words per thread in registers, moved through LDS once per pass.  The lanes of equal digits are found first; one of them counts
+// all of them (a popular id's entries would add to one counter one after the other; 6000 entries 19.6 -> 16.2 us.  In the launches above the same
+// costs registers that are missed: 17.2 -> 18.5.)  Gradient of n lookups into 84 433 rows of 1024 bf16, this way / by the launches above:
+// n = 4096 35 / 48 us, 8192 37 / 50, 16 384 82 / 54; into 2000 rows, where there is little to clear beside it: 4096 23 / 30 us, 8192 30 / 33.
 constexpr int SMALL_NT = 1024, SMALL_WAVES = SMALL_NT / 64, SMALL_PER = 8, SMALL_MAX = SMALL_NT * SMALL_PER, SMALL_INDEX_BITS = 13;
 static_assert(SMALL_MAX == 1 << SMALL_INDEX_BITS, "an index fits its bits");
+
+// same[q]: the lanes of the wave whose digit of round q is this lane's, of those that `same` holds on entry.  Bit by bit for all rounds: they do
+// not wait for one another.
+template <int Q> __device__ __forceinline__ void match_digits(const unsigned (&digit)[Q], u64 (&same)[Q], int rounds, int bits) {
+    for (int k = 0; k < bits; ++k) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            if (q >= rounds) break;
+            const int bit = __builtin_amdgcn_sbfe((int)digit[q], k, 1);       // 0 or -1
+            const u64 set = __ballot(bit != 0);
+            const unsigned lo = (unsigned)same[q] & ~((unsigned)set ^ (unsigned)bit), hi = (unsigned)(same[q] >> 32) & ~((unsigned)(set >> 32) ^ (unsigned)bit);
+            same[q] = (u64)hi << 32 | lo;
+        }
+    }
+}
 
 template <typename I> __global__ __launch_bounds__(SMALL_NT) void sp_sort_small_kernel(SortParams p, int passes) {
     __shared__ unsigned buf[SMALL_MAX];
@@ -418,11 +434,24 @@ template <typename I> __global__ __launch_bounds__(SMALL_NT) void sp_sort_small_
     }
     for (int pass = 0; pass < passes; ++pass) {
         const int shift = SMALL_INDEX_BITS + pass * p.bits;
+        unsigned digit[SMALL_PER];
+        u64 same[SMALL_PER];
+#pragma unroll
+        for (int q = 0; q < SMALL_PER; ++q) {
+            const bool ok = q < rounds && first + q * 64 < n;
+            digit[q] = ok ? (v[q] >> shift) & mask : 0u;
+            same[q] = __ballot(ok);
+        }
+        match_digits(digit, same, rounds, p.bits);
         for (int i = tid; i < SMALL_WAVES * SORT_BINS; i += SMALL_NT) (&off[0][0])[i] = 0u;
         __syncthreads();
+        unsigned rank[SMALL_PER];                              // among the wave's entries of the digit in this round
 #pragma unroll
         for (int q = 0; q < SMALL_PER; ++q)
-            if (q < rounds && first + q * 64 < n) atomicAdd(&off[wave][(v[q] >> shift) & mask], 1u);
+            if (q < rounds && first + q * 64 < n) {
+                rank[q] = (unsigned)__popcll(same[q] & ((1ull << lane) - 1ull));
+                if (rank[q] == 0) atomicAdd(&off[wave][digit[q]], (unsigned)__popcll(same[q]));
+            }
         __syncthreads();
         unsigned inc = 0, all = 0;
         if (tid < SORT_BINS) {                                 // a thread per digit: entries of smaller digits, then of the waves before
@@ -448,22 +477,12 @@ template <typename I> __global__ __launch_bounds__(SMALL_NT) void sp_sort_small_
         __syncthreads();
         volatile unsigned *mine = off[wave];
 #pragma unroll
-        for (int q = 0; q < SMALL_PER; ++q) {
-            if (q >= rounds) break;
-            const bool ok = first + q * 64 < n;
-            const unsigned digit = ok ? (v[q] >> shift) & mask : 0u;
-            u64 same = __ballot(ok);
-            for (int k = 0; k < p.bits; ++k) {
-                const u64 set = __ballot((digit >> k) & 1u);
-                same &= (digit >> k) & 1u ? set : ~set;
-            }
-            if (ok) {
-                const unsigned rank = (unsigned)__popcll(same & ((1ull << lane) - 1ull));
-                const unsigned at = mine[digit] + rank;
-                if (rank == 0) mine[digit] = at + (unsigned)__popcll(same);       // (as in the launches above)
+        for (int q = 0; q < SMALL_PER; ++q)
+            if (q < rounds && first + q * 64 < n) {
+                const unsigned at = mine[digit[q]] + rank[q];
+                if (rank[q] == 0) mine[digit[q]] = at + (unsigned)__popcll(same[q]);    // (as in the launches above)
                 buf[at] = v[q];
             }
-        }
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < SMALL_PER; ++q)
@@ -517,7 +536,7 @@ __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70
 
 // One group of G lanes per chunk of the sorted entries and slab of columns: runs of equal ids are summed as they come.  A run that
 // lies inside the chunk is a row of the gradient and is written; one that began before or goes on behind it leaves its sum in `part`.
-// What bounds it is the gather: 1.2 M entries, each a row of 516 bytes, are 0.61 GB in 54 us, 11 TB/s out of the L2s (47 us with four times the
+// What bounds it is the gather: 1.2 M entries, each a row of 516 bytes, are 0.61 GB in 53 us, 11.5 TB/s out of the L2s (47 us with four times the
 // waves, which the joins then lose again).
 template <typename T, typename TO, int G, int N> __global__ __launch_bounds__(256) void sp_embed_reduce_kernel(ReduceParams p) {
     constexpr int U = 8;
@@ -557,7 +576,7 @@ template <typename T, typename TO, int G, int N> __global__ __launch_bounds__(25
         if (lane < n) {
             key = (int)p.key[i + lane];
             const unsigned r = p.pay[i + lane];
-            from = key != none && (i64)r < p.n_rows ? (int)r : -1;
+            from = ((i64)r < p.n_rows ? (int)r : -1) | (key == none ? -1 : 0);      // (no branch: both are requested at once)
             weight = p.w ? p.w[i + lane] : 1.f;
         }
         for (int j = 0; j < n; j += U) {
@@ -595,8 +614,8 @@ template <typename T, typename TO, int G, int N> __global__ __launch_bounds__(25
 
 // Up to 1024 entries need no sort at all: a workgroup owns DIRECT_IDS ids or fewer (and a slab of columns), looks through all entries, keeps
 // those of its ids in their order, sums each id's and clears the rows that have none.  One launch, no workspace.  Gradient of n lookups
-// into 84 433 rows of 1024 bf16, this way / by the sort above: n = 64 24 / 33 us, 512 27 / 36, 1024 28 / 35, 2048 36 / 35; into 2000 rows:
-// 8.8 / 18, 10 / 19, 16 / 20, 31 / 20 (what a popular id has is summed by one group).
+// into 84 433 rows of 1024 bf16, this way / by the sort above: n = 64 24 / 33 us, 512 27 / 36, 1024 28 / 33, 2048 36 / 33; into 2000 rows:
+// 8.8 / 18, 10 / 19, 16 / 18, 31 / 20 (what a popular id has is summed by one group).
 constexpr int DIRECT_MAX = 1024, DIRECT_IDS = 2048, DIRECT_NONE = 0x7FFFFFFF;
 struct DirectParams {
     ReduceParams r;              // in, out, n, n_vocab, ld_in, ld_out, n_rows, dim, slabs, accumulate, scale
