@@ -149,7 +149,7 @@ typedef struct sp_distill_args {
 int sp_distill_loss(const sp_distill_args *args);        /* writes loss and stats (either may be NULL) */
 int sp_distill_grad(const sp_distill_args *args);        /* reads stats, writes grad */
 int sp_distill_loss_grad(const sp_distill_args *args);   /* writes loss (may be NULL) and grad */
-int64_t sp_distill_workspace_bytes(const sp_distill_args *args);
+int64_t sp_distill_workspace_bytes(const sp_distill_args *args);      /* of sp_distill_loss, or, where `grad` is set, of sp_distill_loss_grad */
 
 #ifdef __cplusplus
 }

@@ -318,7 +318,8 @@ template <typename T> int launch_adjust(AdjustParams p, bool counts, hipStream_t
 
 enum { DISTILL_LOSS = 1, DISTILL_GRAD = 2 };
 constexpr int DI_NT = 512;                               // threads of a workgroup
-constexpr i64 SCAN_WGS = 1024, GRAD_WGS = 2048;          // workgroups that few rows are cut for
+constexpr i64 SCAN_WGS = 512, GRAD_WGS = 2048;           // workgroups that few rows are cut for
+constexpr i64 CACHE_BYTES = 256 << 20;                   // between the L2s and the memory
 
 int check_distill(const sp_distill_args *a, int what) {
     if (!a || a->struct_size != sizeof(sp_distill_args)) return fail(SP_EINVAL, "sp_distill_args size mismatch");
@@ -337,19 +338,52 @@ int check_distill(const sp_distill_args *a, int what) {
     return SP_OK;
 }
 
-// Workgroups of a row: few rows are cut so that about `want` workgroups run, in pieces of at least 2048 columns.
-int splits_of(const sp_distill_args *a, i64 want) {
-    if (a->n_rows <= 0) return 1;
-    i64 s = ceil_div(want, a->n_rows);
-    const i64 most = a->n_cols / 2048;
-    s = s > most ? most : s;
-    return s < 1 ? 1 : (int)s;
+// Workgroups of a row: few rows are cut so that about `want` workgroups run, in pieces of at least `piece` bytes; rows of less than `whole` are not.
+int splits_of(const sp_distill_args *a, i64 want, i64 whole, i64 piece) {
+    const i64 bytes = a->n_cols * (a->dtype == SP_DT_F32 ? 4 : 2);
+    if (a->n_rows <= 0 || bytes < whole) return 1;
+    const i64 s = ceil_div(want, a->n_rows), most = bytes / piece;
+    return (int)(s > most ? most : s);
+}
+// A row in pieces needs a second launch for the loss: 1 row of 200 KB whole / in pieces 9 / 13 us, 256 rows 13 / 18; 64 rows of 400 KB 18 / 13,
+// 256 rows 29 / 25; 1 row of 1.2 MB 22 / 12.  (With pieces for 1024 workgroups 512 rows of 200 .. 1200 KB take 4 .. 8 % longer.)
+int scan_splits(const sp_distill_args *a) { return splits_of(a, SCAN_WGS, 384 << 10, 128 << 10); }
+// The gradient: every piece reads the row's list again, 2048 workgroups are worth that only where the scores come from memory.  (2048 / 1024:
+// 1024 x 84 432 float32 with the loss 231 / 242 us, 512 x 200 000 259 / 265, 256 x 100 000 80 / 75, 512 x 100 000 bf16 83 / 77.  Pieces of 4 KB: 64 x
+// 40 000 float32 31 us, of 32 KB 23.5, of 64 KB 24.4.)
+int grad_splits(const sp_distill_args *a) {
+    const bool cached = a->n_rows * a->n_cols * (a->dtype == SP_DT_F32 ? 4 : 2) <= CACHE_BYTES;
+    return splits_of(a, cached ? GRAD_WGS / 2 : GRAD_WGS, 64 << 10, 32 << 10);
 }
 i64 chunk_of(const sp_distill_args *a, int splits) { return ceil_div(ceil_div(a->n_cols, splits), 64) * 64; }
 
-size_t distill_stats_bytes(const sp_distill_args *a) { return ((size_t)a->n_rows * 8 + 255) & ~(size_t)255; }
+// The one-call kernel keeps `nt * 16` vectors of 16 bytes in registers and more in a share of the LDS of a CU that `wgs` workgroups have.
+constexpr i64 LDS_BYTES = 163840;
+i64 lds_room(const sp_distill_args *a, int nt, int wgs) {
+    const i64 r = (LDS_BYTES / wgs - ListLds::grad_bytes(a->k, nt) - 512) / 16;
+    return r < 0 ? 0 : r;
+}
+// It is taken from as many rows on as fill the card, a workgroup each, and for fewer rows that a CU can keep: one launch instead of three.  (One
+// kernel / scan, join and gradient: 1 row of 40 000 bf16 12.0 / 16.1 us, of 100 000 17.7 / 16.0, of 100 000 float32 14.2 / 16.1; 64 rows 12.1 / 23.4,
+// 22.6 / 29.2, 19.6 / 31.2.  Rows of 300 000 bf16, which are not kept: 1 36 / 16, 64 42 / 37, 128 49 / 53; 256 of 100 000 bf16 28 / 44.)
+constexpr i64 FUSED_ROWS = 256;
+bool one_kernel(const sp_distill_args *a) {
+    return a->n_rows >= FUSED_ROWS || a->n_cols / (a->dtype == SP_DT_F32 ? 4 : 8) <= 16 * 1024 + lds_room(a, 1024, 1);
+}
 
-DistillParams distill_params(const sp_distill_args *a) {
+// the workspace: row statistics between the two halves of a call that is not one kernel, and the partial ones of rows in several pieces
+size_t distill_stats_bytes(const sp_distill_args *a) { return one_kernel(a) ? 0 : ((size_t)a->n_rows * 8 + 255) & ~(size_t)255; }
+i64 distill_ws_bytes(const sp_distill_args *a, bool grad) {
+    if (grad && one_kernel(a)) return 0;
+    const int splits = scan_splits(a);
+    return (grad ? (i64)distill_stats_bytes(a) : 0) + (splits > 1 ? a->n_rows * splits * 8 : 0);
+}
+int check_workspace(const void *ws, i64 have, i64 need) {
+    if (need > 0 && (!ws || have < need)) return fail(SP_EWORKSPACE, "workspace too small: need %lld bytes, got %lld", need, ws ? have : 0ll);
+    return SP_OK;
+}
+
+DistillParams distill_params(const sp_distill_args *a, bool both = false) {
     DistillParams p{};
     p.student = a->student; p.grad = a->grad;
     p.n_rows = a->n_rows; p.n_cols = a->n_cols; p.ld_student = a->ld_student; p.ld_grad = a->ld_grad;
@@ -357,7 +391,7 @@ DistillParams distill_params(const sp_distill_args *a) {
     p.tau = a->temperature; p.inv_tau = 1.f / a->temperature; p.c = (float)(1.4426950408889634074 / (double)a->temperature);
     p.cols = a->cols; p.values = a->values; p.counts = a->counts; p.teacher_lse = a->teacher_lse;
     p.loss = a->loss; p.stats = a->stats; p.grad_loss = a->grad_loss;
-    p.part = (float *)((unsigned char *)a->workspace + distill_stats_bytes(a));
+    p.part = (float *)((unsigned char *)a->workspace + (both ? distill_stats_bytes(a) : 0));
     return p;
 }
 
@@ -366,11 +400,9 @@ int allow_lds(const void *kernel, size_t bytes) {
     if (bytes > 48 * 1024) HIP_TRY(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     return SP_OK;
 }
-constexpr i64 LDS_BYTES = 163840;   // of a CU
-constexpr i64 FUSED_ROWS = 256;      // from as many rows on a workgroup per row fills the card
 
 int launch_scan(const sp_distill_args *a, DistillParams p, hipStream_t stream) {
-    p.splits = splits_of(a, SCAN_WGS);
+    p.splits = scan_splits(a);
     p.chunk = chunk_of(a, p.splits);
     const size_t lists = (size_t)ListLds::loss_bytes(a->k);
     return with_type(a->dtype, [&](auto tag) {
@@ -384,7 +416,7 @@ int launch_scan(const sp_distill_args *a, DistillParams p, hipStream_t stream) {
     });
 }
 int launch_grad(const sp_distill_args *a, DistillParams p, hipStream_t stream) {
-    p.splits = splits_of(a, GRAD_WGS);
+    p.splits = grad_splits(a);
     p.chunk = chunk_of(a, p.splits);
     return with_type(a->dtype, [&](auto tag) {
         using T = decltype(tag);
@@ -394,16 +426,6 @@ int launch_grad(const sp_distill_args *a, DistillParams p, hipStream_t stream) {
         HIP_TRY(hipGetLastError());
         return (int)SP_OK;
     });
-}
-
-// the row statistics between the two halves of a call that is not one kernel, and the partial ones of rows in several pieces
-i64 distill_ws_bytes(const sp_distill_args *a) {
-    const int splits = splits_of(a, SCAN_WGS);
-    return a->n_rows >= FUSED_ROWS && splits == 1 ? 0 : (i64)distill_stats_bytes(a) + a->n_rows * splits * 8;
-}
-int check_workspace(const void *ws, i64 have, i64 need) {
-    if (need > 0 && (!ws || have < need)) return fail(SP_EWORKSPACE, "workspace too small: need %lld bytes, got %lld", need, ws ? have : 0ll);
-    return SP_OK;
 }
 
 }  // namespace
@@ -475,14 +497,14 @@ int sp_adjust_scores(const sp_adjust_args *a) {
 int64_t sp_distill_workspace_bytes(const sp_distill_args *a) {
     if (!a || a->struct_size != sizeof(sp_distill_args)) return fail(SP_EINVAL, "sp_distill_args size mismatch");
     if (a->n_rows < 0 || a->n_rows > I32_MAX || a->n_cols < 0 || a->n_cols > COLS_MAX) return fail(SP_EINVAL, "bad shape");
-    return (int64_t)distill_ws_bytes(a);
+    return (int64_t)distill_ws_bytes(a, a->grad != nullptr);
 }
 
 int sp_distill_loss(const sp_distill_args *a) {
     sp_set_error(0, "");
     TRY(check_distill(a, DISTILL_LOSS));
     if (a->n_rows == 0) return SP_OK;
-    TRY(check_workspace(a->workspace, a->workspace_bytes, distill_ws_bytes(a)));
+    TRY(check_workspace(a->workspace, a->workspace_bytes, distill_ws_bytes(a, false)));
     OnDevice dev;
     TRY(dev.enter(a->device));
     return launch_scan(a, distill_params(a), (hipStream_t)a->stream);
@@ -503,12 +525,12 @@ int sp_distill_loss_grad(const sp_distill_args *a) {
     TRY(check_distill(a, DISTILL_LOSS | DISTILL_GRAD));
     if (a->n_rows == 0) return SP_OK;
     if (a->n_rows > 1 && a->ld_grad < a->n_cols) return fail(SP_EINVAL, "rows of grad overlap");
-    TRY(check_workspace(a->workspace, a->workspace_bytes, distill_ws_bytes(a)));
+    TRY(check_workspace(a->workspace, a->workspace_bytes, distill_ws_bytes(a, true)));
     OnDevice dev;
     TRY(dev.enter(a->device));
     hipStream_t stream = (hipStream_t)a->stream;
-    DistillParams p = distill_params(a);
-    if (a->n_rows < FUSED_ROWS) {
+    DistillParams p = distill_params(a, true);
+    if (!one_kernel(a)) {
         p.stats = (float *)a->workspace;
         TRY(launch_scan(a, p, stream));
         return launch_grad(a, p, stream);
@@ -518,10 +540,7 @@ int sp_distill_loss_grad(const sp_distill_args *a) {
         // The row in registers and LDS, by the smallest kind of workgroup that holds all of it: 8 of 256 threads on a CU, 4 or 2 of 512, one
         // of 1024; the last one takes longer rows as well, and reads the rest twice.
         const i64 vecs = a->n_cols / VecOf<T>::N;
-        auto room = [&](int nt, int wgs) {                     // vectors in a share of the LDS
-            const i64 r = (LDS_BYTES / wgs - ListLds::grad_bytes(a->k, nt) - 512) / 16;
-            return r < 0 ? (i64)0 : r;
-        };
+        auto room = [&](int nt, int wgs) { return lds_room(a, nt, wgs); };
         auto launch = [&](auto kernel, int nt, int rv, int wgs) {
             const i64 more = vecs - (i64)nt * rv;
             p.stage = (int)(more < 0 ? 0 : more < room(nt, wgs) ? more : room(nt, wgs));

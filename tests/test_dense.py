@@ -602,10 +602,12 @@ def test_distill_every_listed_place(dtype, n, v):
 
 
 @gpu
+@pytest.mark.parametrize("n", [257, 5])
 @pytest.mark.parametrize("dtype,v,k", [(torch.float32, 150_001, 3), (torch.float32, 110_003, 4096), (torch.bfloat16, 300_007, 300), (torch.float16, 131_072, 64)])
-def test_distill_rows_longer_than_a_workgroup_keeps(dtype, v, k):
-    """The one call on rows that do not fit registers and LDS (their rest is read twice), in place as well, next to the two calls."""
-    n, some = 257, [0, 100, 256]
+def test_distill_rows_longer_than_a_workgroup_keeps(dtype, v, k, n):
+    """The one call on rows that do not fit registers and LDS (their rest is read twice, or few of them are cut into pieces), in place as well,
+    next to the two calls."""
+    some = [0, n // 2, n - 1]
     gen = torch.Generator(device="cuda").manual_seed(v)
     z = (torch.randn(n, v, generator=gen, device="cuda") * 2).to(dtype)
     cols = torch.randint(0, v, (n, k), generator=gen, device="cuda")
@@ -620,6 +622,44 @@ def test_distill_rows_longer_than_a_workgroup_keeps(dtype, v, k):
     check(loss[some], ref[0], loss_b, "loss of the one call")
     check(grad[some], ref[2], grad_b, "grad of the one call")
     assert torch.equal(dense.distill_loss_grad(z, cols, values, out=z)[1], grad) and torch.equal(z, grad)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,v", [(torch.float32, 120_001), (torch.bfloat16, 400_003), (torch.float16, 220_000)])
+def test_distill_masked_pieces(dtype, v):
+    """Rows long enough to be cut: pieces that are -inf altogether, one column left, the lowest value everywhere, a padded row of NaN, a row of -inf."""
+    rng = np.random.default_rng(v)
+    n, k = 5, 9
+    z = torch.from_numpy(rng.standard_normal((n, v)).astype(np.float32) * 3).to(dtype)
+    cols, values = lists(rng, n, v, k)
+    counts = torch.full((n,), k, dtype=torch.int32)
+    z[0, : v * 2 // 3] = -math.inf
+    cols[0] = torch.arange(v - k, v)
+    z[1, :] = -math.inf
+    z[1, v - 3] = 1.5
+    counts[1], cols[1, 0] = 1, v - 3                                               # p = q = 1 there
+    z[2, :] = torch.finfo(dtype).min
+    z[3, :] = math.nan
+    counts[3] = 0
+    z[4, :] = -math.inf
+    ref = distill_ref(z, cols, values, counts, 1.0, None, None)
+    loss_b, grad_b = distill_bounds(torch.where(z < -1e4, torch.zeros((), dtype=dtype), z), cols, 1.0, ref, None, dtype)
+    want_loss, want_grad = ref[0].clone(), ref[2].clone()
+    want_loss[3], want_loss[4], loss_b[3], grad_b[3] = 0.0, math.inf, 0.0, 0.0
+    want_grad[3], want_grad[4] = 0.0, -ref[4][4]                                   # a row of -inf only has q = 0
+    # the lowest value everywhere: q = 1 / v, which lowest + log v does not tell in 64 bits either (2^128 against log v < 2^4)
+    logp, p = ref[6][2], ref[3][2]
+    want_loss[2] = torch.where(p > 0, p * (logp + math.log(v)), 0.0).sum()
+    want_grad[2] = 1.0 / v - ref[4][2]
+    loss_b[2], grad_b[2] = 400 * U, 40 * U + half_step(dtype) * (want_grad[2].abs() + 40 * U) + tiny(dtype)
+    z, args = z.cuda(), (cols.cuda(), values.cuda(), counts.cuda())
+    loss, stats = dense.distill_loss(z, *args, return_stats=True)
+    check(loss, want_loss, loss_b, "loss")
+    check(dense.distill_grad(z, stats, *args), want_grad, grad_b, "grad")
+    loss, grad = dense.distill_loss_grad(z, *args)
+    check(loss, want_loss, loss_b, "loss of the one call")
+    check(grad, want_grad, grad_b, "grad of the one call")
+    assert torch.equal(dense.distill_loss_grad(z, *args, out=z)[1], grad)
 
 
 @gpu
@@ -941,6 +981,7 @@ def test_c_entries_refuse():
     d.temperature = 1.0
     assert "NULL" in _c("sp_distill_loss", d)[1]
     d.student = d.cols = d.values = 64
+    d.n_cols = 1 << 20                                                             # (rows in pieces: their sums need a workspace)
     assert _c("sp_distill_loss", d)[0] == -5
     assert "grad is NULL" in _c("sp_distill_grad", d)[1]
     d.grad = 64
