@@ -300,7 +300,8 @@ constexpr i64 AD_WGS = 2048;
 CsrPattern pattern_of(const sp_csr_pattern &m) { return {m.indptr, m.indices, m.n_rows, m.nnz, m.index64}; }
 
 template <typename T> int launch_adjust(AdjustParams p, bool counts, hipStream_t stream) {
-    // a row in segments of up to AD_SEG columns; few rows in shorter ones, down to 2048, so that about AD_WGS workgroups run
+    // A row in segments of up to AD_SEG columns; few rows in shorter ones, down to 2048, so that about AD_WGS workgroups run.  (512 / 1024 / 2048 / 4096
+    // of them: 64 x 100 000 f16 with target lists 21 / 19 / 16.6 / 17.4 us, 512 x 10 000 bf16 with a history, a filter and a bias 18.7 / 15.0 / 13.0 / 14.2.)
     i64 segs = ceil_div(p.n_cols, AD_SEG);
     const i64 want = ceil_div(AD_WGS, p.n_rows), most = ceil_div(p.n_cols, 2048);
     if (segs < want) segs = want < most ? want : most;
