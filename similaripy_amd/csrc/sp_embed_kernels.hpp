@@ -445,7 +445,7 @@ template <typename I> __global__ __launch_bounds__(SMALL_NT) void sp_sort_small_
         match_digits(digit, same, rounds, p.bits);
         for (int i = tid; i < SMALL_WAVES * SORT_BINS; i += SMALL_NT) (&off[0][0])[i] = 0u;
         __syncthreads();
-        unsigned rank[SMALL_PER];                              // among the wave's entries of the digit in this round
+        unsigned rank[SMALL_PER];                              // among the equal digits of its 64 entries
 #pragma unroll
         for (int q = 0; q < SMALL_PER; ++q)
             if (q < rounds && first + q * 64 < n) {

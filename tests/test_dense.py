@@ -269,6 +269,31 @@ def test_embed_grad_wide_rows(dtype, rows, dim):
 
 
 @gpu
+@pytest.mark.parametrize("dim", [3, 16, 129, 600])
+@pytest.mark.parametrize("chunk,longest", [(8, 2300), (16, 9000)])
+def test_embed_grad_runs_over_chunks(dim, chunk, longest):
+    """Ids that occur so often that their entries, sorted, end just before, at and just behind the ends of 1 .. 10 chunks and of hundreds."""
+    rng = np.random.default_rng(dim)
+    runs = [c * chunk + d for c in (0, 1, 2, 6, 7, 8, 9, 10) for d in (-1, 0, 1) if c * chunk + d > 0] + [longest] + [1, 2, 3] * 20
+    runs += [chunk * 9] * 3 + [chunk] * 5
+    ids = np.repeat(np.arange(len(runs)) * 3, runs)
+    n, vocab = len(ids), 3 * len(runs)
+    assert (2048 < n <= 6144) == (chunk == 8)
+    at = rng.permutation(n)
+    grad = torch.from_numpy(rng.standard_normal((n, dim)).astype(np.float32))
+    idx = torch.from_numpy(ids[at].astype(np.int64))
+    want = torch.zeros(vocab, dim, dtype=torch.float64).index_add_(0, idx, grad.double())
+    mag = torch.zeros(vocab, dim, dtype=torch.float64).index_add_(0, idx, grad.double().abs())
+    bound = (2 * torch.bincount(idx, minlength=vocab).double()[:, None] + 1) * U * mag      # an addition an entry, the joins' as many at most, one rounding
+    for _ in range(2):
+        check(dense.embed_rows_grad(grad.cuda(), idx.cuda(), vocab), want, bound)
+    base = torch.ones(vocab, dim, device="cuda")
+    dense.embed_rows_grad(grad.cuda(), idx.cuda(), vocab, out=base, accumulate=True)
+    check(base, want + 1, bound + U * (mag + 1))
+    assert (base[1::3] == 1).all()
+
+
+@gpu
 def test_embed_autograd():
     """The graph's gradient is embed_rows_grad's, also through a broadcast sum, for a table used twice, and against differences."""
     rng = np.random.default_rng(3)
