@@ -80,7 +80,9 @@ template <typename F> __device__ __forceinline__ void scan_list(const CsrPattern
 
 constexpr int AD_SEG = 16384;      // most columns of a segment: 2 KB of LDS for each kind of bit
 constexpr int AD_SLOTS = 2048;     // slots of the hash table {column, count}: 16 KB
-constexpr int AD_HASHED = 1536;    // entries it takes; more are counted in tiles of 2 * AD_SLOTS columns
+constexpr int AD_HASHED = 1536;    // columns it takes (and one more for each thread); more are counted in tiles of 4 * AD_SLOTS columns, 16 bits each,
+                                   // or, of a history that 16 bits do not count, of 2 * AD_SLOTS
+static_assert(AD_HASHED + 1 + AD_NT < AD_SLOTS, "a free slot is left");
 
 __device__ __forceinline__ unsigned ad_slot(int c) { return ((unsigned)c * 2654435761u) >> (32 - 11); }
 static_assert(AD_SLOTS == 1 << 11, "ad_slot");
@@ -111,14 +113,15 @@ __device__ __forceinline__ void table_clear(unsigned *table) {
         table[AD_SLOTS + i] = 0u;
     }
 }
-__device__ __forceinline__ void table_count(unsigned *table, int c) {
-    unsigned h = ad_slot(c);
-    for (;;) {                                                 // (at most AD_HASHED of AD_SLOTS are taken: there is a free one)
-        const unsigned was = atomicCAS(&table[h], ~0u, (unsigned)c);
+__device__ __forceinline__ bool table_count(unsigned *table, int c) {      // true: a column that was not there
+    unsigned h = ad_slot(c), was;
+    for (;;) {                                                 // (not all of AD_SLOTS are taken)
+        was = atomicCAS(&table[h], ~0u, (unsigned)c);
         if (was == ~0u || was == (unsigned)c) break;
         h = (h + 1) & (AD_SLOTS - 1);
     }
     atomicAdd(&table[AD_SLOTS + h], 1u);
+    return was == ~0u;
 }
 __device__ __forceinline__ unsigned table_find(const unsigned *table, int c) {      // 0: not there
     unsigned h = ad_slot(c);
@@ -162,17 +165,18 @@ template <typename T, bool COUNTS> __global__ __launch_bounds__(AD_NT) void sp_a
         if (p.filter.indptr) __syncthreads();
     }
     if (p.filter.indptr) scan_list(p.filter, filter, c0, 0, width, [&](int c) { atomicOr(&gone[c >> 5], 1u << (c & 31)); });
-    bool hashed = true;
+    bool hashed = true;                                        // else the counts are taken tile by tile
+    const bool narrow = COUNTS && history.e - history.b <= 0xFFFF;
     if (COUNTS) {
         if (history.e - history.b <= AD_HASHED)
             scan_list(p.history, history, c0, 0, width, [&](int c) { atomicOr(&hit[c >> 5], 1u << (c & 31)); table_count(table, c); });
-        else {                                                 // a long history: how much of it lies in this segment decides
-            int mine = 0;
-            scan_list(p.history, history, c0, 0, width, [&](int c) { atomicOr(&hit[c >> 5], 1u << (c & 31)); ++mine; });
-            if (mine) atomicAdd(&n_hits, mine);
+        else {                                                 // a long history: how many columns of this segment are in it decides
+            scan_list(p.history, history, c0, 0, width, [&](int c) {
+                atomicOr(&hit[c >> 5], 1u << (c & 31));
+                if (*(volatile int *)&n_hits <= AD_HASHED && table_count(table, c)) atomicAdd(&n_hits, 1);
+            });
             __syncthreads();
             hashed = n_hits <= AD_HASHED;
-            if (hashed) scan_list(p.history, history, c0, 0, width, [&](int c) { table_count(table, c); });
         }
     }
     __syncthreads();
@@ -180,7 +184,7 @@ template <typename T, bool COUNTS> __global__ __launch_bounds__(AD_NT) void sp_a
     const unsigned char *bits = p.allowed ? (const unsigned char *)(p.allowed + row * p.ld_allowed) + c0 / 8 : nullptr;
     const i64 bias0 = row * p.ld_bias + c0;
 
-    // N columns from c on: what becomes of their scores, with their biases and the byte of `allowed` that holds column c.  tile >= 0: the count of column c is table[c - tile]
+    // N columns from c on: what becomes of their scores, with their biases and the byte of `allowed` that holds column c.  tile >= 0: the counts are those of a tile
     auto adjust = [&](auto nc, float *y, const float *bias, unsigned allow, int c, int tile) {
         constexpr int M = decltype(nc)::value;
         if (COUNTS) {
@@ -190,7 +194,8 @@ template <typename T, bool COUNTS> __global__ __launch_bounds__(AD_NT) void sp_a
                 float v = y[0];
 #pragma unroll
                 for (int j = 1; j < M; ++j) v = at == j ? y[j] : v;
-                v = pen.of(v, tile >= 0 ? table[c + at - tile] : table_find(table, c + at));
+                const int t = c + at - tile;
+                v = pen.of(v, tile < 0 ? table_find(table, c + at) : narrow ? table[t >> 1] >> (t & 1) * 16 & 0xFFFFu : table[t]);
 #pragma unroll
                 for (int j = 0; j < M; ++j) y[j] = at == j ? v : y[j];
             }
@@ -250,14 +255,15 @@ template <typename T, bool COUNTS> __global__ __launch_bounds__(AD_NT) void sp_a
         stream(0, width, -1);
         return;
     }
-    const int step = hashed ? AD_SEG : 2 * AD_SLOTS;
+    const int step = hashed ? AD_SEG : narrow ? 4 * AD_SLOTS : 2 * AD_SLOTS;
     for (int from = 0; from < width; from += step) {
         const int to = min(from + step, width);
         if (!hashed) {
             __syncthreads();                                   // (the tile before has been read)
-            for (int i = tid; i < to - from; i += AD_NT) table[i] = 0u;
+            for (int i = tid; i < 2 * AD_SLOTS; i += AD_NT) table[i] = 0u;
             __syncthreads();
-            scan_list(p.history, history, c0, from, to - from, [&](int c) { atomicAdd(&table[c], 1u); });
+            if (narrow) scan_list(p.history, history, c0, from, to - from, [&](int c) { atomicAdd(&table[c >> 1], 1u << (c & 1) * 16); });
+            else scan_list(p.history, history, c0, from, to - from, [&](int c) { atomicAdd(&table[c], 1u); });
             __syncthreads();
         }
         stream(from, to, hashed ? -1 : from);
