@@ -5,13 +5,14 @@
 // The lists are the sparse product's selectors (similaripy/cython_code/s_plus.h:159-188 looks every candidate up in its row's
 // list); here the row is dense, so the lookup is turned round: a workgroup first writes what the row's lists say about its segment
 // of columns into LDS and then streams the segment past it without a barrier.  Two bits per column (masked, listed in the history) are
-// all that most columns need; the count of a listed column is in a hash table.  A history with more entries in the segment than the
+// all that most columns need; the count of a listed column is in a hash table.  A history with more columns in the segment than the
 // table holds is counted column by column instead, a tile at a time in the table's memory.  Lists need no order, and a column
 // listed several times is counted exactly (integer LDS adds: their order does not matter).
 //
-// Measured: 512 x 100 000 bf16 with a history and a filter of 144 entries and a float32 bias 54 us; 1021 x 84 431 f16 with 1000 target
+// Measured: 512 x 100 000 bf16 with a history and a filter of 144 entries and a float32 bias 52 us; 1021 x 84 431 f16 with 1000 target
 // columns, 64 filtered ones and packed bits 86 us.  The same rows without lists and bias move at 5.9 TB/s (34.4 us) and 5.0 TB/s (69 us):
-// the bias costs 11 us (as many bytes again, from L2), the lists the rest, in registers and in the start of every workgroup.  Writing the
+// the bias costs 11 us (as many bytes again, from L2), the lists the rest, in registers and in the start of every workgroup.  Long histories are
+// bound by the instructions of listed columns, which a wave executes for its lane with the most of them: 231 us with 4000 entries a row.  Writing the
 // listed columns once more after the stream instead was no faster for 144 entries a row and twice as slow for 1000.
 #pragma once
 #include <type_traits>
@@ -80,8 +81,10 @@ template <typename F> __device__ __forceinline__ void scan_list(const CsrPattern
 
 constexpr int AD_SEG = 16384;      // most columns of a segment: 2 KB of LDS for each kind of bit
 constexpr int AD_SLOTS = 2048;     // slots of the hash table {column, count}: 16 KB
-constexpr int AD_HASHED = 1536;    // columns it takes (and one more for each thread); more are counted in tiles of 4 * AD_SLOTS columns, 16 bits each,
-                                   // or, of a history that 16 bits do not count, of 2 * AD_SLOTS
+// Columns it takes (and one more for each thread); more are counted in tiles of 4 * AD_SLOTS columns, 16 bits each, or, of a history that 16 bits
+// do not count, of 2 * AD_SLOTS.  A fuller table saves readings of the list and costs longer searches.  (512 / 1024 / 1536, 512 x 100 000 bf16: mean
+// histories of 1000 entries 92 / 88 / 84 us, of 4000 231 / 231 / 243; 512 x 10 000 with 2000 entries 59 / 63 / 76.)
+constexpr int AD_HASHED = 1024;
 static_assert(AD_HASHED + 1 + AD_NT < AD_SLOTS, "a free slot is left");
 
 __device__ __forceinline__ unsigned ad_slot(int c) { return ((unsigned)c * 2654435761u) >> (32 - 11); }
@@ -135,7 +138,7 @@ __device__ __forceinline__ unsigned table_find(const unsigned *table, int c) {  
 
 // One workgroup per segment of a row
 template <typename T, bool COUNTS> __global__ __launch_bounds__(AD_NT) void sp_adjust_kernel(AdjustParams p) {
-    constexpr int N = VecOf<T>::N, U = 1;      // vectors in flight per thread: occupancy does more than depth (1: 54 / 86 us, 2: 55 / 90, 4: 62 / 115 for the two shapes above)
+    constexpr int N = VecOf<T>::N, U = 1;      // vectors in flight per thread: occupancy does more than depth (1: 54 / 86 us, 2: 55 / 90, 4: 62 / 115 for the two shapes above, as first measured)
     __shared__ unsigned gone[AD_SEG / 32];                     // masked by filter or target lists
     __shared__ unsigned hit[COUNTS ? AD_SEG / 32 : 1];         // listed in the history
     __shared__ unsigned table[COUNTS ? 2 * AD_SLOTS : 1];      // hash: columns, then counts; tiles: counts

@@ -427,6 +427,23 @@ def test_adjust_infinities_nan_and_layouts(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("cols,distinct,entries", [(16_384, 1024, 1600), (16_384, 1025, 3000), (16_384, 1300, 60_000), (16_384, 5000, 65_535), (16_384, 5000, 65_536),
+                                                   (16_384, 9000, 70_000), (40_001, 20_000, 40_000), (2048, 2048, 2048), (5000, 1, 2_000_000)])
+def test_adjust_long_histories(cols, distinct, entries):
+    """Histories at, below and above what a segment's table holds and what 16 bits count: every count is exact, in place as well."""
+    rng = np.random.default_rng(entries)
+    listed = rng.permutation(cols)[:distinct]
+    ids = np.concatenate([listed, rng.choice(listed, entries - distinct)])
+    count = torch.from_numpy(np.bincount(ids, minlength=cols))
+    indptr = torch.tensor([0, 0, entries], dtype=torch.int32, device="cuda")
+    history = (indptr, torch.from_numpy(rng.permutation(ids).astype(np.int32)).cuda())
+    scores = torch.zeros(2, cols, device="cuda")
+    want = torch.stack([torch.zeros(cols, dtype=torch.int64), -count])              # 0 - 0 - 1 * count, below 2^24: exact
+    assert torch.equal(dense.adjust_scores(scores, history=history, frequency=1.0).long().cpu(), want)
+    assert torch.equal(dense.adjust_scores(scores, history=history, frequency=1.0, out=scores).long().cpu(), want)
+
+
+@gpu
 def test_adjust_counts_repeats_exactly():
     """A column listed 100 000 times: the count is a whole number, the penalty its exact multiple."""
     scores = torch.zeros(1, 100, device="cuda")
