@@ -45,20 +45,22 @@ __device__ __forceinline__ MaxSum wave_join(MaxSum a, float c) {
 }
 
 // exp2((z - m) c) is taken as exp2(z c - off) 2^-r, one fused operation per score with off = m c rounded and r = m c - off what the
-// rounding left (exact as a fused operation, the same for the whole row): scores far from 0 lose nothing.  Where m c leaves float32 (a row of the type's
-// lowest value) the scores that are not m itself are too far below it to count: a power of two in the place of c then keeps
-// z c - off exactly 0 for them that are.
+// rounding left (exact as a fused operation, the same for the whole row): scores far from 0 lose nothing.  Up to |m c| = 2^31 r is at most
+// 64.  Beyond (a row masked with -1e10, -1e30, the type's lowest value) 2^r would leave float32, and every score that is not m itself lies
+// at least 2^-24 |m| below it, 128 in the exponent: its q is below 2^-126 and counts as 0.  A power of two in the place of c, the one that makes
+// that distance at least 256, then keeps z c - off exactly 0 for the scores that are m.
+constexpr float OFF_MAX = 2147483648.f;
 struct Exponent {
     float c, off;
 };
-__device__ __forceinline__ bool off_fits(float m, float c) { return fabsf(m * c) <= 3.402823466e38f || m == NEG_INF; }
+__device__ __forceinline__ bool off_fits(float m, float c) { return fabsf(m * c) <= OFF_MAX || m == NEG_INF; }
 __device__ __forceinline__ Exponent exponent_of(float m, float c) {
     if (m == NEG_INF) return {c, 0.f};
     if (off_fits(m, c)) return {c, m * c};
     if (fabsf(m) > 3.402823466e38f) return {c, m};              // +inf, NaN: every q is NaN or 0
     int e;
-    (void)frexpf(m, &e);
-    const float pow2 = ldexpf(1.f, 126 - e);
+    (void)frexpf(m, &e);                                       // -69 <= e <= 128: temperatures are at least 1e-30
+    const float pow2 = ldexpf(1.f, 33 - e);
     return {pow2, m * pow2};
 }
 __device__ __forceinline__ float correction_of(float m, Exponent x) { return m == NEG_INF ? 1.f : exp2_fast(-__fmaf_rn(m, x.c, -x.off)); }      // 2^-r
@@ -82,14 +84,14 @@ template <int N> __device__ __forceinline__ void add_vec(Running &a, const float
     float m = a.m;
 #pragma unroll
     for (int j = 0; j < N; ++j) m = fmaxf(m, z[j]);
-    const float off = fminf(fmaxf(m * c, -3.402823466e38f), 3.402823466e38f);
+    const float off = fminf(fmaxf(m * c, -OFF_MAX), OFF_MAX);      // (below, the sum stays as it is, relative to 2^-OFF_MAX; above, it is not used)
     float s = a.s * exp2_fast(a.off - off);
 #pragma unroll
     for (int j = 0; j < N; ++j) s += exp2_fast(__fmaf_rn(z[j], c, -off));
     a = {m, off, s};
 }
 
-// (a maximum whose m c leaves float32 has no sum here: it is nothing next to a larger one, and the row is summed again otherwise)
+// (a maximum whose m c is beyond OFF_MAX has no sum here: it is nothing next to a larger one, and the row is summed again otherwise)
 __device__ __forceinline__ MaxSum finish(const Running &a, float c) {
     return {a.m, a.m == NEG_INF || !off_fits(a.m, c) ? (a.s != a.s ? a.s : 0.f) : a.s * exp2_fast(-__fmaf_rn(a.m, c, -a.off))};
 }
