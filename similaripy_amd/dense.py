@@ -125,6 +125,12 @@ def _extent(t):
     return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
 
 
+def _written(out) -> None:
+    """The caller's output has been written behind torch's back: its version goes up, so that a backward pass that has saved it raises."""
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
+
+
 # torch's own way to a stream's handle costs as much as a launch; torch.compile's generated code uses this one
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -190,6 +196,7 @@ def _embed_forward(table, indices, indptr, data, scale, out):
     flat = None if out is None else out.view(n_rows, dim) if out.dim() != 2 else out
     res = _out("out", flat, (n_rows, dim), table.dtype, table.device, (table, False))
     _abi.call_dense("sp_embed_rows", _embed_args(table, res, indices, indptr, data, n_rows, table.shape[0], dim, scale))
+    _written(out)
     return out if out is not None else res if len(lead) == 1 else res.view(lead + (dim,))
 
 
@@ -273,6 +280,7 @@ def embed_rows_grad(grad: torch.Tensor, indices: torch.Tensor, n_vocab: int, ind
         ws = torch.empty(need, dtype=torch.uint8, device=grad.device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
     _abi.call_dense("sp_embed_rows_grad", a)
+    _written(out)
     return res
 
 
@@ -367,6 +375,7 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
     a = _abi.SpAdjustArgs(0, 0, device.index or 0, _DT[scores.dtype], n, n_cols, _ld(scores), _ld(res), scores.data_ptr(), res.data_ptr(), tptr, t64, bdt,
                           h, f, t, rep, pres, freq, rep_all, pres_all, freq_all, 0, bptr, ldb, aptr, lda, _stream(device))
     _abi.call_dense("sp_adjust_scores", a)
+    _written(out)
     return res
 
 
@@ -499,6 +508,7 @@ def distill_grad(student: torch.Tensor, stats: torch.Tensor, cols: torch.Tensor,
     grad, g = _grad_outputs(a, student, grad_loss, out)
     a.stats = stats.data_ptr()
     _abi.call_dense("sp_distill_grad", a)
+    _written(out)
     del keep, g
     return grad
 
@@ -515,5 +525,6 @@ def distill_loss_grad(student: torch.Tensor, cols: torch.Tensor, values: torch.T
     a.loss = loss.data_ptr()
     ws = _workspace(a, student.device)
     _abi.call_dense("sp_distill_loss_grad", a)
+    _written(out)
     del ws, keep, g
     return loss, grad

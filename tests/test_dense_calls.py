@@ -67,3 +67,63 @@ def test_distill_masks_of_any_size(dtype, mask, tau, n, v):
     check(grad[some], ref[2], grad_b, "grad of the one call")
     assert not loss.isnan().any() and not grad.isnan().any()
     assert torch.equal(dense.distill_loss_grad(z, *args, temperature=tau, out=z)[1], grad)
+
+
+# ---- what torch has to know: changed outputs, tangents, traces --------------------------------------------------------------------
+
+def small(device):
+    """A call of every function, as (function of named operands, its float operands)."""
+    z = torch.randn(3, 8, device=device)
+    ids = torch.tensor([0, 2, 1], device=device)
+    ptr = torch.tensor([0, 1, 3], device=device)
+    w = torch.ones(3, device=device)
+    cols, values = torch.tensor([[0, 1]] * 3, device=device), torch.randn(3, 2, device=device)
+    stats = torch.ones(3, 2, device=device)
+    return {
+        "embed_rows": (lambda table, data: dense.embed_rows(table, ids, ptr, data), {"table": z, "data": w}),
+        "embed_rows out": (lambda out: dense.embed_rows(z, ids, out=out), {"out": torch.empty(3, 8, device=device)}),
+        "embed_rows_grad": (lambda grad, data: dense.embed_rows_grad(grad, ids, 5, ptr, data), {"grad": z[:2].clone(), "data": w}),
+        "embed_rows_grad out": (lambda out: dense.embed_rows_grad(z, ids, 3, out=out), {"out": torch.empty(3, 8, device=device)}),
+        "adjust_scores": (lambda scores, bias, repetition, presence, frequency: dense.adjust_scores(
+            scores, history=(torch.tensor([0, 1, 1, 1], device=device), ids[:1]), bias=bias, repetition=repetition, presence=presence, frequency=frequency),
+            {"scores": z, "bias": torch.zeros(8, device=device), "repetition": w, "presence": w, "frequency": w}),
+        "adjust_scores out": (lambda out: dense.adjust_scores(z, bias=z[0].clone(), out=out), {"out": torch.empty(3, 8, device=device)}),
+        "distill_loss": (lambda student, values, teacher_lse: dense.distill_loss(student, cols, values, teacher_lse=teacher_lse),
+                         {"student": z, "values": values, "teacher_lse": w * 2}),
+        "distill_grad": (lambda student, stats, values, grad_loss: dense.distill_grad(student, stats, cols, values, grad_loss=grad_loss),
+                         {"student": z, "stats": stats, "values": values, "grad_loss": w}),
+        "distill_grad out": (lambda out: dense.distill_grad(z, stats, cols, values, out=out), {"out": torch.empty(3, 8, device=device)}),
+        "distill_loss_grad": (lambda student, values, grad_loss, teacher_lse: dense.distill_loss_grad(
+            student, cols, values, grad_loss=grad_loss, teacher_lse=teacher_lse), {"student": z, "values": values, "grad_loss": w, "teacher_lse": w}),
+        "distill_loss_grad out": (lambda out: dense.distill_loss_grad(z, cols, values, out=out), {"out": torch.empty(3, 8, device=device)}),
+    }
+
+
+CALLS = list(small("cpu"))
+DEVICES = ["cpu", pytest.param("cuda", marks=gpu)]
+
+
+@gpu
+@pytest.mark.parametrize("name", [c for c in CALLS if c.endswith(" out")])
+def test_outputs_count_as_changed(name):
+    """A tensor that an autograd graph has saved may be written by a call, but not unnoticed: its version goes up, also through views."""
+    fn, operands = small("cuda")[name]
+    out = operands["out"]
+    before, row = out._version, out[1]
+    fn(**operands)
+    assert out._version > before and row._version == out._version
+    with torch.inference_mode():                        # (tensors made there have no version)
+        fn, operands = small("cuda")[name]
+        fn(**operands)
+
+
+@gpu
+def test_backward_of_an_overwritten_student():
+    """The backward pass needs the scores: overwritten in place meanwhile, it raises as it does for torch's own operators."""
+    leaf = torch.randn(3, 50, device="cuda", requires_grad=True)
+    cols, values = torch.tensor([[0, 1]] * 3, device="cuda"), torch.randn(3, 2, device="cuda")
+    scores = leaf * 1.0
+    loss = dense.distill_loss(scores, cols, values)
+    dense.adjust_scores(scores.detach(), bias=torch.ones(50, device="cuda"), out=scores.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.sum().backward()
