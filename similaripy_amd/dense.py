@@ -20,7 +20,7 @@ no operand but where its function says so.
 
 Autograd and graph capture: inside a capture the functions that build an autograd graph refuse inputs that require a gradient
 (the backward pass of a captured graph would meet leaves whose gradients belong to another stream): capture the explicit
-``embed_rows_grad``, ``distill_grad`` or ``distill_loss_grad`` instead.
+``embed_rows_grad``, ``distill_grad`` or ``distill_loss_grad`` instead.  Operands with a forward-mode tangent are refused.
 """
 from __future__ import annotations
 
@@ -28,6 +28,7 @@ import math
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _abi
@@ -155,6 +156,14 @@ def _not_capturing(name: str, instead: str) -> None:
         raise RuntimeError(f"{name} on tensors that require a gradient cannot be captured into a graph: capture {instead} on detached tensors")
 
 
+def _no_tangents(*operands) -> None:
+    """Every entry begins with this: the kernels read plain memory, an operand's tangent would be dropped (a derivative of 0)."""
+    if forward_ad._current_level >= 0:
+        for t in operands:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the dense operators have no forward-mode derivative: an operand has a tangent")
+
+
 # ---- embedding rows ------------------------------------------------------------------------------------------------------------
 
 def _rows(t):
@@ -231,6 +240,7 @@ def embed_rows(table: torch.Tensor, indices: torch.Tensor, indptr: Optional[torc
     data      [nnz] float32 weights (the CSR's data), default ones
     out       optional output (no autograd graph is built then)
     """
+    _no_tangents(table, data, scale, out)
     _dense("table", table)
     scale = float(scale)
     if data is not None:
@@ -256,6 +266,7 @@ def embed_rows_grad(grad: torch.Tensor, indices: torch.Tensor, n_vocab: int, ind
     out         optional [n_vocab, dim] output
     accumulate  add to ``out``; rows of ids that do not occur are neither read nor written
     """
+    _no_tangents(grad, data, scale, out)
     if not isinstance(grad, torch.Tensor):
         raise TypeError(f"grad must be a torch.Tensor, got {type(grad).__name__}")
     if indptr is None and grad.dim() != 2 and grad.dim() > 0:
@@ -333,6 +344,7 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
     target_cols  (indptr, indices): columns that are not listed become ``-inf``
     out          optional output; may be ``scores`` itself
     """
+    _no_tangents(scores, repetition, presence, frequency, bias, out)
     _dense("scores", scores)
     _no_grad_here("adjust_scores", scores)
     n, n_cols = scores.shape
@@ -473,6 +485,7 @@ def distill_loss(student: torch.Tensor, cols: torch.Tensor, values: torch.Tensor
     return_stats also return [n, 2] float32, every row's maximum ``m`` and the sum of ``exp((student - m) / temperature)``, which
                  :func:`distill_grad` takes (their log-sum-exp ``m / temperature + log(sum)`` in two parts)
     """
+    _no_tangents(student, values, temperature, teacher_lse)
     _fixed("values", values)
     if teacher_lse is not None:
         _fixed("teacher_lse", teacher_lse)
@@ -502,6 +515,7 @@ def distill_grad(student: torch.Tensor, stats: torch.Tensor, cols: torch.Tensor,
     grad_loss  [n] float32 gradient of every row's loss, default ones
     out        optional output; may be ``student`` itself
     """
+    _no_tangents(student, stats, values, grad_loss, temperature, teacher_lse, out)
     a, keep = _distill_args(student, cols, values, counts, temperature, teacher_lse)
     _no_grad_here("distill_grad", student)
     stats = _floats("stats", stats, student.device, 2 * student.shape[0])
@@ -518,6 +532,7 @@ def distill_loss_grad(student: torch.Tensor, cols: torch.Tensor, values: torch.T
                       out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Loss and gradient of :func:`distill_loss` in one call, for a training step that knows the gradient of the losses beforehand
     (``1 / n`` for their mean).  Arguments as in :func:`distill_grad`."""
+    _no_tangents(student, values, grad_loss, temperature, teacher_lse, out)
     a, keep = _distill_args(student, cols, values, counts, temperature, teacher_lse)
     _no_grad_here("distill_loss_grad", student)
     loss = torch.empty(student.shape[0], dtype=torch.float32, device=student.device)

@@ -127,3 +127,20 @@ def test_backward_of_an_overwritten_student():
     dense.adjust_scores(scores.detach(), bias=torch.ones(50, device="cuda"), out=scores.detach())
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.sum().backward()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("name", CALLS)
+def test_forward_mode_is_refused(name, device):
+    """An operand with a tangent: the result would have none, a derivative of 0."""
+    import torch.autograd.forward_ad as fwd
+    fn, operands = small(device)[name]
+    for which, t in operands.items():
+        with fwd.dual_level():
+            dual = fwd.make_dual(t.clone(), torch.ones_like(t))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                fn(**{**operands, which: dual})
+    if device == "cuda":                                # a level that these operands are not part of is nobody's business
+        with fwd.dual_level():
+            fwd.make_dual(torch.ones(2), torch.ones(2))
+            fn(**operands)
