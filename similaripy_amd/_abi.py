@@ -535,12 +535,11 @@ _dense_fns = {}      # entries of include/sp_dense.h that have been called
 
 
 def call_dense(symbol: str, args) -> int:
-    """One entry of include/sp_dense.h: 0, or the bytes a workspace query answers."""
+    """One entry of include/sp_dense.h (`args` with its struct_size): 0, or the bytes a workspace query answers."""
     fn = _dense_fns.get(symbol)
     if fn is None:
         fn = _dense_fns[symbol] = getattr(load(), symbol)
-    args.struct_size = C.sizeof(args)
-    rc = fn(C.byref(args))
+    rc = fn(args)                  # (by reference: what its argtypes say)
     if rc < 0:
         raise HipLibraryError(f"{symbol} failed ({rc}): {last_error()}")
     return rc

@@ -20,10 +20,12 @@ no operand but where its function says so.
 
 Autograd and graph capture: inside a capture the functions that build an autograd graph refuse inputs that require a gradient
 (the backward pass of a captured graph would meet leaves whose gradients belong to another stream): capture the explicit
-``embed_rows_grad``, ``distill_grad`` or ``distill_loss_grad`` instead.  Operands with a forward-mode tangent are refused.
+``embed_rows_grad``, ``distill_grad`` or ``distill_loss_grad`` instead.  Operands with a forward-mode tangent are refused, and so
+are calls inside ``torch.jit.trace``, ``make_fx`` and ``torch.export``; ``torch.compile`` runs them between its graphs.
 """
 from __future__ import annotations
 
+import ctypes as C
 import math
 from typing import Optional, Tuple, Union
 
@@ -40,6 +42,7 @@ _PerRow = Union[float, torch.Tensor]
 
 _DT = {torch.float32: _abi.SP_DT_F32, torch.bfloat16: _abi.SP_DT_BF16, torch.float16: _abi.SP_DT_F16}
 _INT = (torch.int32, torch.int64)
+_EMBED_SIZE, _ADJUST_SIZE, _DISTILL_SIZE = (C.sizeof(s) for s in (_abi.SpEmbedArgs, _abi.SpAdjustArgs, _abi.SpDistillArgs))
 
 
 # ---- argument checks ---------------------------------------------------------------------------------------------------------
@@ -132,12 +135,14 @@ def _written(out) -> None:
         torch.autograd.graph.increment_version(out)
 
 
-# torch's own way to a stream's handle costs as much as a launch; torch.compile's generated code uses this one
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
 def _stream(device) -> int:
-    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# torch's own way to a stream's handle costs as much as a launch; torch.compile's generated code uses this one
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    def _stream(device, _raw=torch._C._cuda_getCurrentRawStream) -> int:  # noqa: F811
+        return _raw(device.index)
 
 
 def _no_grad_here(name: str, t) -> None:
@@ -156,8 +161,16 @@ def _not_capturing(name: str, instead: str) -> None:
         raise RuntimeError(f"{name} on tensors that require a gradient cannot be captured into a graph: capture {instead} on detached tensors")
 
 
-def _no_tangents(*operands) -> None:
-    """Every entry begins with this: the kernels read plain memory, an operand's tangent would be dropped (a derivative of 0)."""
+_is_tracing, _modes, _pre_dispatch = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._ops.mode_stack_state_for_pre_dispatch()
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
+def _plain(*operands) -> None:
+    """Every entry begins with this.  The kernels read and write memory behind torch's back: a tangent would be dropped (a derivative of 0),
+    and a recorded graph (torch.jit.trace, make_fx, torch.export) would hold the allocation of the output and nothing else.  torch.compile breaks
+    its graph at these calls and needs no refusal."""
+    if _is_tracing() or (_modes() and torch._C._get_dispatch_mode(_PROXY) is not None) or (_pre_dispatch.count() and torch._ops._get_dispatch_mode_pre_dispatch(_PROXY) is not None):
+        raise RuntimeError("the dense operators cannot be traced: a recorded graph would not hold their kernels")
     if forward_ad._current_level >= 0:
         for t in operands:
             if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
@@ -190,7 +203,7 @@ def _csr_of(indices, indptr, data, device):
 
 def _embed_args(src, out, indices, indptr, data, n_rows, n_vocab, dim, scale, accumulate=0):
     dev = src.device
-    return _abi.SpEmbedArgs(0, 0, dev.index or 0, _DT[src.dtype], _DT[out.dtype], 1 if indices.dtype == torch.int64 else 0, accumulate, scale,
+    return _abi.SpEmbedArgs(_EMBED_SIZE, 0, dev.index, _DT[src.dtype], _DT[out.dtype], 1 if indices.dtype == torch.int64 else 0, accumulate, scale,
                             n_rows, n_vocab, dim, indices.numel(), _ld(src), _ld(out), src.data_ptr(), indices.data_ptr(),
                             None if indptr is None else indptr.data_ptr(), None if data is None else data.data_ptr(), out.data_ptr(), _stream(dev))
 
@@ -240,7 +253,7 @@ def embed_rows(table: torch.Tensor, indices: torch.Tensor, indptr: Optional[torc
     data      [nnz] float32 weights (the CSR's data), default ones
     out       optional output (no autograd graph is built then)
     """
-    _no_tangents(table, data, scale, out)
+    _plain(table, data, scale, out)
     _dense("table", table)
     scale = float(scale)
     if data is not None:
@@ -266,7 +279,7 @@ def embed_rows_grad(grad: torch.Tensor, indices: torch.Tensor, n_vocab: int, ind
     out         optional [n_vocab, dim] output
     accumulate  add to ``out``; rows of ids that do not occur are neither read nor written
     """
-    _no_tangents(grad, data, scale, out)
+    _plain(grad, data, scale, out)
     if not isinstance(grad, torch.Tensor):
         raise TypeError(f"grad must be a torch.Tensor, got {type(grad).__name__}")
     if indptr is None and grad.dim() != 2 and grad.dim() > 0:
@@ -344,7 +357,7 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
     target_cols  (indptr, indices): columns that are not listed become ``-inf``
     out          optional output; may be ``scores`` itself
     """
-    _no_tangents(scores, repetition, presence, frequency, bias, out)
+    _plain(scores, repetition, presence, frequency, bias, out)
     _dense("scores", scores)
     _no_grad_here("adjust_scores", scores)
     n, n_cols = scores.shape
@@ -384,7 +397,7 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
         keep.append(allowed)
         aptr, lda = allowed.data_ptr(), 0 if allowed.dim() == 1 else words
     res = _out("out", out, (n, n_cols), scores.dtype, device, (scores, True), (bias, False))
-    a = _abi.SpAdjustArgs(0, 0, device.index or 0, _DT[scores.dtype], n, n_cols, _ld(scores), _ld(res), scores.data_ptr(), res.data_ptr(), tptr, t64, bdt,
+    a = _abi.SpAdjustArgs(_ADJUST_SIZE, 0, device.index, _DT[scores.dtype], n, n_cols, _ld(scores), _ld(res), scores.data_ptr(), res.data_ptr(), tptr, t64, bdt,
                           h, f, t, rep, pres, freq, rep_all, pres_all, freq_all, 0, bptr, ldb, aptr, lda, _stream(device))
     _abi.call_dense("sp_adjust_scores", a)
     _written(out)
@@ -422,7 +435,7 @@ def _distill_args(student, cols, values, counts, temperature, teacher_lse):
     temperature = float(temperature)
     if not 1e-30 < temperature < 1e30:
         raise ValueError(f"temperature must be positive, got {temperature}")
-    a = _abi.SpDistillArgs(0, 0, device.index or 0, _DT[student.dtype], n, n_cols, _ld(student), 0, k, 1 if cols.dtype == torch.int64 else 0,
+    a = _abi.SpDistillArgs(_DISTILL_SIZE, 0, device.index, _DT[student.dtype], n, n_cols, _ld(student), 0, k, 1 if cols.dtype == torch.int64 else 0,
                            _DT[values.dtype], temperature, student.data_ptr(), cols.data_ptr(), values.data_ptr(),
                            None if counts is None else counts.data_ptr(), None if teacher_lse is None else teacher_lse.data_ptr())
     a.stream = _stream(device)
@@ -485,7 +498,7 @@ def distill_loss(student: torch.Tensor, cols: torch.Tensor, values: torch.Tensor
     return_stats also return [n, 2] float32, every row's maximum ``m`` and the sum of ``exp((student - m) / temperature)``, which
                  :func:`distill_grad` takes (their log-sum-exp ``m / temperature + log(sum)`` in two parts)
     """
-    _no_tangents(student, values, temperature, teacher_lse)
+    _plain(student, values, temperature, teacher_lse)
     _fixed("values", values)
     if teacher_lse is not None:
         _fixed("teacher_lse", teacher_lse)
@@ -515,7 +528,7 @@ def distill_grad(student: torch.Tensor, stats: torch.Tensor, cols: torch.Tensor,
     grad_loss  [n] float32 gradient of every row's loss, default ones
     out        optional output; may be ``student`` itself
     """
-    _no_tangents(student, stats, values, grad_loss, temperature, teacher_lse, out)
+    _plain(student, stats, values, grad_loss, temperature, teacher_lse, out)
     a, keep = _distill_args(student, cols, values, counts, temperature, teacher_lse)
     _no_grad_here("distill_grad", student)
     stats = _floats("stats", stats, student.device, 2 * student.shape[0])
@@ -532,7 +545,7 @@ def distill_loss_grad(student: torch.Tensor, cols: torch.Tensor, values: torch.T
                       out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Loss and gradient of :func:`distill_loss` in one call, for a training step that knows the gradient of the losses beforehand
     (``1 / n`` for their mean).  Arguments as in :func:`distill_grad`."""
-    _no_tangents(student, values, grad_loss, temperature, teacher_lse, out)
+    _plain(student, values, grad_loss, temperature, teacher_lse, out)
     a, keep = _distill_args(student, cols, values, counts, temperature, teacher_lse)
     _no_grad_here("distill_loss_grad", student)
     loss = torch.empty(student.shape[0], dtype=torch.float32, device=student.device)

@@ -78,16 +78,17 @@ def small(device):
     ptr = torch.tensor([0, 1, 3], device=device)
     w = torch.ones(3, device=device)
     cols, values = torch.tensor([[0, 1]] * 3, device=device), torch.randn(3, 2, device=device)
-    stats = torch.ones(3, 2, device=device)
+    stats, row = torch.ones(3, 2, device=device), torch.zeros(8, device=device)
+    history = (torch.tensor([0, 1, 1, 1], device=device), ids[:1])
     return {
         "embed_rows": (lambda table, data: dense.embed_rows(table, ids, ptr, data), {"table": z, "data": w}),
         "embed_rows out": (lambda out: dense.embed_rows(z, ids, out=out), {"out": torch.empty(3, 8, device=device)}),
         "embed_rows_grad": (lambda grad, data: dense.embed_rows_grad(grad, ids, 5, ptr, data), {"grad": z[:2].clone(), "data": w}),
         "embed_rows_grad out": (lambda out: dense.embed_rows_grad(z, ids, 3, out=out), {"out": torch.empty(3, 8, device=device)}),
         "adjust_scores": (lambda scores, bias, repetition, presence, frequency: dense.adjust_scores(
-            scores, history=(torch.tensor([0, 1, 1, 1], device=device), ids[:1]), bias=bias, repetition=repetition, presence=presence, frequency=frequency),
+            scores, history=history, bias=bias, repetition=repetition, presence=presence, frequency=frequency),
             {"scores": z, "bias": torch.zeros(8, device=device), "repetition": w, "presence": w, "frequency": w}),
-        "adjust_scores out": (lambda out: dense.adjust_scores(z, bias=z[0].clone(), out=out), {"out": torch.empty(3, 8, device=device)}),
+        "adjust_scores out": (lambda out: dense.adjust_scores(z, bias=row, out=out), {"out": torch.empty(3, 8, device=device)}),
         "distill_loss": (lambda student, values, teacher_lse: dense.distill_loss(student, cols, values, teacher_lse=teacher_lse),
                          {"student": z, "values": values, "teacher_lse": w * 2}),
         "distill_grad": (lambda student, stats, values, grad_loss: dense.distill_grad(student, stats, cols, values, grad_loss=grad_loss),
@@ -144,3 +145,40 @@ def test_forward_mode_is_refused(name, device):
         with fwd.dual_level():
             fwd.make_dual(torch.ones(2), torch.ones(2))
             fn(**operands)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("name", CALLS)
+def test_traces_are_refused(name, device):
+    """A recorded graph would hold the output's allocation and nothing else."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    fn, operands = small(device)[name]
+    fn_of = lambda *ts: fn(**dict(zip(operands, ts)))  # noqa: E731
+    for kw in ({}, {"pre_dispatch": True}, {"tracing_mode": "fake"}):
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(fn_of, **kw)(*operands.values())
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(fn_of, tuple(operands.values()))
+    if device == "cuda":
+        fn(**operands)
+
+
+@gpu
+def test_compiled_programs():
+    """torch.compile leaves the calls outside its graphs: the results are those of the eager program, gradients too."""
+    cols, values = torch.tensor([[0, 1], [5, 2]], device="cuda"), torch.randn(2, 2, device="cuda")
+    ids, ptr = torch.tensor([0, 3, 1], device="cuda"), torch.tensor([0, 2, 3], device="cuda")
+
+    def program(table, weight):
+        scores = torch.relu(dense.embed_rows(table, ids, ptr) @ weight) + 1.0
+        loss = dense.distill_loss(scores, cols, values)
+        return loss.sum(), dense.adjust_scores((scores * 2.0).detach(), bias=weight[0].detach())
+
+    results = []
+    for f in (program, torch.compile(program, backend="eager")):
+        gen = torch.Generator(device="cuda").manual_seed(1)
+        table, weight = (torch.randn(s, generator=gen, device="cuda").requires_grad_() for s in ((4, 6), (6, 9)))
+        loss, scores = f(table, weight)
+        loss.backward()
+        results.append((loss.detach(), scores, table.grad, weight.grad))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
