@@ -83,7 +83,7 @@ int check_embed(const sp_embed_args *a) {
 
 // Calls f with the lanes of a group and the elements of a lane: 16 bytes a lane, or one element where a row has fewer; the fewest lanes that
 // cover a row, 8 .. 64 (columns beyond 64 lanes make further slabs).
-template <int N, typename F> int with_group(i64 dim, F f) {
+template <int N, typename F> auto with_group(i64 dim, F f) {
     using Wide = std::integral_constant<int, N>;
     if (dim < N) return f(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
     const i64 lanes = ceil_div(dim, N);
@@ -118,6 +118,31 @@ template <typename T> int line_slabs(i64 dim, i64 ld) {
     return 1;
 }
 
+// Workgroups of 256 threads of a lookup or of bags; `cut`: slabs by XCD, or 1.  Bags: a workgroup takes four rows of a slab.
+template <typename T> i64 embed_blocks(const sp_embed_args *a, int cut) {
+    return with_group<VecOf<T>::N>(a->dim / cut, [&](auto gc, auto nc) -> i64 {
+        const i64 slabs = ceil_div(a->dim, decltype(gc)::value * decltype(nc)::value), fours = ceil_div(a->n_rows, 4);
+        if (!a->indptr) return ceil_div(a->n_rows * slabs, 256 / decltype(gc)::value);
+        return cut > 1 ? ceil_div(fours, 8 / slabs) * 8 : fours * slabs;
+    });
+}
+// Slabs by XCD of the bags: for a table beyond the L2 of one from which more rows are taken than it has, and for few bags; not where a
+// workgroup for every four bags of a slab is more than one launch has.
+template <typename T> int bag_slabs(const sp_embed_args *a) {
+    const i64 row_bytes = a->dim * (i64)sizeof(T);
+    const bool large = a->nnz >= a->n_vocab && a->n_vocab * row_bytes > L2_BYTES && row_bytes >= 1024;
+    const int slabs = a->indptr && (large || a->n_rows <= FEW_BAGS) && (uintptr_t)a->src % 128 == 0 ? line_slabs<T>(a->dim, a->ld_src) : 1;
+    return slabs > 1 && !too_many(embed_blocks<T>(a, slabs), 256) ? slabs : 1;
+}
+
+int check_embed_launch(const sp_embed_args *a) {
+    return with_type(a->dtype, [&](auto tag) {
+        using T = decltype(tag);
+        if (a->n_vocab > 0 && too_many(embed_blocks<T>(a, bag_slabs<T>(a)), 256)) return fail(SP_EINVAL, "too many rows for one launch");
+        return (int)SP_OK;
+    });
+}
+
 int run_embed(const sp_embed_args *a) {
     hipStream_t stream = (hipStream_t)a->stream;
     return with_type(a->dtype, [&](auto tag) {
@@ -129,26 +154,19 @@ int run_embed(const sp_embed_args *a) {
             HIP_TRY(hipGetLastError());
             return (int)SP_OK;
         }
-        auto run = [&](auto gc, auto nc, int by_xcd) {
+        const int cut = bag_slabs<T>(a);
+        return with_group<VecOf<T>::N>(a->dim / cut, [&](auto gc, auto nc) {
             constexpr int G = decltype(gc)::value, N = decltype(nc)::value;
             EmbedParams p = embed_params(a);
             p.slabs = (int)ceil_div(a->dim, G * N);
-            p.by_xcd = by_xcd;
-            const i64 fours = ceil_div(a->n_rows, 4);          // bags: a workgroup takes four rows of a slab
-            const i64 blocks = !a->indptr ? ceil_div(a->n_rows * p.slabs, 256 / G) : by_xcd ? ceil_div(fours, 8 / p.slabs) * 8 : fours * p.slabs;
-            if (too_many(blocks, 256)) return fail(SP_EINVAL, "too many rows for one launch");
-            auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p); };
+            p.by_xcd = cut > 1;
+            const unsigned blocks = (unsigned)embed_blocks<T>(a, cut);
+            auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, p); };
             if (a->indptr) a->index64 ? launch(sp_embed_rows_kernel<T, i64, G, N>) : launch(sp_embed_rows_kernel<T, int, G, N>);
             else a->index64 ? launch(sp_embed_lookup_kernel<T, i64, G, N>) : launch(sp_embed_lookup_kernel<T, int, G, N>);
             HIP_TRY(hipGetLastError());
             return (int)SP_OK;
-        };
-        // by XCD: a table beyond the L2 of one from which more rows are taken than it has, and few bags
-        const i64 row_bytes = a->dim * (i64)sizeof(T);
-        const bool large = a->nnz >= a->n_vocab && a->n_vocab * row_bytes > L2_BYTES && row_bytes >= 1024;
-        const int slabs = a->indptr && (large || a->n_rows <= FEW_BAGS) && (uintptr_t)a->src % 128 == 0 ? line_slabs<T>(a->dim, a->ld_src) : 1;
-        if (slabs > 1) return with_group<VecOf<T>::N>(a->dim / slabs, [&](auto gc, auto nc) { return run(gc, nc, 1); });
-        return with_group<VecOf<T>::N>(a->dim, [&](auto gc, auto nc) { return run(gc, nc, 0); });
+        });
     });
 }
 
@@ -443,6 +461,7 @@ int sp_embed_rows(const sp_embed_args *a) {
     if (a->n_rows == 0 || a->dim == 0) return SP_OK;
     if (!a->out || (a->n_vocab > 0 && !a->src)) return fail(SP_EINVAL, "NULL table or out");
     if (a->n_rows > 1 && a->ld_out < a->dim) return fail(SP_EINVAL, "rows of out overlap");
+    TRY(check_embed_launch(a));
     OnDevice dev;
     TRY(dev.enter(a->device));
     return run_embed(a);

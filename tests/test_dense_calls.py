@@ -182,3 +182,66 @@ def test_compiled_programs():
         loss.backward()
         results.append((loss.detach(), scores, table.grad, weight.grad))
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+# ---- bags beyond the launch of the column cut ------------------------------------------------------------------------------------
+
+@gpu
+def test_bags_more_than_the_column_cut_can_launch():
+    """2^23 and more bags of a large table of rows of 1 KB: cut by columns they would need more threads than a launch has."""
+    n, vocab, dim = 2**23 + 5, 100_000, 512
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    table = torch.randn(vocab, dim, generator=gen, device="cuda").to(torch.bfloat16)
+    ids = torch.randint(0, vocab, (vocab + 1,), generator=gen, device="cuda", dtype=torch.int32)
+    at = torch.arange(vocab + 1, device="cuda") * 83                                # rows with an entry, the last one among them
+    at[-1] = n - 1
+    indptr = torch.zeros(n + 1, dtype=torch.int32, device="cuda")
+    indptr[at + 1] = 1
+    indptr = torch.cumsum(indptr, 0, dtype=torch.int32)
+    out = dense.embed_rows(table, ids, indptr)
+    assert torch.equal(out[at], table[ids.long()])                                 # bags of one entry: the row itself
+    filled = sum(int((part.view(torch.int16) != 0).any(1).sum()) for part in out.split(2**20))
+    assert filled == vocab + 1
+
+
+def embed_refusal(symbol="sp_embed_rows", **fields):
+    """What the C entry says, without a device, to a call of these sizes: "" where it would launch."""
+    import ctypes as C
+
+    from similaripy_amd import _abi
+    a = _abi.SpEmbedArgs()
+    a.struct_size = C.sizeof(a)
+    a.src = a.out = a.indices = a.workspace = 1 << 20
+    a.workspace_bytes, a.scale = 1 << 60, 1.0
+    for name, value in fields.items():
+        setattr(a, name, value)
+    rc = getattr(_abi.load(), symbol)(C.byref(a))
+    assert rc in (-1, -2)                               # refused, or no device
+    return _abi.last_error() if rc == -1 else ""
+
+
+no_device = pytest.mark.skipif(torch.cuda.is_available(), reason="the calls name memory that is not there: only without a device")
+
+
+@no_device
+@pytest.mark.parametrize("dim", [512, 1024, 4096, 8192, 768, 1792, 2304])
+def test_launch_limits_of_bags(dim):
+    """Bags of bf16 rows: a wave for every slab of 1 KB whatever the column cut of large tables would need."""
+    slabs = -(-dim // 512)
+    limit = 4 * ((2**32 - 1) // 256 // slabs)           # four bags and one slab are a workgroup of 256 threads
+    size = dict(dtype=1, out_dtype=1, n_vocab=100_000, dim=dim, ld_src=dim, ld_out=dim, nnz=200_000, indptr=1 << 20)
+    for n in (1, 8192, 8193, 2**23 - 4, 2**23 - 3, 2**23, 2**24 + 1, limit):
+        assert n > limit or embed_refusal(n_rows=n, **size) == ""
+    for n in (limit + 1, 2**27):
+        assert "too many rows" in embed_refusal(n_rows=n, **size)
+    assert embed_refusal(n_rows=2**27, **{**size, "n_vocab": 0}) == ""
+
+
+@no_device
+@pytest.mark.parametrize("dtype,dim,lanes", [(0, 3, 8), (0, 32, 8), (0, 33, 16), (1, 128, 16), (1, 512, 64), (0, 256, 64), (0, 1000, 256)])
+def test_launch_limits_of_lookups(dtype, dim, lanes):
+    """A row of a lookup has 8 .. 64 lanes for every KB of it."""
+    limit = (2**32 - 1) // 256 * 256 // lanes
+    size = dict(dtype=dtype, out_dtype=dtype, n_vocab=100_000, dim=dim, ld_src=dim, ld_out=dim)
+    assert embed_refusal(n_rows=limit, nnz=limit, **size) == ""
+    assert "too many rows" in embed_refusal(n_rows=limit + 1, nnz=limit + 1, **size)
