@@ -221,6 +221,21 @@ GradLayout grad_layout(const sp_embed_args *a) {
     return L;
 }
 
+// ids of a workgroup where nothing is sorted
+int direct_ids(const sp_embed_args *a) {
+    const i64 per = ceil_div(a->n_vocab, DIRECT_WGS);
+    return (int)(per < DIRECT_IDS ? per : DIRECT_IDS);
+}
+int check_grad_launch(const sp_embed_args *a) {
+    if (a->nnz == 0 || a->n_rows == 0) return SP_OK;
+    const int cut = a->nnz <= DIRECT_MAX ? 1 : grad_layout(a).slabs;
+    auto slabs_of = [&](auto gc, auto nc) { return ceil_div(a->dim, decltype(gc)::value * decltype(nc)::value); };
+    const i64 slabs = a->dtype == SP_DT_F32 ? with_group<4>(a->dim / cut, slabs_of) : with_group<8>(a->dim / cut, slabs_of);
+    if (a->nnz <= DIRECT_MAX && too_many(ceil_div(a->n_vocab, direct_ids(a)) * slabs, 256)) return fail(SP_EINVAL, "too many rows for one launch");
+    if (a->nnz > DIRECT_MAX && too_many(grad_layout(a).chunks * slabs, 256)) return fail(SP_EINVAL, "too many entries for one launch");
+    return SP_OK;
+}
+
 template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a) {
     hipStream_t stream = (hipStream_t)a->stream;
     FillParams fill{};
@@ -239,13 +254,11 @@ template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a)
         r.in = a->src; r.out = a->out; r.n = a->nnz; r.n_vocab = a->n_vocab; r.n_rows = a->n_rows; r.ld_in = a->ld_src; r.ld_out = a->ld_out;
         r.dim = (int)a->dim; r.accumulate = a->accumulate; r.scale = a->scale;
         d.indices = a->indices; d.indptr = a->indptr; d.data = a->data;
-        const i64 per = ceil_div(a->n_vocab, DIRECT_WGS);
-        d.per = (int)(per < DIRECT_IDS ? per : DIRECT_IDS);
+        d.per = direct_ids(a);
         return with_group<VecOf<T>::N>(a->dim, [&](auto gc, auto nc) {
             constexpr int G = decltype(gc)::value, N = decltype(nc)::value;
             r.slabs = (int)ceil_div(a->dim, G * N);
             const i64 blocks = ceil_div(a->n_vocab, d.per) * r.slabs;
-            if (too_many(blocks, 256)) return fail(SP_EINVAL, "too many rows for one launch");
             auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, d); };
             a->index64 ? launch(sp_embed_grad_direct_kernel<T, TO, i64, G, N>) : launch(sp_embed_grad_direct_kernel<T, TO, int, G, N>);
             HIP_TRY(hipGetLastError());
@@ -299,7 +312,6 @@ template <typename T, typename TO> int run_embed_grad_as(const sp_embed_args *a)
             r.slabs = (int)ceil_div(a->dim, G * N);
             r.by_xcd = L.slabs > 1;
             const i64 blocks = r.by_xcd ? ceil_div(ceil_div(L.chunks, GROUPS), 8 / r.slabs) * 8 : ceil_div(L.chunks * r.slabs, GROUPS);
-            if (too_many(L.chunks * r.slabs, 256)) return fail(SP_EINVAL, "too many entries for one launch");
             hipLaunchKernelGGL((sp_embed_reduce_kernel<T, TO, G, N>), dim3((unsigned)blocks), dim3(256), 0, stream, r);
             if (L.chunks > 1) hipLaunchKernelGGL((sp_embed_join_kernel<TO, G, N>), dim3((unsigned)(ceil_div(L.chunks - 1, GROUPS) * r.slabs)), dim3(256), 0, stream, r);
             return (int)SP_OK;
@@ -479,6 +491,7 @@ int sp_embed_rows_grad(const sp_embed_args *a) {
     if (a->n_vocab == 0 || a->dim == 0) return SP_OK;
     if (!a->out || (a->n_rows > 0 && !a->src)) return fail(SP_EINVAL, "NULL gradient or out");
     if (a->n_vocab > 1 && a->ld_out < a->dim) return fail(SP_EINVAL, "rows of out overlap");
+    TRY(check_grad_launch(a));
     TRY(check_workspace(a->workspace, a->workspace_bytes, a->nnz > 0 ? (i64)grad_layout(a).total : 0));
     OnDevice dev;
     TRY(dev.enter(a->device));

@@ -245,3 +245,16 @@ def test_launch_limits_of_lookups(dtype, dim, lanes):
     size = dict(dtype=dtype, out_dtype=dtype, n_vocab=100_000, dim=dim, ld_src=dim, ld_out=dim)
     assert embed_refusal(n_rows=limit, nnz=limit, **size) == ""
     assert "too many rows" in embed_refusal(n_rows=limit + 1, nnz=limit + 1, **size)
+
+
+@no_device
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_launch_limits_of_gradients(dtype):
+    """Refused before anything is sorted or cleared: rows so wide that the sums, or the unsorted form, have more workgroups than a launch."""
+    wide = 256 if dtype == 0 else 512                   # columns of a slab
+    size = dict(dtype=dtype, out_dtype=dtype)
+    for slabs, n, vocab, fits in ((4095, 102_400, 3, True), (4096, 102_400, 3, False), (2**14, 102_400, 3, False),          # 4096 chunks
+                                  (16, 1000, 2**31 - 2, False), (15, 1000, 2**31 - 2, True), (2**20, 5, 15, True), (2**20, 5, 16, False)):
+        dim = slabs * wide
+        said = embed_refusal("sp_embed_rows_grad", n_rows=n, nnz=n, n_vocab=vocab, dim=dim, ld_src=dim, ld_out=dim, **size)
+        assert said == "" if fits else "too many" in said, (slabs, n, vocab, said)
