@@ -51,8 +51,32 @@ def find_hipcc() -> str:
     raise RuntimeError("hipcc not found (looked at $HIPCC, /opt/rocm/bin/hipcc, PATH)")
 
 
+def _flags() -> list:
+    return [*HIPCC_FLAGS, *os.environ.get("SIMILARIPY_AMD_HIPCC_EXTRA", "").split()]      # (profiling builds only, e.g. -DSP_ABLATION=1)
+
+
+def _stamp(made: Path) -> Path:
+    """Where the command that made a file is kept."""
+    return made.with_name(made.name + ".cmd")
+
+
+def _made_by(made: Path) -> str | None:
+    try:
+        return _stamp(made).read_text()
+    except FileNotFoundError:
+        return None
+
+
+def _put(tmp: Path, made: Path, command: str) -> None:
+    """Moves a finished file into place; at no time does another command stand beside it."""
+    _stamp(made).unlink(missing_ok=True)
+    os.replace(tmp, made)
+    _stamp(made).write_text(command)
+
+
 def is_stale() -> bool:
-    if not LIB_PATH.exists():
+    """The library is missing, older than its sources or made with other flags (a library without its command counts by time alone)."""
+    if not LIB_PATH.exists() or _made_by(LIB_PATH) not in (None, " ".join(_flags())):
         return True
     t = LIB_PATH.stat().st_mtime
     return any(p.exists() and p.stat().st_mtime > t for p in SOURCES + HEADERS)
@@ -62,12 +86,16 @@ def _object(src: Path) -> Path:
     return LIB_DIR / (src.stem + ".o")
 
 
+def _command(src: Path) -> list:
+    return [find_hipcc(), *_flags(), "-I", str(INCLUDE_DIR), "-c", str(src)]
+
+
 def _compile(src: Path, verbose: bool) -> None:
     """One translation unit -> its object next to the library (written aside, then moved into place)."""
     obj = _object(src)
     tmp = obj.with_suffix(".o.tmp%d" % os.getpid())
-    extra = os.environ.get("SIMILARIPY_AMD_HIPCC_EXTRA", "").split()      # profiling builds only, e.g. -DSP_ABLATION=1
-    cmd = [find_hipcc(), *HIPCC_FLAGS, *extra, "-I", str(INCLUDE_DIR), "-c", "-o", str(tmp), str(src)]
+    made_by = " ".join(_command(src))
+    cmd = [*_command(src), "-o", str(tmp)]
     if verbose:
         print(" ".join(cmd))
     proc = subprocess.run(cmd, capture_output=True, text=True)
@@ -78,18 +106,19 @@ def _compile(src: Path, verbose: bool) -> None:
         proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError("hipcc failed:\n" + proc.stdout + proc.stderr)
-    os.replace(tmp, obj)
+    _put(tmp, obj, made_by)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the HIP library if missing or older than its sources (the units that changed; all of them with `force`). Returns its path."""
+    """Compile the HIP library if missing, older than its sources or made with other flags (the units of which that is so; all of them with
+    `force`). Returns its path."""
     if not force and not is_stale():
         return LIB_PATH
     LIB_DIR.mkdir(parents=True, exist_ok=True)
 
     def stale(src):
         obj = _object(src)
-        return force or not obj.exists() or any(p.exists() and p.stat().st_mtime > obj.stat().st_mtime for p in [src, *UNITS[src]])
+        return force or not obj.exists() or _made_by(obj) != " ".join(_command(src)) or any(p.exists() and p.stat().st_mtime > obj.stat().st_mtime for p in [src, *UNITS[src]])
     todo = [s for s in SOURCES if stale(s)]
     with ThreadPoolExecutor(max_workers=max(1, len(todo))) as pool:
         for done in [pool.submit(_compile, s, verbose) for s in todo]:
@@ -99,7 +128,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError("hipcc failed to link:\n" + proc.stdout + proc.stderr)
-    os.replace(tmp, LIB_PATH)
+    _put(tmp, LIB_PATH, " ".join(_flags()))
     return LIB_PATH
 
 
