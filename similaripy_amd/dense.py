@@ -328,9 +328,10 @@ def _pattern(name: str, csr, device, keep):
 
 
 def _per_row(name: str, v, device, n, keep):
-    """(pointer, value for all rows) of a number or one float32 per row."""
-    if isinstance(v, torch.Tensor) and v.dim() > 0:
-        v = _floats(name, v, device, n)
+    """(pointer, value for all rows) of a number or one float32 per row.  A tensor of no dimensions on a device is not read here, which would wait
+    for the device: the rows share it."""
+    if isinstance(v, torch.Tensor) and (v.dim() > 0 or v.is_cuda):
+        v = _floats(name, v, device, n) if v.dim() > 0 else v.to(device, torch.float32).expand(n).contiguous()
         keep.append(v)
         return v.data_ptr(), 0.0
     return None, float(v)
@@ -349,7 +350,8 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
     targets      [n] int32 / int64: the row of ``history``, ``filter_cols`` and ``target_cols`` each row of scores belongs to (absolute
                  row ids, as ``target_rows`` of the similarity functions); default ``0 .. n-1``.  A row outside a pattern is empty there.
     history      (indptr, indices) of a CSR pattern: ids in any order, repeats count, ids outside the columns are passed over
-    repetition, presence, frequency   a number, or one float32 per row (repetition positive)
+    repetition, presence, frequency   a number (or a tensor of no dimensions), or one float32 per row (repetition positive; tensors on a device are not
+                 checked)
     bias         [n_cols] or [n, n_cols], any of the three types
     allowed      int32 words of packed bits, [words] or [n, words] with ``words = ceil(n_cols / 32)``: column c stays where bit ``c % 32``
                  of word ``c // 32`` is set

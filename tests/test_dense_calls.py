@@ -258,3 +258,42 @@ def test_launch_limits_of_gradients(dtype):
         dim = slabs * wide
         said = embed_refusal("sp_embed_rows_grad", n_rows=n, nnz=n, n_vocab=vocab, dim=dim, ld_src=dim, ld_out=dim, **size)
         assert said == "" if fits else "too many" in said, (slabs, n, vocab, said)
+
+
+# ---- numbers -----------------------------------------------------------------------------------------------------------------------
+
+@gpu
+def test_numbers_on_the_device():
+    """A parameter of no dimensions is read by the kernel: no wait for the device, a captured call follows its value."""
+    z = torch.randn(3, 40, device="cuda")
+    h = (torch.tensor([0, 2, 3, 3], device="cuda"), torch.tensor([4, 4, 9], device="cuda"))
+    want = dense.adjust_scores(z, history=h, repetition=1.5, presence=0.25, frequency=2.0)
+    p = [torch.tensor(x, device="cuda", dtype=t) for x, t in ((1.5, torch.float32), (0.25, torch.bfloat16), (2, torch.int64))]
+    call = lambda: dense.adjust_scores(z, history=h, repetition=p[0], presence=p[1], frequency=p[2])  # noqa: E731
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        got = call()
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert torch.equal(got, want)
+    assert torch.equal(dense.adjust_scores(z, history=h, repetition=p[0].cpu(), presence=p[1].cpu(), frequency=p[2].cpu()), want)
+
+
+@gpu
+def test_numbers_on_the_device_captured():
+    z = torch.randn(3, 40, device="cuda")
+    h = (torch.tensor([0, 2, 3, 3], device="cuda"), torch.tensor([4, 4, 9], device="cuda"))
+    p = [torch.tensor(x, device="cuda") for x in (1.5, 0.25, 2.0)]
+    call = lambda: dense.adjust_scores(z, history=h, repetition=p[0], presence=p[1], frequency=p[2])  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        res = call()
+    for x in (1.25, 2.0, 3.0):
+        for t in p:
+            t.fill_(x)
+        g.replay()
+        assert torch.equal(res, dense.adjust_scores(z, history=h, repetition=x, presence=x, frequency=x))
+        torch.cuda.synchronize()
