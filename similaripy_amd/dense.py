@@ -156,6 +156,11 @@ def _fixed(name: str, t) -> None:
         raise ValueError(f"{name} has no gradient here: detach it")
 
 
+def _number(name: str, v) -> float:
+    _fixed(name, v)
+    return float(v)
+
+
 def _not_capturing(name: str, instead: str) -> None:
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{name} on tensors that require a gradient cannot be captured into a graph: capture {instead} on detached tensors")
@@ -255,7 +260,7 @@ def embed_rows(table: torch.Tensor, indices: torch.Tensor, indptr: Optional[torc
     """
     _plain(table, data, scale, out)
     _dense("table", table)
-    scale = float(scale)
+    scale = _number("scale", scale)
     if data is not None:
         _fixed("data", data)
     if out is None and table.requires_grad and torch.is_grad_enabled():
@@ -298,7 +303,7 @@ def embed_rows_grad(grad: torch.Tensor, indices: torch.Tensor, n_vocab: int, ind
     if dtype not in (grad.dtype, torch.float32):
         raise ValueError(f"the result must be {grad.dtype} or float32, got {dtype}")
     res = _out("out", out, (n_vocab, dim), dtype, grad.device, (grad, False))
-    a = _embed_args(grad, res, indices, indptr, data, n_rows, n_vocab, dim, float(scale), 1 if accumulate else 0)
+    a = _embed_args(grad, res, indices, indptr, data, n_rows, n_vocab, dim, _number("scale", scale), 1 if accumulate else 0)
     need = _abi.call_dense("sp_embed_rows_grad_workspace_bytes", a)
     if need:
         ws = torch.empty(need, dtype=torch.uint8, device=grad.device)
@@ -331,10 +336,11 @@ def _per_row(name: str, v, device, n, keep):
     """(pointer, value for all rows) of a number or one float32 per row.  A tensor of no dimensions on a device is not read here, which would wait
     for the device: the rows share it."""
     if isinstance(v, torch.Tensor) and (v.dim() > 0 or v.is_cuda):
+        _fixed(name, v)
         v = _floats(name, v, device, n) if v.dim() > 0 else v.to(device, torch.float32).expand(n).contiguous()
         keep.append(v)
         return v.data_ptr(), 0.0
-    return None, float(v)
+    return None, _number(name, v)
 
 
 def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = None, history: _Pattern = None, repetition: _PerRow = 1.0,
@@ -434,7 +440,7 @@ def _distill_args(student, cols, values, counts, temperature, teacher_lse):
             raise ValueError(f"counts must have {n} elements, got shape {tuple(counts.shape)}")
     if teacher_lse is not None:
         teacher_lse = _floats("teacher_lse", teacher_lse, device, n)
-    temperature = float(temperature)
+    temperature = _number("temperature", temperature)
     if not 1e-30 < temperature < 1e30:
         raise ValueError(f"temperature must be positive, got {temperature}")
     a = _abi.SpDistillArgs(_DISTILL_SIZE, 0, device.index, _DT[student.dtype], n, n_cols, _ld(student), 0, k, 1 if cols.dtype == torch.int64 else 0,
@@ -502,6 +508,7 @@ def distill_loss(student: torch.Tensor, cols: torch.Tensor, values: torch.Tensor
     """
     _plain(student, values, temperature, teacher_lse)
     _fixed("values", values)
+    _fixed("temperature", temperature)
     if teacher_lse is not None:
         _fixed("teacher_lse", teacher_lse)
     if isinstance(student, torch.Tensor) and student.requires_grad and torch.is_grad_enabled():

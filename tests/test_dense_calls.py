@@ -297,3 +297,25 @@ def test_numbers_on_the_device_captured():
         g.replay()
         assert torch.equal(res, dense.adjust_scores(z, history=h, repetition=x, presence=x, frequency=x))
         torch.cuda.synchronize()
+
+
+@gpu
+@pytest.mark.parametrize("device", ["cpu", "cuda"])
+def test_numbers_that_require_a_gradient(device):
+    """scale, temperature, repetition, presence and frequency have no gradient: one that asks for it is refused, not read."""
+    z = torch.randn(3, 40, device="cuda")
+    ids = torch.tensor([0, 1], device="cuda")
+    h = (torch.tensor([0, 2, 3, 3], device="cuda"), torch.tensor([4, 4, 9], device="cuda"))
+    cols, values, stats = torch.tensor([[0, 1]] * 3, device="cuda"), torch.ones(3, 2, device="cuda"), torch.ones(3, 2, device="cuda")
+    x = torch.tensor(1.5, device=device, requires_grad=True)
+    for name, call in (("scale", lambda: dense.embed_rows(z, ids, scale=x)), ("scale", lambda: dense.embed_rows_grad(z[:2], ids, 3, scale=x)),
+                       ("repetition", lambda: dense.adjust_scores(z, history=h, repetition=x)), ("presence", lambda: dense.adjust_scores(z, history=h, presence=x)),
+                       ("frequency", lambda: dense.adjust_scores(z, history=h, frequency=x)),
+                       ("temperature", lambda: dense.distill_loss(z, cols, values, temperature=x)),
+                       ("temperature", lambda: dense.distill_loss(z.clone().requires_grad_(), cols, values, temperature=x)),
+                       ("temperature", lambda: dense.distill_grad(z, stats, cols, values, temperature=x)),
+                       ("temperature", lambda: dense.distill_loss_grad(z, cols, values, temperature=x))):
+        with pytest.raises(ValueError, match=f"{name} has no gradient here"):
+            call()
+        with torch.no_grad():
+            call()
