@@ -540,7 +540,10 @@ def distill_grad(student: torch.Tensor, stats: torch.Tensor, cols: torch.Tensor,
     _plain(student, stats, values, grad_loss, temperature, teacher_lse, out)
     a, keep = _distill_args(student, cols, values, counts, temperature, teacher_lse)
     _no_grad_here("distill_grad", student)
-    stats = _floats("stats", stats, student.device, 2 * student.shape[0])
+    n = student.shape[0]
+    stats = _floats("stats", stats, student.device, 2 * n)
+    if stats.dim() != 1 and stats.shape != (n, 2):
+        raise ValueError(f"stats must have shape ({n}, 2) or ({2 * n},), got {tuple(stats.shape)}")
     grad, g = _grad_outputs(a, student, grad_loss, out)
     a.stats = stats.data_ptr()
     _abi.call_dense("sp_distill_grad", a)

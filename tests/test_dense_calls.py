@@ -319,3 +319,17 @@ def test_numbers_that_require_a_gradient(device):
             call()
         with torch.no_grad():
             call()
+
+
+@gpu
+def test_statistics_of_another_layout():
+    """Row statistics are pairs: [2, n] holds as many elements and is something else."""
+    z = torch.randn(5, 40, device="cuda")
+    cols, values = torch.tensor([[0, 1]] * 5, device="cuda"), torch.randn(5, 2, device="cuda")
+    _, stats = dense.distill_loss(z, cols, values, return_stats=True)
+    want = dense.distill_grad(z, stats, cols, values)
+    for wrong in (stats.T, stats.T.contiguous(), stats.reshape(1, 5, 2), stats[:4]):
+        with pytest.raises(ValueError, match="stats must"):
+            dense.distill_grad(z, wrong, cols, values)
+    assert torch.equal(dense.distill_grad(z, stats.reshape(-1), cols, values), want)
+    assert torch.equal(dense.distill_grad(z, torch.stack([stats, stats], 2)[:, :, 0], cols, values), want)      # strided
