@@ -117,11 +117,31 @@ def _out(name: str, out, shape, dtype, device, *inputs):
             continue
         if in_place and t.data_ptr() == out.data_ptr() and t.shape == out.shape and (shape[0] <= 1 or t.stride(0) == out.stride(0)):
             continue
-        a0, a1 = _extent(out)
-        b0, b1 = _extent(t)
-        if a0 < b1 and b0 < a1:
+        if _overlap(out, t):
             raise ValueError(f"{name} shares memory with an input")
     return out
+
+
+def _overlap(out, t) -> bool:
+    """Whether rows of `out` and of `t` share memory: columns of one store that lie beside each other do not.  (With different distances
+    between rows only what is apart altogether counts as apart.)"""
+    a0, a1 = _extent(out)
+    b0, b1 = _extent(t)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    a, b = _row_bytes(out), _row_bytes(t)
+    steps = {x.stride(0) * x.element_size() for x in (out, t) if x.dim() == 2 and x.shape[0] > 1}
+    if a is None or b is None or len(steps) != 1:
+        return True
+    step = steps.pop()
+    at = (a0 - b0) % step if step else 0
+    return at < b or at + a > step
+
+
+def _row_bytes(t):
+    """Bytes of one row, None where they are not next to each other."""
+    last = t.shape[-1]
+    return None if last > 1 and t.stride(-1) != 1 else last * t.element_size()
 
 
 def _extent(t):

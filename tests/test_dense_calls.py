@@ -333,3 +333,38 @@ def test_statistics_of_another_layout():
             dense.distill_grad(z, wrong, cols, values)
     assert torch.equal(dense.distill_grad(z, stats.reshape(-1), cols, values), want)
     assert torch.equal(dense.distill_grad(z, torch.stack([stats, stats], 2)[:, :, 0], cols, values), want)      # strided
+
+
+# ---- outputs beside inputs ---------------------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_outputs_in_the_columns_beside_their_inputs(dtype):
+    """Rows of one store: the output's columns lie beside the input's, before or behind them, one row further as well."""
+    rng = np.random.default_rng(0)
+    n, v = 6, 37
+    store = torch.from_numpy(rng.standard_normal((n + 1, 3 * v))).to(dtype).cuda()
+    keep = store.clone()
+    bias = torch.from_numpy(rng.standard_normal(v)).to(dtype).cuda()
+    cols, values = torch.tensor([[1, 5]] * n, device="cuda"), torch.randn(n, 2, device="cuda")
+    ids = torch.arange(n, device="cuda")
+    src = store[:n, v:2 * v]
+    for out in (store[:n, :v], store[:n, 2 * v:], store[1:, :v], store[1:, 2 * v:]):
+        assert torch.equal(dense.adjust_scores(src, bias=bias, out=out), dense.adjust_scores(src.clone(), bias=bias))
+        assert torch.equal(dense.distill_loss_grad(src, cols, values, out=out)[1], dense.distill_loss_grad(src.clone(), cols, values)[1])
+        assert torch.equal(dense.embed_rows(src, ids, out=out), src)
+        assert torch.equal(dense.embed_rows_grad(src, ids, n, out=out), src)
+        assert torch.equal(src, keep[:n, v:2 * v])
+    one = store[2:3, :v]                                                           # one row between the rows of the other
+    assert torch.equal(dense.embed_rows(src, ids[3:4], out=one), src[3:4])
+    assert torch.equal(dense.adjust_scores(store[2:3, v:2 * v], bias=store[2, :v]), dense.adjust_scores(src[2:3].clone(), bias=store[2, :v].clone()))
+    for out in (store[:n, 1:v + 1], store[:n, 2 * v - 1:3 * v - 1], store[1:, v:2 * v], store[1:, v + 1:2 * v + 1], store[n - 1:n, v - 1:2 * v - 1]):
+        with pytest.raises(ValueError, match="shares memory"):
+            if out.shape[0] == 1:
+                dense.embed_rows(src, ids[:1], out=out)
+            else:
+                dense.adjust_scores(src, out=out)
+    wide = torch.zeros(4 * n, v, dtype=dtype, device="cuda")                       # other distances between rows: only apart altogether
+    with pytest.raises(ValueError, match="shares memory"):
+        dense.adjust_scores(wide[:2 * n:2], out=wide[1:n + 1])
+    dense.adjust_scores(wide[:2 * n:2], out=wide[2 * n:3 * n])
