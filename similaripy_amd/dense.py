@@ -99,9 +99,9 @@ def _ld(t) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _out(name: str, out, shape, dtype, device, *inputs):
-    """The caller's output, or a new one.  An output may be one of the ``inputs`` marked as such (same start, same rows), else it
-    must not share memory with any of them."""
+def _out(name: str, out, shape, dtype, device, operands, in_place=None):
+    """The caller's output, or a new one.  It may be `in_place` (same start, same rows), and shares memory with no other operand: the kernels
+    read lists, weights and statistics while they write."""
     if out is None:
         return torch.empty(shape, dtype=dtype, device=device)
     _dense(name, out)
@@ -112,12 +112,12 @@ def _out(name: str, out, shape, dtype, device, *inputs):
         raise ValueError(f"{name} must not require a gradient")
     if shape[0] > 1 and out.stride(0) < shape[1]:
         raise ValueError(f"the rows of {name} overlap")
-    for t, in_place in inputs:
-        if t is None or not t.numel() or not out.numel():
-            continue
-        if in_place and t.data_ptr() == out.data_ptr() and t.shape == out.shape and (shape[0] <= 1 or t.stride(0) == out.stride(0)):
-            continue
-        if _overlap(out, t):
+    if not out.numel():
+        return out
+    if in_place is not None and not (in_place.data_ptr() == out.data_ptr() and (shape[0] <= 1 or in_place.stride(0) == out.stride(0))):
+        operands = (in_place, *operands)
+    for t in operands:
+        if t is not None and t.numel() and _overlap(out, t):
             raise ValueError(f"{name} shares memory with an input")
     return out
 
@@ -139,9 +139,9 @@ def _overlap(out, t) -> bool:
 
 
 def _row_bytes(t):
-    """Bytes of one row, None where they are not next to each other."""
-    last = t.shape[-1]
-    return None if last > 1 and t.stride(-1) != 1 else last * t.element_size()
+    """Bytes of one row of a matrix, or of all of a vector; None where they are not next to each other."""
+    last = t.shape[-1] if t.dim() else 1
+    return None if t.dim() > 2 or last > 1 and t.stride(-1) != 1 else last * t.element_size()
 
 
 def _extent(t):
@@ -241,7 +241,7 @@ def _embed_forward(table, indices, indptr, data, scale, out):
     if out is not None and tuple(out.shape) != lead + (dim,):
         raise ValueError(f"out must have shape {lead + (dim,)}, got {tuple(out.shape)}")
     flat = None if out is None else out.view(n_rows, dim) if out.dim() != 2 else out
-    res = _out("out", flat, (n_rows, dim), table.dtype, table.device, (table, False))
+    res = _out("out", flat, (n_rows, dim), table.dtype, table.device, (table, indices, indptr, data))
     _abi.call_dense("sp_embed_rows", _embed_args(table, res, indices, indptr, data, n_rows, table.shape[0], dim, scale))
     _written(out)
     return out if out is not None else res if len(lead) == 1 else res.view(lead + (dim,))
@@ -322,7 +322,7 @@ def embed_rows_grad(grad: torch.Tensor, indices: torch.Tensor, n_vocab: int, ind
     dtype = dtype or (grad.dtype if out is None else out.dtype)
     if dtype not in (grad.dtype, torch.float32):
         raise ValueError(f"the result must be {grad.dtype} or float32, got {dtype}")
-    res = _out("out", out, (n_vocab, dim), dtype, grad.device, (grad, False))
+    res = _out("out", out, (n_vocab, dim), dtype, grad.device, (grad, indices, indptr, data))
     a = _embed_args(grad, res, indices, indptr, data, n_rows, n_vocab, dim, _number("scale", scale), 1 if accumulate else 0)
     need = _abi.call_dense("sp_embed_rows_grad_workspace_bytes", a)
     if need:
@@ -396,6 +396,7 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
         targets = _ints("targets", targets, device)
         if targets.dim() != 1 or targets.numel() != n:
             raise ValueError(f"targets must have {n} elements, got shape {tuple(targets.shape)}")
+        keep.append(targets)
         tptr, t64 = targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0
     h = _pattern("history", history, device, keep)
     f = _pattern("filter_cols", filter_cols, device, keep)
@@ -424,7 +425,7 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
             raise ValueError(f"allowed must have shape {(words,)} or {(n, words)}, got {tuple(allowed.shape)}")
         keep.append(allowed)
         aptr, lda = allowed.data_ptr(), 0 if allowed.dim() == 1 else words
-    res = _out("out", out, (n, n_cols), scores.dtype, device, (scores, True), (bias, False))
+    res = _out("out", out, (n, n_cols), scores.dtype, device, keep, scores)
     a = _abi.SpAdjustArgs(_ADJUST_SIZE, 0, device.index, _DT[scores.dtype], n, n_cols, _ld(scores), _ld(res), scores.data_ptr(), res.data_ptr(), tptr, t64, bdt,
                           h, f, t, rep, pres, freq, rep_all, pres_all, freq_all, 0, bptr, ldb, aptr, lda, _stream(device))
     _abi.call_dense("sp_adjust_scores", a)
@@ -539,11 +540,11 @@ def distill_loss(student: torch.Tensor, cols: torch.Tensor, values: torch.Tensor
     return (loss, stats) if return_stats else loss
 
 
-def _grad_outputs(a, student, grad_loss, out):
+def _grad_outputs(a, student, grad_loss, out, operands):
     n = student.shape[0]
     if grad_loss is not None:
         grad_loss = _floats("grad_loss", grad_loss, student.device, n)
-    grad = _out("out", out, tuple(student.shape), student.dtype, student.device, (student, True))
+    grad = _out("out", out, tuple(student.shape), student.dtype, student.device, (grad_loss, *operands), student)
     a.grad_loss, a.grad, a.ld_grad = None if grad_loss is None else grad_loss.data_ptr(), grad.data_ptr(), _ld(grad)
     return grad, grad_loss
 
@@ -564,7 +565,7 @@ def distill_grad(student: torch.Tensor, stats: torch.Tensor, cols: torch.Tensor,
     stats = _floats("stats", stats, student.device, 2 * n)
     if stats.dim() != 1 and stats.shape != (n, 2):
         raise ValueError(f"stats must have shape ({n}, 2) or ({2 * n},), got {tuple(stats.shape)}")
-    grad, g = _grad_outputs(a, student, grad_loss, out)
+    grad, g = _grad_outputs(a, student, grad_loss, out, (stats, *keep))
     a.stats = stats.data_ptr()
     _abi.call_dense("sp_distill_grad", a)
     _written(out)
@@ -581,7 +582,7 @@ def distill_loss_grad(student: torch.Tensor, cols: torch.Tensor, values: torch.T
     a, keep = _distill_args(student, cols, values, counts, temperature, teacher_lse)
     _no_grad_here("distill_loss_grad", student)
     loss = torch.empty(student.shape[0], dtype=torch.float32, device=student.device)
-    grad, g = _grad_outputs(a, student, grad_loss, out)
+    grad, g = _grad_outputs(a, student, grad_loss, out, keep)
     a.loss = loss.data_ptr()
     ws = _workspace(a, student.device)
     _abi.call_dense("sp_distill_loss_grad", a)

@@ -368,3 +368,33 @@ def test_outputs_in_the_columns_beside_their_inputs(dtype):
     with pytest.raises(ValueError, match="shares memory"):
         dense.adjust_scores(wide[:2 * n:2], out=wide[1:n + 1])
     dense.adjust_scores(wide[:2 * n:2], out=wide[2 * n:3 * n])
+
+
+@gpu
+def test_outputs_over_any_operand_are_refused():
+    """Kernels read lists, weights and statistics while they write: an output over any of them is refused."""
+    n, v = 4, 64
+    raw = torch.zeros(4096, dtype=torch.float32, device="cuda")
+    out = raw[:n * v].view(n, v)
+    over = lambda numel, dtype=torch.float32: raw[100:100 + numel * (2 if dtype == torch.int64 else 1)].view(dtype)  # noqa: E731
+    z, ids, ptr = torch.randn(n, v, device="cuda"), torch.tensor([0, 1, 2, 3], device="cuda"), torch.tensor([0, 1, 2, 3, 4], device="cuda")
+    cols, values = torch.zeros(n, 2, dtype=torch.int64, device="cuda"), torch.ones(n, 2, device="cuda")
+    stats = torch.ones(n, 2, device="cuda")
+    i64 = torch.int64
+    pattern = (ptr, ids)
+    for call in (
+        lambda: dense.embed_rows(z, over(4, i64), out=out), lambda: dense.embed_rows(z, ids, over(5, i64), out=out), lambda: dense.embed_rows(z, ids, ptr, over(4), out=out),
+        lambda: dense.embed_rows_grad(z, over(4, i64), n, out=out), lambda: dense.embed_rows_grad(z, ids, n, over(5, i64), out=out),
+        lambda: dense.embed_rows_grad(z, ids, n, ptr, over(4), out=out),
+        lambda: dense.adjust_scores(z, targets=over(4, i64), out=out), lambda: dense.adjust_scores(z, allowed=over(2, torch.int32), out=out),
+        lambda: dense.adjust_scores(z, filter_cols=(over(5, i64), ids), out=out), lambda: dense.adjust_scores(z, target_cols=(ptr, over(4, i64)), out=out),
+        lambda: dense.adjust_scores(z, history=(ptr, over(4, i64)), out=out), lambda: dense.adjust_scores(z, history=pattern, repetition=over(4), out=out),
+        lambda: dense.adjust_scores(z, history=pattern, presence=over(4), out=out), lambda: dense.adjust_scores(z, history=pattern, frequency=over(4), out=out),
+        lambda: dense.distill_grad(z, over(8).view(n, 2), cols, values, out=out), lambda: dense.distill_grad(z, stats, over(8, i64), values, out=out),
+        lambda: dense.distill_grad(z, stats, cols, over(8), out=out), lambda: dense.distill_grad(z, stats, cols, values, over(4, torch.int32), out=out),
+        lambda: dense.distill_grad(z, stats, cols, values, grad_loss=over(4), out=out), lambda: dense.distill_grad(z, stats, cols, values, teacher_lse=over(4), out=out),
+        lambda: dense.distill_loss_grad(z, over(8, i64), values, out=out), lambda: dense.distill_loss_grad(z, cols, over(8), out=out),
+        lambda: dense.distill_loss_grad(z, cols, values, over(4, torch.int32), out=out), lambda: dense.distill_loss_grad(z, cols, values, grad_loss=over(4), out=out),
+    ):
+        with pytest.raises(ValueError, match="out shares memory"):
+            call()
