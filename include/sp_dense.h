@@ -100,7 +100,7 @@ typedef struct sp_adjust_args {
     sp_csr_pattern history;    /* ids whose scores are penalised; the count of a column is how often its row lists it */
     sp_csr_pattern filter;     /* listed columns become -inf */
     sp_csr_pattern target;     /* columns that are NOT listed become -inf */
-    const float *repetition;   /* [n_rows] or NULL: all rows repetition_all */
+    const float *repetition;   /* [n_rows] or NULL: all rows repetition_all (> 0 where a history is given) */
     const float *presence;     /* [n_rows] or NULL: presence_all */
     const float *frequency;    /* [n_rows] or NULL: frequency_all */
     float    repetition_all, presence_all, frequency_all;

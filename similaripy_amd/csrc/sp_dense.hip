@@ -513,6 +513,9 @@ int sp_adjust_scores(const sp_adjust_args *a) {
     if (a->n_rows == 0 || a->n_cols == 0) return SP_OK;
     if (!a->scores || !a->out) return fail(SP_EINVAL, "NULL scores or out");
     if (a->n_rows > 1 && a->ld_out < a->n_cols) return fail(SP_EINVAL, "rows of out overlap");
+    // a history without any penalty changes nothing
+    const bool counts = a->history.indptr && (a->repetition || a->presence || a->frequency || a->repetition_all != 1.f || a->presence_all != 0.f || a->frequency_all != 0.f);
+    if (counts && !a->repetition && !(a->repetition_all > 0.f)) return fail(SP_EINVAL, "repetition_all must be positive");
     OnDevice dev;
     TRY(dev.enter(a->device));
     AdjustParams p{};
@@ -522,8 +525,6 @@ int sp_adjust_scores(const sp_adjust_args *a) {
     p.repetition = a->repetition; p.presence = a->presence; p.frequency = a->frequency;
     p.repetition_all = a->repetition_all; p.presence_all = a->presence_all; p.frequency_all = a->frequency_all;
     p.bias = a->bias; p.ld_bias = a->ld_bias; p.allowed = a->allowed; p.ld_allowed = a->ld_allowed;
-    // a history without any penalty changes nothing
-    const bool counts = a->history.indptr && (a->repetition || a->presence || a->frequency || a->repetition_all != 1.f || a->presence_all != 0.f || a->frequency_all != 0.f);
     return with_type(a->dtype, [&](auto tag) {
         using T = decltype(tag);
         return launch_adjust<T>(p, counts, (hipStream_t)a->stream);

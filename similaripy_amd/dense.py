@@ -402,7 +402,7 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
     f = _pattern("filter_cols", filter_cols, device, keep)
     t = _pattern("target_cols", target_cols, device, keep)
     rep, rep_all = _per_row("repetition", repetition, device, n, keep)
-    if rep is None and not rep_all > 0.0:
+    if rep is None and not rep_all >= 2.0 ** -149:      # (float32's smallest: what is below becomes 0)
         raise ValueError(f"repetition must be positive, got {repetition}")
     pres, pres_all = _per_row("presence", presence, device, n, keep)
     freq, freq_all = _per_row("frequency", frequency, device, n, keep)

@@ -398,3 +398,32 @@ def test_outputs_over_any_operand_are_refused():
     ):
         with pytest.raises(ValueError, match="out shares memory"):
             call()
+
+
+# ---- numbers at the ends of float32 --------------------------------------------------------------------------------------------
+
+@gpu
+def test_repetition_that_is_0_in_float32():
+    z = torch.ones(1, 4, device="cuda")
+    h = (torch.tensor([0, 1], device="cuda"), torch.tensor([2], device="cuda"))
+    with pytest.raises(ValueError, match="repetition must be positive"):
+        dense.adjust_scores(z, history=h, repetition=1e-46)
+    assert dense.adjust_scores(z, history=h, repetition=2.0 ** -100)[0, 2].item() == 2.0 ** 100
+
+
+def test_c_repetition_must_be_positive():
+    """A history with a penalty but repetition_all left at 0 divides by 0."""
+    import ctypes as C
+
+    from similaripy_amd import _abi
+    a = _abi.SpAdjustArgs()
+    a.struct_size = C.sizeof(a)
+    a.n_rows, a.n_cols, a.ld_scores, a.ld_out, a.device = 1, 4, 4, 4, 1 << 20      # (no such device: nothing is launched)
+    a.scores = a.out = a.history.indptr = a.history.indices = 64
+    a.history.n_rows = a.history.nnz = 1
+    a.presence_all = 1.0
+    for r in (0.0, -1.0, math.nan):
+        a.repetition_all = r
+        assert _abi.load().sp_adjust_scores(C.byref(a)) == -1 and "repetition" in _abi.last_error()
+    a.repetition_all = 1.0
+    assert _abi.load().sp_adjust_scores(C.byref(a)) < 0 and "repetition" not in _abi.last_error()
