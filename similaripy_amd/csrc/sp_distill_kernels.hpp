@@ -233,7 +233,7 @@ __device__ __forceinline__ float list_loss(const DistillParams &p, ListSums l, M
     float cross = 0.f;
     for (int j = threadIdx.x & 63; j < p.k; j += 64)
         if (list.prob[j] != 0.f) cross += list.prob[j] * (list.z[j] == NEG_INF ? NEG_INF : __fmaf_rn(list.z[j] - high, p.inv_tau, -logs));
-    return p.tau * p.tau * (l.plogp - wave_sum(cross));
+    return p.tau * (p.tau * (l.plogp - wave_sum(cross)));      // (tau^2 alone may leave float32: 0 * inf for an empty list)
 }
 // The chains, by the wave that has made the list: column c of [c0, c1) is in the chain of the thread that writes it with the row, vector by
 // vector ((c - c0) / N) % NT, from column `tail` on one by one.  (What a thread writes twice ends as the later of its two stores: no barrier

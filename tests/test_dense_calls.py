@@ -427,3 +427,22 @@ def test_c_repetition_must_be_positive():
         assert _abi.load().sp_adjust_scores(C.byref(a)) == -1 and "repetition" in _abi.last_error()
     a.repetition_all = 1.0
     assert _abi.load().sp_adjust_scores(C.byref(a)) < 0 and "repetition" not in _abi.last_error()
+
+
+@gpu
+@pytest.mark.parametrize("tau", [1e-25, 1e-21, 1e19, 1e21, 1e25])
+def test_distill_temperatures_whose_square_leaves_float32(tau):
+    """tau^2 is 0 or inf there, the loss is not: it is near tau (max - score) for small tau, and 0 of an empty list or for p = q."""
+    z = torch.tensor([[3.0, 1.0, -2.0, 0.5], [1.0, 2.0, 4.0, 8.0]], device="cuda")
+    cols, values = torch.tensor([[1, 2], [0, 1]], device="cuda"), torch.tensor([[5.0, 1.0], [1.0, 3.0]], device="cuda")
+    counts = torch.tensor([2, 0], dtype=torch.int32, device="cuda")
+    loss, stats = dense.distill_loss(z, cols, values, counts, temperature=tau, return_stats=True)
+    one, grad = dense.distill_loss_grad(z, cols, values, counts, temperature=tau)
+    assert torch.equal(loss, one) and loss[1].item() == 0.0 and (grad[1] == 0).all()
+    if tau < 1:                                         # p is 1 at the list's best (column 1), q at the row's best
+        assert abs(loss[0].item() - np.float32(tau) * 2.0) <= 1e-5 * tau
+        assert (grad[0].double().cpu() - tau * torch.tensor([1.0, -1.0, 0.0, 0.0])).abs().max() <= 1e-6 * tau
+    else:                                               # p is 1/2 twice, q 1/4: tau^2 log 2
+        want = float(tau) ** 2 * math.log(2.0)
+        assert loss[0].item() == math.inf if want > 3.5e38 else abs(loss[0].item() - want) <= 1e-5 * want
+        assert (grad[0].double().cpu() / tau - torch.tensor([0.25, -0.25, -0.25, 0.25])).abs().max() <= 1e-6
