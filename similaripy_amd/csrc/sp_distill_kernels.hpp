@@ -215,7 +215,8 @@ template <typename T> __device__ __forceinline__ ListSums list_sums(const Distil
     for (int j = lane; j < p.k; j += 64) {
         float prob = 0.f;
         if (list.col[j] >= 0) {
-            const float logp = top == NEG_INF ? NEG_INF : __fmaf_rn(list.prob[j] - top, p.inv_tau, shift);
+            // (a value of -inf has no mass, also where all of the teacher's are -inf and teacher_lse with them)
+            const float logp = top == NEG_INF || list.prob[j] == NEG_INF ? NEG_INF : __fmaf_rn(list.prob[j] - top, p.inv_tau, shift);
             prob = exp2_fast(logp * LOG2E);
             r.mass += prob;
             if (prob != 0.f) r.plogp += prob * logp;

@@ -446,3 +446,19 @@ def test_distill_temperatures_whose_square_leaves_float32(tau):
         want = float(tau) ** 2 * math.log(2.0)
         assert loss[0].item() == math.inf if want > 3.5e38 else abs(loss[0].item() - want) <= 1e-5 * want
         assert (grad[0].double().cpu() / tau - torch.tensor([0.25, -0.25, -0.25, 0.25])).abs().max() <= 1e-6
+
+
+@gpu
+@pytest.mark.parametrize("n", [3, 300])
+def test_distill_teacher_without_mass(n):
+    """A teacher whose scores are all -inf has a log-sum-exp of -inf too: its list has no mass, loss and gradient are 0."""
+    z = torch.randn(n, 40, device="cuda")
+    cols, values = torch.tensor([[3, 7]] * n, device="cuda"), torch.ones(n, 2, device="cuda")
+    lse = torch.full((n,), 2.0, device="cuda")
+    values[1], lse[1] = -math.inf, -math.inf
+    values[2, 0] = -math.inf
+    loss, stats = dense.distill_loss(z, cols, values, teacher_lse=lse, return_stats=True)
+    two = dense.distill_grad(z, stats, cols, values, teacher_lse=lse)
+    one, grad = dense.distill_loss_grad(z, cols, values, teacher_lse=lse)
+    assert torch.equal(one, loss) and loss[1].item() == 0.0 and (grad[1] == 0).all() and (two[1] == 0).all()
+    assert loss.isfinite().all() and grad.isfinite().all() and grad[2, 7].item() < 0 < grad[2, 3].item()
