@@ -462,3 +462,71 @@ def test_distill_teacher_without_mass(n):
     one, grad = dense.distill_loss_grad(z, cols, values, teacher_lse=lse)
     assert torch.equal(one, loss) and loss[1].item() == 0.0 and (grad[1] == 0).all() and (two[1] == 0).all()
     assert loss.isfinite().all() and grad.isfinite().all() and grad[2, 7].item() < 0 < grad[2, 3].item()
+
+
+# ---- refusals, each for its own reason -----------------------------------------------------------------------------------------
+
+def refusals():
+    """(call, exception, fragment of its message): every operand made for its call."""
+    def Z(*shape, **kw):
+        return torch.zeros(*(shape or (4, 6)), device="cuda", **kw)
+
+    def I(*values, dtype=torch.int64):  # noqa: E743
+        return torch.tensor(values, dtype=dtype, device="cuda")
+    ids, i32 = I(0, 0, 0), I(0, 0, 0, 0, dtype=torch.int32)
+    cols, vals = torch.zeros(4, 2, dtype=torch.int32, device="cuda"), Z(4, 2)
+    leaf = lambda *shape: Z(*shape).requires_grad_()  # noqa: E731
+    E, G, A, L = dense.embed_rows, dense.embed_rows_grad, dense.adjust_scores, dense.distill_loss
+    D, B = dense.distill_grad, dense.distill_loss_grad
+    return [
+        (lambda: E(Z().T, ids), ValueError, "table must have contiguous rows"), (lambda: E(Z(4), ids), ValueError, r"table must have 2 dimension"),
+        (lambda: E([1], ids), TypeError, "table must be a torch.Tensor"), (lambda: E(Z().double(), ids), TypeError, "table must be float32, bfloat16 or float16"),
+        (lambda: E(Z(), ids.float()), TypeError, "indices must be int32 or int64"), (lambda: E(Z(), [0]), TypeError, "indices must be a torch.Tensor"),
+        (lambda: E(Z(), ids.cpu()), ValueError, "indices is on cpu"), (lambda: E(Z(), ids, i32), TypeError, "indptr must be int64"),
+        (lambda: E(Z(), ids, None, Z(3)), ValueError, "data needs indptr"), (lambda: E(Z(), ids, I(0, 3), Z(2)), ValueError, "data must have 3 elements"),
+        (lambda: E(Z(), ids, I(0, 3), Z(3).double()), TypeError, "data must be float32"), (lambda: E(Z(), ids, I(0, 3), leaf(3)), ValueError, "data has no gradient here"),
+        (lambda: E(leaf(), ids, I(0, 3), leaf(3)), ValueError, "data has no gradient here"), (lambda: E(Z(), ids.reshape(3, 1), I(0, 3)), ValueError, "indices must have 1 dimension"),
+        (lambda: E(Z(), ids, ids[:0]), ValueError, "indptr must have 1 dimension and at least one element"),
+        (lambda: E(Z(), ids, out=[1]), TypeError, "out must be a torch.Tensor"), (lambda: E(Z(), ids, out=Z(3, 5)), ValueError, r"out must have shape \(3, 6\)"),
+        (lambda: E(Z(), ids, out=Z(3, 6).half()), ValueError, "out must be torch.float32"), (lambda: (lambda t: E(t, ids, out=t[:3]))(Z()), ValueError, "shares memory"),
+        (lambda: E(leaf(), ids, out=Z(3, 6)), ValueError, "builds no autograd graph"), (lambda: E(Z(), ids, out=leaf(3, 6)), ValueError, "out must not require a gradient"),
+        (lambda: G([1], ids, 5), TypeError, "grad must be a torch.Tensor"), (lambda: G(Z(), ids, 5), ValueError, "grad has 4 rows, the indices make 3"),
+        (lambda: G(Z(3, 6), ids, -1), ValueError, "n_vocab must not be negative"), (lambda: G(Z(3, 6), ids, 5, accumulate=True), ValueError, "accumulate needs out"),
+        (lambda: G(Z(3, 6), ids, 5, dtype=torch.float16), ValueError, "the result must be torch.float32 or float32"),
+        (lambda: G(leaf(3, 6), ids, 5), ValueError, "builds no autograd graph"), (lambda: G(Z(3, 6), ids, 5, out=Z(1, 6).expand(5, 6)), ValueError, "rows of out overlap"),
+        (lambda: (lambda t: G(t[:3], ids, 4, out=t))(Z()), ValueError, "shares memory"),
+        (lambda: A([1]), TypeError, "scores must be a torch.Tensor"), (lambda: A(leaf()), ValueError, "adjust_scores builds no autograd graph"),
+        (lambda: A(Z(), targets=ids), ValueError, "targets must have 4 elements"), (lambda: A(Z(), targets=ids.float()), TypeError, "targets must be int32 or int64"),
+        (lambda: A(Z(), history=i32), TypeError, r"history must be a pair \(indptr, indices\)"), (lambda: A(Z(), history=(i32, ids)), TypeError, "history must be int64"),
+        (lambda: A(Z(), filter_cols=(ids[:0], ids)), ValueError, "filter_cols: indptr and indices"),
+        (lambda: A(Z(), target_cols=(ids, ids.reshape(3, 1))), ValueError, "target_cols: indptr and indices"),
+        (lambda: A(Z(), repetition=0.0), ValueError, "repetition must be positive"), (lambda: A(Z(), repetition=torch.tensor(0.0)), ValueError, "repetition must be positive"),
+        (lambda: A(Z(), repetition=math.nan), ValueError, "repetition must be positive"), (lambda: A(Z(), repetition=Z(3)), ValueError, "repetition must have 4 elements"),
+        (lambda: A(Z(), presence=Z(4).double()), TypeError, "presence must be float32"), (lambda: A(Z(), frequency=leaf(4)), ValueError, "frequency has no gradient here"),
+        (lambda: A(Z(), bias=Z(5)), ValueError, r"bias must have shape \(6,\) or \(4, 6\)"), (lambda: A(Z(), bias=leaf(6)), ValueError, "builds no autograd graph"),
+        (lambda: A(Z(), bias=Z(6, 4).T), ValueError, "bias must have contiguous rows"), (lambda: A(Z(), bias=Z(6).cpu()), ValueError, "bias must be on a HIP device"),
+        (lambda: A(Z(), allowed=i32[:2]), ValueError, r"allowed must have shape \(1,\) or \(4, 1\)"), (lambda: A(Z(), allowed=ids[:1]), TypeError, "allowed must be int32"),
+        (lambda: (lambda t: A(t[:3], out=t[1:]))(Z()), ValueError, "shares memory"), (lambda: A(Z(), out=Z(4, 7)), ValueError, r"out must be torch.float32 of shape \(4, 6\)"),
+        (lambda: L([1], cols, vals), TypeError, "student must be a torch.Tensor"), (lambda: L(Z(), cols[:3], vals), ValueError, "cols must hold the same number of slots"),
+        (lambda: L(Z(), cols.T, vals), ValueError, r"cols must have shape \(4, k\)"), (lambda: L(Z(), cols.float(), vals), TypeError, "cols must be int32 or int64"),
+        (lambda: L(Z(), cols, vals[:3]), ValueError, r"values must have shape \(4, 2\)"), (lambda: L(Z(), cols, vals.T), ValueError, r"values must have shape \(4, 2\)"),
+        (lambda: L(Z(), cols, vals.double()), TypeError, "values must be float32, bfloat16 or float16"), (lambda: L(Z(), cols, [1]), TypeError, "values must be a torch.Tensor"),
+        (lambda: L(Z(), cols, vals.cpu()), ValueError, "values is on cpu"), (lambda: L(Z(), cols, leaf(4, 2)), ValueError, "values has no gradient here"),
+        (lambda: L(leaf(), cols, leaf(4, 2)), ValueError, "values has no gradient here"), (lambda: L(Z(), cols, vals, ids), TypeError, "counts must be int32"),
+        (lambda: L(Z(), cols, vals, i32[:3]), ValueError, "counts must have 4 elements"), (lambda: L(Z(), cols, vals, teacher_lse=Z(3)), ValueError, "teacher_lse must have 4 elements"),
+        (lambda: L(leaf(), cols, vals, teacher_lse=leaf(4)), ValueError, "teacher_lse has no gradient here"),
+        *((lambda t=t: L(Z(), cols, vals, temperature=t), ValueError, "temperature must be positive") for t in (0.0, -1.0, math.nan, math.inf)),
+        (lambda: L(Z(), torch.zeros(4, 4097, dtype=torch.int32, device="cuda"), Z(4, 4097)), ValueError, "at most 4096"),
+        (lambda: D(Z(), Z(4), cols, vals), ValueError, "stats must have 8 elements"), (lambda: D(leaf(), Z(4, 2), cols, vals), ValueError, "distill_grad builds no autograd graph"),
+        (lambda: D(Z(), Z(4, 2), cols, vals, out=Z(4, 5)), ValueError, "out must be torch.float32 of shape"), (lambda: D(Z(), Z(4, 2).half(), cols, vals), TypeError, "stats must be float32"),
+        (lambda: B(leaf(), cols, vals), ValueError, "distill_loss_grad builds no autograd graph"), (lambda: B(Z(), cols, vals, grad_loss=Z(3)), ValueError, "grad_loss must have 4 elements"),
+        (lambda: B(Z(), cols, vals, out=Z(1, 6).expand(4, 6)), ValueError, "rows of out overlap"),
+    ]
+
+
+@gpu
+def test_refusals_say_why():
+    for i, (call, exception, message) in enumerate(refusals()):
+        with pytest.raises(exception, match=message):
+            call()
+            raise AssertionError(f"call {i} went through: {message}")
