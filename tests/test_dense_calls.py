@@ -530,3 +530,60 @@ def test_refusals_say_why():
         with pytest.raises(exception, match=message):
             call()
             raise AssertionError(f"call {i} went through: {message}")
+
+
+# ---- score adjustment: histories at the limits of a segment's table and tiles -----------------------------------------------------
+
+def long_history(rng, cols, distinct, entries, popular=0):
+    """Ids of `distinct` of the columns, each at least once; one of them (and the column beside it) `popular` times more."""
+    listed = rng.permutation(cols)[:distinct]
+    more = entries - distinct - popular
+    ids = np.concatenate([listed, np.full(popular, listed[0]), rng.choice(listed, more)])
+    return rng.permutation(ids), np.bincount(ids, minlength=cols)
+
+
+@gpu
+@pytest.mark.parametrize("distinct,entries,popular", [(1024, 1024, 0), (1024, 1025, 1), (1024, 4000, 0), (1025, 1025, 0), (1025, 4000, 0), (1023, 70_000, 60_000),
+                                                      (1025, 65_535, 64_510), (1025, 65_536, 64_511), (1500, 65_535, 60_000), (2048, 65_535, 0), (1500, 200_000, 150_000)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_adjust_limits_of_the_table(dtype, distinct, entries, popular):
+    """Rows of one segment of 2048 columns: as many distinct ids as the table takes and one more, histories that 16 bits count and one entry more,
+    with a column that has nearly all of them between columns that have few."""
+    rng = np.random.default_rng(distinct + entries)
+    ids, count = long_history(rng, 2048, distinct, entries, popular)
+    if popular:                                         # both halves of a word are counted
+        a = ids[np.argmax(np.bincount(ids)[ids])]
+        assert count[a] > popular
+    count = torch.from_numpy(count)
+    history = (torch.tensor([0, 0, entries], dtype=torch.int32, device="cuda"), torch.from_numpy(ids.astype(np.int32)).cuda())
+    scores = torch.zeros(2, 2048, dtype=dtype, device="cuda")
+    want = torch.stack([torch.zeros(2048), -count.float() / 16]).to(dtype)          # counts below 2^24: exact until the one rounding
+    got = dense.adjust_scores(scores, history=history, frequency=1 / 16)
+    assert torch.equal(got.cpu(), want)
+    assert torch.equal(dense.adjust_scores(scores, history=history, frequency=1 / 16, out=scores), got)
+
+
+@gpu
+@pytest.mark.parametrize("cols", [16_384, 40_001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_adjust_tiles_of_wide_segments(dtype, cols):
+    """Rows enough for segments of 14 336 and 16 384 columns: counts in two tiles of 16 bits and four of 32, in rows beside rows without a history."""
+    rng = np.random.default_rng(cols)
+    n = 2048
+    kinds = [long_history(rng, cols, d, e, p) for d, e, p in ((cols * 5 // 16, 30_000, 0), (cols * 5 // 16, 65_535, 50_000), (cols * 5 // 16, 65_536, 50_000),
+                                                             (cols, 300_000, 100_000), (700, 900, 0))]
+    indptr = torch.from_numpy(np.cumsum([0] + [len(k[0]) for k in kinds])).to(torch.int32).cuda()
+    history = (indptr, torch.from_numpy(np.concatenate([k[0] for k in kinds]).astype(np.int32)).cuda())
+    targets = torch.full((n,), -1, dtype=torch.int32)
+    at = torch.from_numpy(rng.permutation(n)[:40])
+    targets[at] = torch.arange(40, dtype=torch.int32) % 5
+    scores = torch.full((n, cols), 1.0, dtype=dtype, device="cuda")
+    counts = torch.from_numpy(np.stack([k[1] for k in kinds])).float().cuda()
+    # (2 - 1 on listed columns, then the count / 16; products and sums of small whole numbers over 16 are exact)
+    listed = torch.where(counts > 0, 1.0 / 0.5 - (1.0 + counts / 16), 1.0).to(dtype)
+    want = scores.clone()
+    want[at.cuda()] = listed[(targets[at].long()).cuda()]
+    kw = dict(targets=targets.cuda(), history=history, repetition=0.5, presence=1.0, frequency=1 / 16)
+    got = dense.adjust_scores(scores, **kw)
+    assert torch.equal(got, want)
+    assert torch.equal(dense.adjust_scores(scores, out=scores, **kw), want)
