@@ -587,3 +587,58 @@ def test_adjust_tiles_of_wide_segments(dtype, cols):
     got = dense.adjust_scores(scores, **kw)
     assert torch.equal(got, want)
     assert torch.equal(dense.adjust_scores(scores, out=scores, **kw), want)
+
+
+# ---- types and strides that only the documentation names ----------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,v,k", [(3, 501, 20), (300, 9001, 130), (2, 120_001, 300)])
+def test_distill_teachers_of_half_precision(dtype, vtype, n, v, k):
+    """A teacher's values in 16 bits: the same as their float32 values, and the formula."""
+    rng = np.random.default_rng(n + k)
+    z = torch.from_numpy(rng.standard_normal((n, v)).astype(np.float32) * 3).to(dtype)
+    cols = torch.from_numpy(np.stack([rng.permutation(v)[:k] for _ in range(n)]))
+    values = torch.from_numpy(rng.standard_normal((n, k)).astype(np.float32) * 2 + 3).to(vtype)
+    counts = torch.from_numpy(rng.integers(0, k + 1, n).astype(np.int32))
+    ref = distill_ref(z, cols, values, counts, 2.0, None, None)
+    loss_b, grad_b = distill_bounds(z, cols, 2.0, ref, None, dtype)
+    dev = (z.cuda(), cols.cuda(), values.cuda(), counts.cuda())
+    loss, grad = dense.distill_loss_grad(*dev, temperature=2.0)
+    check(loss, ref[0], loss_b, "loss")
+    check(grad, ref[2], grad_b, "grad")
+    wide = dense.distill_loss_grad(dev[0], dev[1], dev[2].float(), dev[3], temperature=2.0)
+    assert torch.equal(loss, wide[0]) and torch.equal(grad, wide[1])
+    one, stats = dense.distill_loss(*dev, temperature=2.0, return_stats=True)
+    check(one, ref[0], loss_b, "loss alone")
+    check(dense.distill_grad(dev[0], stats, *dev[1:], temperature=2.0), ref[2], grad_b, "grad alone")
+
+
+@gpu
+def test_strided_lists_and_parameters():
+    """Every second element of a larger tensor, a column of a matrix, a row that stands for all: as their copies."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731
+    i = lambda hi, *s: torch.randint(0, hi, s, generator=gen, device="cuda")  # noqa: E731
+    every = lambda t: torch.stack([t, torch.full_like(t, 77)], -1)[..., 0]  # noqa: E731
+    n, v, k = 5, 70, 6
+    table, ids, ptr, w = r(v, 9), i(v, 40), torch.tensor([0, 3, 3, 20, 31, 40], device="cuda"), r(40)
+    assert torch.equal(dense.embed_rows(table, every(ids), every(ptr), every(w)), dense.embed_rows(table, ids, ptr, w))
+    look = i(v, 4, 6)
+    assert torch.equal(dense.embed_rows(table, look.T), table[look.T])
+    g = r(n, 9)
+    assert torch.equal(dense.embed_rows_grad(g, every(ids), v, every(ptr), every(w)), dense.embed_rows_grad(g, ids, v, ptr, w))
+    z, h = r(n, v), (torch.tensor([0, 2, 9, 9, 12, 15], device="cuda"), i(v, 15))
+    rep, bias, bits = 1 + r(n).abs(), r(v), i(2**31 - 1, n, 3).int()
+    want = dense.adjust_scores(z, targets=torch.arange(n, device="cuda"), history=h, repetition=rep, bias=bias, allowed=bits, filter_cols=h)
+    pair = (every(h[0]), every(h[1]))
+    assert torch.equal(dense.adjust_scores(z, targets=every(torch.arange(n, device="cuda")), history=pair, repetition=every(rep), bias=every(bias),
+                                           allowed=every(bits), filter_cols=pair), want)
+    assert torch.equal(dense.adjust_scores(z, bias=bias.expand(n, v)), dense.adjust_scores(z, bias=bias))
+    cols, values, counts, lse, gl = i(v, n, k), r(n, k), torch.tensor([6, 0, 3, 1, 5], dtype=torch.int32, device="cuda"), r(n) + 4, r(n)
+    want = dense.distill_loss_grad(z, cols, values, counts, grad_loss=gl, teacher_lse=lse)
+    got = dense.distill_loss_grad(z, every(cols), every(values), every(counts), grad_loss=every(gl), teacher_lse=every(lse))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    one = dense.distill_loss_grad(z, cols, values, grad_loss=gl[:1].expand(n))
+    assert torch.equal(one[1], dense.distill_loss_grad(z, cols, values, grad_loss=gl[:1].repeat(n))[1])
