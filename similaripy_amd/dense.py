@@ -149,6 +149,13 @@ def _extent(t):
     return first, first + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
 
 
+def _nothing(t) -> int:
+    """The pointer of an operand that has none: an empty one.  A wrapper tensor has none either; 0 would say that the operand is not given."""
+    if t.numel():
+        raise TypeError(f"an operand has no memory of its own ({type(t).__name__}): pass the tensor that it wraps")
+    return 0
+
+
 def _written(out) -> None:
     """The caller's output has been written behind torch's back: its version goes up, so that a backward pass that has saved it raises."""
     if out is not None:
@@ -230,7 +237,7 @@ def _embed_args(src, out, indices, indptr, data, n_rows, n_vocab, dim, scale, ac
     dev = src.device
     return _abi.SpEmbedArgs(_EMBED_SIZE, 0, dev.index, _DT[src.dtype], _DT[out.dtype], 1 if indices.dtype == torch.int64 else 0, accumulate, scale,
                             n_rows, n_vocab, dim, indices.numel(), _ld(src), _ld(out), src.data_ptr(), indices.data_ptr(),
-                            None if indptr is None else indptr.data_ptr(), None if data is None else data.data_ptr(), out.data_ptr(), _stream(dev))
+                            None if indptr is None else indptr.data_ptr() or _nothing(indptr), None if data is None else data.data_ptr() or _nothing(data), out.data_ptr(), _stream(dev))
 
 
 def _embed_forward(table, indices, indptr, data, scale, out):
@@ -349,7 +356,7 @@ def _pattern(name: str, csr, device, keep):
     if indptr.dim() != 1 or indptr.numel() < 1 or indices.dim() != 1:
         raise ValueError(f"{name}: indptr and indices must have 1 dimension, indptr at least one element")
     keep += (indptr, indices)
-    return _abi.SpCsrPattern(indptr.data_ptr(), indices.data_ptr(), indptr.numel() - 1, indices.numel(), 1 if indices.dtype == torch.int64 else 0)
+    return _abi.SpCsrPattern(indptr.data_ptr() or _nothing(indptr), indices.data_ptr(), indptr.numel() - 1, indices.numel(), 1 if indices.dtype == torch.int64 else 0)
 
 
 def _per_row(name: str, v, device, n, keep):
@@ -359,7 +366,7 @@ def _per_row(name: str, v, device, n, keep):
         _fixed(name, v)
         v = _floats(name, v, device, n) if v.dim() > 0 else v.to(device, torch.float32).expand(n).contiguous()
         keep.append(v)
-        return v.data_ptr(), 0.0
+        return v.data_ptr() or _nothing(v), 0.0
     return None, _number(name, v)
 
 
@@ -397,7 +404,7 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
         if targets.dim() != 1 or targets.numel() != n:
             raise ValueError(f"targets must have {n} elements, got shape {tuple(targets.shape)}")
         keep.append(targets)
-        tptr, t64 = targets.data_ptr(), 1 if targets.dtype == torch.int64 else 0
+        tptr, t64 = targets.data_ptr() or _nothing(targets), 1 if targets.dtype == torch.int64 else 0
     h = _pattern("history", history, device, keep)
     f = _pattern("filter_cols", filter_cols, device, keep)
     t = _pattern("target_cols", target_cols, device, keep)
@@ -416,7 +423,7 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
         if bias.dim() == 1 and not bias.is_contiguous():
             bias = bias.contiguous()
         keep.append(bias)
-        bptr, bdt, ldb = bias.data_ptr(), _DT[bias.dtype], 0 if bias.dim() == 1 else bias.stride(0)
+        bptr, bdt, ldb = bias.data_ptr() or _nothing(bias), _DT[bias.dtype], 0 if bias.dim() == 1 else bias.stride(0)
     aptr, lda = None, 0
     if allowed is not None:
         words = (n_cols + 31) // 32
@@ -424,7 +431,7 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
         if tuple(allowed.shape) not in ((words,), (n, words)):
             raise ValueError(f"allowed must have shape {(words,)} or {(n, words)}, got {tuple(allowed.shape)}")
         keep.append(allowed)
-        aptr, lda = allowed.data_ptr(), 0 if allowed.dim() == 1 else words
+        aptr, lda = allowed.data_ptr() or _nothing(allowed), 0 if allowed.dim() == 1 else words
     res = _out("out", out, (n, n_cols), scores.dtype, device, keep, scores)
     a = _abi.SpAdjustArgs(_ADJUST_SIZE, 0, device.index, _DT[scores.dtype], n, n_cols, _ld(scores), _ld(res), scores.data_ptr(), res.data_ptr(), tptr, t64, bdt,
                           h, f, t, rep, pres, freq, rep_all, pres_all, freq_all, 0, bptr, ldb, aptr, lda, _stream(device))
@@ -466,7 +473,8 @@ def _distill_args(student, cols, values, counts, temperature, teacher_lse):
         raise ValueError(f"temperature must be positive, got {temperature}")
     a = _abi.SpDistillArgs(_DISTILL_SIZE, 0, device.index, _DT[student.dtype], n, n_cols, _ld(student), 0, k, 1 if cols.dtype == torch.int64 else 0,
                            _DT[values.dtype], temperature, student.data_ptr(), cols.data_ptr(), values.data_ptr(),
-                           None if counts is None else counts.data_ptr(), None if teacher_lse is None else teacher_lse.data_ptr())
+                           None if counts is None else counts.data_ptr() or _nothing(counts),
+                           None if teacher_lse is None else teacher_lse.data_ptr() or _nothing(teacher_lse))
     a.stream = _stream(device)
     return a, (cols, values, counts, teacher_lse)
 
@@ -545,7 +553,7 @@ def _grad_outputs(a, student, grad_loss, out, operands):
     if grad_loss is not None:
         grad_loss = _floats("grad_loss", grad_loss, student.device, n)
     grad = _out("out", out, tuple(student.shape), student.dtype, student.device, (grad_loss, *operands), student)
-    a.grad_loss, a.grad, a.ld_grad = None if grad_loss is None else grad_loss.data_ptr(), grad.data_ptr(), _ld(grad)
+    a.grad_loss, a.grad, a.ld_grad = None if grad_loss is None else grad_loss.data_ptr() or _nothing(grad_loss), grad.data_ptr(), _ld(grad)
     return grad, grad_loss
 
 

@@ -642,3 +642,42 @@ def test_strided_lists_and_parameters():
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     one = dense.distill_loss_grad(z, cols, values, grad_loss=gl[:1].expand(n))
     assert torch.equal(one[1], dense.distill_loss_grad(z, cols, values, grad_loss=gl[:1].repeat(n))[1])
+
+
+class Wrapped(torch.Tensor):
+    """A tensor that keeps another one and has no memory of its own, as those of sharded or quantised models."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device, strides=inner.stride())
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        return func(*[a.inner if isinstance(a, Wrapped) else a for a in args], **(kwargs or {}))
+
+
+@gpu
+def test_operands_without_memory():
+    """Their pointer is 0, which says "not given" of an operand that may be left out: refused, as are those that may not."""
+    z, ids, ptr, w = torch.randn(3, 40, device="cuda"), torch.tensor([0, 2, 1], device="cuda"), torch.tensor([0, 1, 3, 3], device="cuda"), torch.ones(3, device="cuda") * 2
+    cols, values, counts = torch.tensor([[0, 1]] * 3, device="cuda"), torch.randn(3, 2, device="cuda"), torch.tensor([1, 2, 0], dtype=torch.int32, device="cuda")
+    bits, row = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.ones(40, device="cuda")
+    W = Wrapped
+    for call in (
+        lambda: dense.embed_rows(z, ids, W(ptr)), lambda: dense.embed_rows(z, ids, ptr, W(w)), lambda: dense.embed_rows(W(z), ids), lambda: dense.embed_rows(z, W(ids)),
+        lambda: dense.embed_rows_grad(z, ids, 3, ptr, W(w)), lambda: dense.embed_rows_grad(z, ids, 3, W(ptr), w), lambda: dense.embed_rows_grad(W(z), ids, 3),
+        lambda: dense.adjust_scores(z, targets=W(ids)), lambda: dense.adjust_scores(z, bias=W(row)), lambda: dense.adjust_scores(z, allowed=W(bits)),
+        lambda: dense.adjust_scores(z, filter_cols=(W(ptr), ids)), lambda: dense.adjust_scores(z, target_cols=(ptr, W(ids))),
+        lambda: dense.adjust_scores(z, history=(ptr, ids), repetition=W(w)), lambda: dense.adjust_scores(z, history=(ptr, ids), presence=W(w)),
+        lambda: dense.adjust_scores(z, history=(ptr, ids), frequency=W(w)), lambda: dense.adjust_scores(W(z)),
+        lambda: dense.distill_loss(z, cols, values, W(counts)), lambda: dense.distill_loss(z, cols, values, teacher_lse=W(w)), lambda: dense.distill_loss(z, W(cols), values),
+        lambda: dense.distill_loss(z, cols, W(values)), lambda: dense.distill_loss_grad(z, cols, values, grad_loss=W(w)), lambda: dense.distill_loss_grad(W(z), cols, values),
+    ):
+        with pytest.raises((TypeError, RuntimeError)):
+            call()
+    none = torch.zeros(0, device="cuda")                # empty operands have no memory either
+    assert dense.adjust_scores(z[:0], history=(ptr, ids), repetition=none, frequency=none).shape == (0, 40)
+    assert (dense.embed_rows(z, ids[:0], torch.zeros(3, dtype=torch.int64, device="cuda"), none) == 0).all()
