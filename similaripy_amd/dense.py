@@ -156,10 +156,8 @@ def _nothing(t) -> int:
     return 0
 
 
-def _written(out) -> None:
-    """The caller's output has been written behind torch's back: its version goes up, so that a backward pass that has saved it raises."""
-    if out is not None:
-        torch.autograd.graph.increment_version(out)
+# the caller's output has been written behind torch's back: its version goes up, so that a backward pass that has saved it raises
+_written = torch.autograd.graph.increment_version
 
 
 def _stream(device) -> int:
@@ -184,7 +182,8 @@ def _fixed(name: str, t) -> None:
 
 
 def _number(name: str, v) -> float:
-    _fixed(name, v)
+    if isinstance(v, torch.Tensor):
+        _fixed(name, v)
     return float(v)
 
 
@@ -193,15 +192,16 @@ def _not_capturing(name: str, instead: str) -> None:
         raise RuntimeError(f"{name} on tensors that require a gradient cannot be captured into a graph: capture {instead} on detached tensors")
 
 
-_is_tracing, _modes, _pre_dispatch = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._ops.mode_stack_state_for_pre_dispatch()
-_PROXY = torch._C._TorchDispatchModeKey.PROXY
+_is_tracing, _modes, _in_keys, _compiling = (torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._dispatch_tls_is_dispatch_key_included,
+                                             torch.compiler.is_dynamo_compiling)
+_PROXY, _PRE_DISPATCH = torch._C._TorchDispatchModeKey.PROXY, torch._C.DispatchKey.PreDispatch
 
 
 def _plain(*operands) -> None:
     """Every entry begins with this.  The kernels read and write memory behind torch's back: a tangent would be dropped (a derivative of 0),
     and a recorded graph (torch.jit.trace, make_fx, torch.export) would hold the allocation of the output and nothing else.  torch.compile breaks
     its graph at these calls and needs no refusal."""
-    if _is_tracing() or (_modes() and torch._C._get_dispatch_mode(_PROXY) is not None) or (_pre_dispatch.count() and torch._ops._get_dispatch_mode_pre_dispatch(_PROXY) is not None):
+    if _is_tracing() or (_modes() and torch._C._get_dispatch_mode(_PROXY) is not None) or (not _compiling() and _in_keys(_PRE_DISPATCH)):
         raise RuntimeError("the dense operators cannot be traced: a recorded graph would not hold their kernels")
     if forward_ad._current_level >= 0:
         for t in operands:
@@ -250,8 +250,10 @@ def _embed_forward(table, indices, indptr, data, scale, out):
     flat = None if out is None else out.view(n_rows, dim) if out.dim() != 2 else out
     res = _out("out", flat, (n_rows, dim), table.dtype, table.device, (table, indices, indptr, data))
     _abi.call_dense("sp_embed_rows", _embed_args(table, res, indices, indptr, data, n_rows, table.shape[0], dim, scale))
-    _written(out)
-    return out if out is not None else res if len(lead) == 1 else res.view(lead + (dim,))
+    if out is not None:
+        _written(out)
+        return out
+    return res if len(lead) == 1 else res.view(lead + (dim,))
 
 
 class _EmbedRows(torch.autograd.Function):
@@ -287,7 +289,8 @@ def embed_rows(table: torch.Tensor, indices: torch.Tensor, indptr: Optional[torc
     """
     _plain(table, data, scale, out)
     _dense("table", table)
-    scale = _number("scale", scale)
+    if type(scale) is not float:
+        scale = _number("scale", scale)
     if data is not None:
         _fixed("data", data)
     if out is None and table.requires_grad and torch.is_grad_enabled():
@@ -336,7 +339,8 @@ def embed_rows_grad(grad: torch.Tensor, indices: torch.Tensor, n_vocab: int, ind
         ws = torch.empty(need, dtype=torch.uint8, device=grad.device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
     _abi.call_dense("sp_embed_rows_grad", a)
-    _written(out)
+    if out is not None:
+        _written(out)
     return res
 
 
@@ -362,12 +366,16 @@ def _pattern(name: str, csr, device, keep):
 def _per_row(name: str, v, device, n, keep):
     """(pointer, value for all rows) of a number or one float32 per row.  A tensor of no dimensions on a device is not read here, which would wait
     for the device: the rows share it."""
-    if isinstance(v, torch.Tensor) and (v.dim() > 0 or v.is_cuda):
+    if not isinstance(v, torch.Tensor):
+        return None, float(v)
+    if v.dim() == 0:
         _fixed(name, v)
-        v = _floats(name, v, device, n) if v.dim() > 0 else v.to(device, torch.float32).expand(n).contiguous()
-        keep.append(v)
-        return v.data_ptr() or _nothing(v), 0.0
-    return None, _number(name, v)
+        if not v.is_cuda:
+            return None, float(v)
+        v = v.to(device, torch.float32).expand(n)
+    v = _floats(name, v, device, n)
+    keep.append(v)
+    return v.data_ptr() or _nothing(v), 0.0
 
 
 def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = None, history: _Pattern = None, repetition: _PerRow = 1.0,
@@ -394,7 +402,8 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
     """
     _plain(scores, repetition, presence, frequency, bias, out)
     _dense("scores", scores)
-    _no_grad_here("adjust_scores", scores)
+    if scores.requires_grad:
+        _no_grad_here("adjust_scores", scores)
     n, n_cols = scores.shape
     device = scores.device
     keep = []
@@ -416,8 +425,9 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
     bptr, bdt, ldb = None, 0, 0
     if bias is not None:
         _dense("bias", bias, 2 if isinstance(bias, torch.Tensor) and bias.dim() == 2 else 1)
-        _same_device("bias", bias, device)
-        _no_grad_here("adjust_scores", bias)
+        if bias.device != device or bias.requires_grad:
+            _same_device("bias", bias, device)
+            _no_grad_here("adjust_scores", bias)
         if tuple(bias.shape) not in ((n_cols,), (n, n_cols)):
             raise ValueError(f"bias must have shape {(n_cols,)} or {(n, n_cols)}, got {tuple(bias.shape)}")
         if bias.dim() == 1 and not bias.is_contiguous():
@@ -436,7 +446,8 @@ def adjust_scores(scores: torch.Tensor, *, targets: Optional[torch.Tensor] = Non
     a = _abi.SpAdjustArgs(_ADJUST_SIZE, 0, device.index, _DT[scores.dtype], n, n_cols, _ld(scores), _ld(res), scores.data_ptr(), res.data_ptr(), tptr, t64, bdt,
                           h, f, t, rep, pres, freq, rep_all, pres_all, freq_all, 0, bptr, ldb, aptr, lda, _stream(device))
     _abi.call_dense("sp_adjust_scores", a)
-    _written(out)
+    if out is not None:
+        _written(out)
     return res
 
 
@@ -537,7 +548,8 @@ def distill_loss(student: torch.Tensor, cols: torch.Tensor, values: torch.Tensor
     """
     _plain(student, values, temperature, teacher_lse)
     _fixed("values", values)
-    _fixed("temperature", temperature)
+    if isinstance(temperature, torch.Tensor):
+        _fixed("temperature", temperature)
     if teacher_lse is not None:
         _fixed("teacher_lse", teacher_lse)
     if isinstance(student, torch.Tensor) and student.requires_grad and torch.is_grad_enabled():
@@ -576,7 +588,8 @@ def distill_grad(student: torch.Tensor, stats: torch.Tensor, cols: torch.Tensor,
     grad, g = _grad_outputs(a, student, grad_loss, out, (stats, *keep))
     a.stats = stats.data_ptr()
     _abi.call_dense("sp_distill_grad", a)
-    _written(out)
+    if out is not None:
+        _written(out)
     del keep, g
     return grad
 
@@ -594,6 +607,7 @@ def distill_loss_grad(student: torch.Tensor, cols: torch.Tensor, values: torch.T
     a.loss = loss.data_ptr()
     ws = _workspace(a, student.device)
     _abi.call_dense("sp_distill_loss_grad", a)
-    _written(out)
+    if out is not None:
+        _written(out)
     del ws, keep, g
     return loss, grad
