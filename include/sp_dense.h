@@ -16,10 +16,14 @@
  * Every pointer is device memory on `device`; every call is asynchronous on `stream`, allocates nothing, leaves the
  * calling thread's current device as it was and may be captured into a graph.  `flags` is 0 (reserved).
  * Same conventions as sp_knn.h: plain pointers and sizes, 0 or a negative SP_E* code, sp_last_error().
- * A launch has fewer than 2^32 threads: calls of more rows than that gives (2^23 of distillation, 2^24 of scores, 2^26
- * of embedding rows of 1 KB and more) are refused with SP_EINVAL and have to be cut by the caller.
- * A launch has fewer than 2^32 threads: calls of more rows than that gives (2^23 of distillation, 2^24 of scores, 2^26
- * of embedding rows of 1 KB and more) are refused with SP_EINVAL and have to be cut by the caller.
+ * A launch has fewer than 2^32 threads.  A call that would need more is refused with SP_EINVAL, before anything is launched,
+ * and has to be cut by the caller.  Threads, with `slabs` = a row's KB rounded up:
+ *   lookup          n_rows * slabs * lanes, the 8, 16, 32 or 64 lanes that cover a row (64: from 513 bytes on) by 16 bytes each
+ *   bags            n_rows * slabs * 64, n_rows rounded up to a multiple of 4, whatever the width
+ *   gradient        256 * slabs for every min(ceil(n_vocab / 512), 2048) ids with up to 1024 entries; for every chunk of the sorted
+ *                   entries, of which there are at most 262144 / lanes, with more
+ *   adjustment      n_rows * 256 * segments, a segment for every 16384 columns (few rows are cut further, up to 2048 segments)
+ *   distillation    (n_rows + 2048) * 512
  * Sums, row statistics and list probabilities are formed in 32 bits or more whatever the type of the tensors.
  */
 #ifndef SP_DENSE_H_
@@ -63,12 +67,14 @@ typedef struct sp_embed_args {
     int64_t      workspace_bytes;
 } sp_embed_args;
 
-/* out[i, :] = scale * sum over the entries j of row i of data[j] * src[indices[j], :], summed in storage order in 32 bits, rounded once */
+/* out[i, :] = scale * sum over the entries j of row i of data[j] * src[indices[j], :], in 32 bits, rounded once.  The order of the additions
+ * depends on the sizes and the row alone (groups of lanes take a row's entries in turn, their sums are added as a tree): equal calls give
+ * equal bits. */
 int sp_embed_rows(const sp_embed_args *args);
 
 /* out[v, :] = scale * sum over the entries j with indices[j] = v of data[j] * src[row of j, :] (+ out[v, :] with accumulate).
- * The entries are sorted by id, stably: the additions of a row happen in an order that depends on the input alone, so equal
- * calls give equal bits. */
+ * The entries are sorted by id, stably, and added in ascending j within a chunk of the sorted entries; the sums of an id that has entries in
+ * several chunks are joined in their order.  No atomics: equal calls give equal bits. */
 int sp_embed_rows_grad(const sp_embed_args *args);
 int64_t sp_embed_rows_grad_workspace_bytes(const sp_embed_args *args);
 

@@ -10,7 +10,8 @@
 // listed several times is counted exactly (integer LDS adds: their order does not matter).
 //
 // Measured: 512 x 100 000 bf16 with a history and a filter of 144 entries and a float32 bias 52 us; 1021 x 84 431 f16 with 1000 target
-// columns, 64 filtered ones and packed bits 86 us.  The same rows without lists and bias move at 5.9 TB/s (34.4 us) and 5.0 TB/s (69 us):
+// columns, 64 filtered ones and packed bits 86 us.  The same rows without lists and bias move at 5.9 TB/s (34.4 us; torch's copy of them takes 36.1) and
+// 5.0 TB/s (69 us):
 // the bias costs 11 us (as many bytes again, from L2), the lists the rest, in registers and in the start of every workgroup.  Long histories are
 // bound by the instructions of listed columns, which a wave executes for its lane with the most of them: 231 us with 4000 entries a row.  Writing the
 // listed columns once more after the stream instead was no faster for 144 entries a row and twice as slow for 1000.

@@ -1,8 +1,10 @@
 // sp_embed_kernels.hpp — rows of a CSR times an embedding table, and the gradient of the table.
 //
 //   out[i, :]  = scale * sum_{j in row i} w_j T[id_j, :]            (a lookup: row i holds entry i alone)
-//   dT[v, :]   = scale * sum_{j: id_j = v} w_j dO[row of j, :]      in ascending j
+//   dT[v, :]   = scale * sum_{j: id_j = v} w_j dO[row of j, :]
 //
+// The order of the additions depends on the sizes and the entries alone: bags take theirs by groups of lanes whose sums are added as a tree,
+// the gradient adds in ascending j within a chunk of the sorted entries and joins the chunks' sums in their order.
 // Both are gathers of whole rows: a group of lanes takes 16 bytes per lane of one row, so that a row is one coalesced access, and
 // requests several rows before it adds the first.  Nothing is added with atomics.
 #pragma once
@@ -62,11 +64,13 @@ template <typename T, typename I, int G, int N> __global__ __launch_bounds__(256
     put<T, N>((T *)p.out + row * p.ld_out + cols.c, v);
 }
 
-// Bags: one wave per row and slab.  What bounds it is the lines of the table that the L2 of an XCD (4 MB) does not hold and the latency of
-// the others: 65 536 bags of 64 out of 100 000 rows of 512 B (Zipf 0.9) read 2.1 GB, half of it past L2, in 184 us.  A large table of wide
-// rows is cut by columns, so that each XCD works on one slab only and holds that many times more rows of it; few rows are cut so that
-// there are waves enough.  (16 384 bags, rows of 2 KB: 245 -> 182 us with eight slabs; 4000 bags, rows of 512 B: 60 -> 27 with four; 65 536
-// bags: 512 B 186 -> 179, 256 B 103 -> 106, a table of 10 MB 142 -> 154, which is why those stay whole.)
+// Bags: one wave per row and slab.  65 536 bags of 64 out of 100 000 rows of 512 B (Zipf 0.9) read 2.1 GB in 186 us, 11 TB/s (in bf16 197; of 256 B,
+// bf16 and fp16, 99 .. 109).  The L2 of an XCD (4 MB) holds 49 % of the lines.  Misses alone do not bound it: cut into four slabs the L2s hold
+// 62 %, which takes a quarter of the misses away, but only 6 % of the time; how much of the rest is the latency of a wave's requests has not been
+// shown.  A large table of wide rows is cut by columns, so that each XCD works on one slab only and holds that many times more rows of it, unless a
+// launch cannot have as many workgroups; few rows are cut so that there are waves enough.  (16 384 bags, rows of 2 KB: 245 -> 182 us with eight slabs;
+// 4000 bags, rows of 512 B: 60 -> 27 with four; 65 536 bags: 512 B 186 -> 179, 256 B 103 -> 106, a table of 10 MB 142 -> 154, which is why those stay
+// whole.)
 // A wave's 64 / G groups take the row's entries in turn; 64 ids and weights are read at once, a lane each, and
 // U rows of the table are on their way per group (an id outside the table reads row 0 and adds nothing).
 template <typename T, typename I, int G, int N> __global__ __launch_bounds__(256) void sp_embed_rows_kernel(EmbedParams p) {

@@ -14,9 +14,10 @@ neighbourhood model's top-k lists, and to be served with the same selectors.
 The compute is hand-written HIP behind include/sp_dense.h; torch is the tensors, the streams and the autograd graph.  Calls are
 asynchronous on torch's current stream of the tensors' device; outputs and workspaces come from torch's allocator, so a call may
 be captured into a graph.  Dense tensors are float32, bfloat16 or float16 with contiguous rows (any distance between rows);
-everything is summed in float32 or wider and rounded once.  There is no CPU fallback.  Rows of one call are limited by what one
-launch can have (2^23 of distillation, 2^24 of scores, 2^26 of wide embedding rows); an output that is given may share memory with
-no operand but where its function says so.
+everything is summed in float32 or wider and rounded once.  There is no CPU fallback.  A call that needs more threads than a launch has
+(2^32) is refused: 2^23 rows of distillation, 2^24 rows of scores by segments of 16 384 columns, 2^26 embedding rows by slabs of 1 KB (include/
+sp_dense.h has the numbers).  An output that is given may share memory with no operand but where its function says so (columns beside
+an input's in one store are not shared); it counts as changed in place for autograd.
 
 Autograd and graph capture: inside a capture the functions that build an autograd graph refuse inputs that require a gradient
 (the backward pass of a captured graph would meet leaves whose gradients belong to another stream): capture the explicit
@@ -306,7 +307,8 @@ def embed_rows_grad(grad: torch.Tensor, indices: torch.Tensor, n_vocab: int, ind
                     out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
     """Gradient of the table of :func:`embed_rows`: ``out[v] = scale * sum(data[j] * grad[row of j] for indices[j] == v)``.
 
-    The entries are sorted by id and added in ascending order in float32: no atomics, equal calls give equal bits.
+    The entries are sorted by id and summed in float32, in ascending order within a chunk of the sorted entries and then chunk by chunk: no
+    atomics, equal calls give equal bits.
 
     grad        [n_rows, dim] gradient of the rows (a lookup's with its leading dimensions flattened or not)
     n_vocab     rows of the table
