@@ -65,7 +65,7 @@ template <typename T, typename I, int G, int N> __global__ __launch_bounds__(256
 }
 
 // Bags: one wave per row and slab.  65 536 bags of 64 out of 100 000 rows of 512 B (Zipf 0.9) read 2.1 GB in 186 us, 11 TB/s (in bf16 197; of 256 B,
-// bf16 and fp16, 99 .. 109).  The L2 of an XCD (4 MB) holds 49 % of the lines.  Misses alone do not bound it: cut into four slabs the L2s hold
+// bf16 and fp16, 99 .. 116).  The L2 of an XCD (4 MB) holds 49 % of the lines.  Misses alone do not bound it: cut into four slabs the L2s hold
 // 62 %, which takes a quarter of the misses away, but only 6 % of the time; how much of the rest is the latency of a wave's requests has not been
 // shown.  A large table of wide rows is cut by columns, so that each XCD works on one slab only and holds that many times more rows of it, unless a
 // launch cannot have as many workgroups; few rows are cut so that there are waves enough.  (16 384 bags, rows of 2 KB: 245 -> 182 us with eight slabs;
